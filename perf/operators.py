@@ -189,8 +189,9 @@ def _halves(case, y):
 
 def _plain_rows(y):
     most = y.abs().amax(dim=1)
-    scales = most / 127
-    q = torch.round(y * torch.where(most > 0, 127 / most, 0)[:, None])
+    top = torch.full_like(most, 127)      # a tensor: a quotient with a number would be a product with a rounded reciprocal
+    scales = most / top
+    q = torch.round(y * torch.where(most > 0, top / most, 0)[:, None])
     return (q * scales[:, None]).to(torch.bfloat16), scales
 
 
