@@ -310,6 +310,20 @@ OI_API int oi_gemm_few(void* out, int out_dtype, long long ldc, const void* x, l
 OI_API int oi_gemm_few_max_k(int M);
 OI_API int oi_gemm_few_status(int* status);
 
+// rows_int8.cu: rows as 8-bit integers with a float32 scale each (q = round(y * (127 / max |y|)), scale = max |y| / 127)
+OI_API int oi_quantize_int8(void* q, long long ldq, float* scales, const void* x, int dtype, long long ldx, int rows, int cols,
+                            void* stream);
+OI_API int oi_rmsnorm_int8(void* q, long long ldq, float* scales, void* x, long long ldx, const void* delta, long long ldd, int dtype,
+                           const void* w, int w_dtype, int rows, int cols, float eps, float w_offset, void* stream);
+OI_API int oi_silu_mul_int8(void* q, long long ldq, float* scales, const void* gate_up, int dtype, long long ldx, int rows, int inter,
+                            int block, int act, void* stream);
+OI_API int oi_dequantize_int8(void* out, int dtype, long long ldo, const void* q, long long ldq, const float* scales, int rows, int cols,
+                              void* stream);
+
+// gemm_int8.cu: out[m, n] = (sum_k x[m, k] w[n, k]) * sx[m] * sw[n] + bias[n], the sums exact in 32-bit integers
+OI_API int oi_linear_int8(void* out, int out_dtype, long long ldo, const void* x, long long ldx, const float* sx, const void* w,
+                          long long ldw, const float* sw, const float* bias, int M, int N, int K, void* stream);
+
 // gemm_tcgen05.cu
 OI_API int oi_gemm_tcgen05(void* C, int c_dtype, long long ldc, const void* A, long long lda, const void* W, long long
        ldw, int M, int N, int K, int tile_n, int act, void* stream);

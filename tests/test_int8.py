@@ -1,0 +1,117 @@
+"""8-bit rows and products: what is refused, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from openinfer_b200.kernels import int8
+from openinfer_b200.kernels import lib as klib
+from openinfer_b200.kernels.lib import KernelError
+
+ROWS = torch.zeros(3, 32, dtype=torch.int8)
+SCALES = torch.ones(3)
+X = torch.zeros(3, 32)
+
+
+def refused(words, call, *args, **kw):
+    with pytest.raises(KernelError, match=words):
+        call(*args, **kw)
+
+
+def test_rows_that_are_not_rows_of_8_bit_integers():
+    def held(values, scales=SCALES):
+        refused(words, int8.dequantize_int8, int8.Int8Rows(values, scales))
+    words = "int8 with float32 scales"
+    held(ROWS.to(torch.uint8))
+    held(ROWS, SCALES.double())
+    words = "at least one integer"
+    held(ROWS[0])
+    held(ROWS[:, :0])
+    held(torch.zeros(32, 3, dtype=torch.int8).t())
+    words = "16-byte borders"
+    held(torch.zeros(3, 33, dtype=torch.int8))
+    held(torch.zeros(3, 48, dtype=torch.int8)[:, 1:33])
+    held(torch.zeros(1, 32, dtype=torch.int8).expand(3, 32))
+    words = "3 scales"
+    held(ROWS, torch.ones(2))
+    held(ROWS, torch.ones(6)[::2])
+    words = "not on a CUDA device"
+    held(ROWS)
+    held(torch.zeros(3, 48, dtype=torch.int8)[:, :33])       # an odd width in rows of 48
+
+
+def test_floating_rows():
+    for call in (int8.quantize_int8, int8.silu_mul_int8, lambda x: int8.rmsnorm_int8(x, torch.ones(32), 1e-6)):
+        refused("float16 is not supported", call, X.half())
+        refused("neighbours next to each other", call, torch.zeros(32, 3).t())
+        refused("neighbours next to each other", call, torch.zeros(32))
+        refused("at least one number", call, X[:, :0])
+        refused("not on a CUDA device", call, X)
+
+
+def test_norm():
+    def norm(x=X, w=torch.ones(32), **kw):
+        int8.rmsnorm_int8(x, w, 1e-6, **kw)
+    refused("weight of 32 numbers", norm, w=torch.ones(31))
+    refused("weight of 32 numbers", norm, w=torch.ones(32).half())
+    refused("weight of 32 numbers", norm, w=torch.ones(64)[::2])
+    refused("must share", norm, delta=X.bfloat16())
+    refused("must share", norm, delta=X[:2])
+    refused("cannot take a sum", norm, x=torch.zeros(1, 32).expand(3, 32), delta=X)
+    both = torch.zeros(4, 32)
+    refused("not overlap", norm, x=both[:3], delta=both[1:])
+    refused("not on a CUDA device", norm, x=both[:2], delta=both[2:])
+    refused("not on a CUDA device", norm, x=X, delta=X)
+
+
+def test_gate():
+    refused("33 numbers", int8.silu_mul_int8, torch.zeros(3, 33))
+    refused("blocks of 5", int8.silu_mul_int8, X, block=5)
+    refused("blocks of 0", int8.silu_mul_int8, X, block=0)
+    refused("has no kernel", int8.silu_mul_int8, X, act="relu")
+
+
+def test_weight_and_product():
+    refused("a scale for each channel", int8.Int8Weight, ROWS, torch.ones(2))
+    refused("a scale for each channel", int8.Int8Weight, ROWS.float(), SCALES)
+    refused("exact in 32 bits", int8.Int8Weight, torch.zeros(1, int8.MAX_WIDTH + 1, dtype=torch.int8), torch.ones(1))
+    refused("exact in 32 bits", int8.Int8Weight, ROWS[:, :0], SCALES)
+    refused("float32 scales", int8.Int8Weight, ROWS, SCALES.bfloat16())
+    w = int8.Int8Weight(torch.ones(5, 33, dtype=torch.int8), torch.ones(10)[::2])     # laid out in rows of 48
+    assert w.values.stride() == (48, 1) and bool((w.values == 1).all()) and w.scales.is_contiguous()
+    kept = int8.Int8Weight(ROWS, SCALES)
+    assert kept.values.data_ptr() == ROWS.data_ptr()
+    rows = int8.Int8Rows(ROWS, SCALES)
+    refused("rows of 32 on cpu and a weight of 5 x 33", int8.linear_int8, rows, w)
+    refused("3 float32 numbers of bias", int8.linear_int8, rows, kept, bias=torch.ones(3).bfloat16())
+    refused("3 float32 numbers of bias", int8.linear_int8, rows, kept, bias=torch.ones(4))
+    refused("float16 is not supported", int8.linear_int8, rows, kept, out_dtype=torch.float16)
+    refused(r"results \[3, 3\]", int8.linear_int8, rows, kept, out=torch.empty(3, 4))
+    refused("must not overlap", int8.linear_int8, rows, kept, out=torch.empty(3, 3).t())
+    refused("must not overlap", int8.linear_int8, rows, kept, out=torch.empty(1, 3).expand(3, 3))
+    refused("not on a CUDA device", int8.linear_int8, rows, kept)
+
+
+@pytest.mark.parametrize("name,args", [
+    ("oi_quantize_int8", (1, 32, 1, 1, 7, 32, 1, 32)),                     # an unknown dtype
+    ("oi_quantize_int8", (1, 32, 1, 1, 0, 32, -1, 32)),
+    ("oi_quantize_int8", (1, 32, 1, 1, 0, 32, 1, 0)),
+    ("oi_quantize_int8", (0, 32, 1, 1, 0, 32, 1, 32)),
+    ("oi_quantize_int8", (1, 16, 1, 1, 0, 32, 2, 32)),                     # rows that overlap
+    ("oi_rmsnorm_int8", (1, 32, 1, 1, 16, 1, 32, 0, 1, 0, 2, 32, 1e-6, 0.0)),
+    ("oi_rmsnorm_int8", (1, 32, 1, 1, 32, 0, 0, 0, 1, 5, 2, 32, 1e-6, 0.0)),
+    ("oi_silu_mul_int8", (1, 32, 1, 1, 0, 64, 1, 32, 5, 1)),
+    ("oi_silu_mul_int8", (1, 32, 1, 1, 0, 64, 1, 32, 32, 9)),
+    ("oi_dequantize_int8", (1, 5, 32, 1, 32, 1, 1, 32)),
+    ("oi_dequantize_int8", (1, 0, 16, 1, 32, 1, 2, 32)),
+    ("oi_linear_int8", (16, 1, 8, 16, 32, 16, 16, 32, 16, 0, 4, 8, 131072)),   # a sum that 32 bits may not hold
+    ("oi_linear_int8", (16, 1, 8, 8, 32, 16, 16, 32, 16, 0, 4, 8, 32)),        # off the 16-byte border
+    ("oi_linear_int8", (16, 1, 8, 16, 33, 16, 16, 32, 16, 0, 4, 8, 32)),
+    ("oi_linear_int8", (16, 1, 8, 16, 32, 16, 16, 16, 16, 0, 4, 8, 32)),
+    ("oi_linear_int8", (16, 1, 4, 16, 32, 16, 16, 32, 16, 0, 4, 8, 32)),       # result rows that overlap
+    ("oi_linear_int8", (16, 6, 8, 16, 32, 16, 16, 32, 16, 0, 4, 8, 32)),
+])
+def test_the_library_refuses_before_it_launches(name, args):
+    L = klib.load(verbose=False)
+    assert getattr(L, name)(*args, None) == 1
+    assert name[3:].encode() in L.oi_last_error()

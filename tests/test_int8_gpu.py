@@ -1,0 +1,412 @@
+"""8-bit rows and their products on the GPU against plain statements in 64 bits and in exact integers.
+
+What is tested bit for bit: products (their sums are whole numbers, and float32(sum) * sx * sw + bias is three float32
+operations in a stated order), the rows of ``quantize_int8`` and ``dequantize_int8`` (likewise). Norms and gates are held to
+bounds that follow from their roundings.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+U = 2.0 ** -24                  # half a step of float32, relative
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def int8():
+    from openinfer_b200.kernels import int8, lib
+    lib.load()
+    return int8
+
+
+def randn(*shape, seed=0, scale=1.0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed + 1000 * sum(shape))
+    return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+def strided(t, pad, dtype=None):
+    """The same numbers on the device in rows that lie further apart, the room between them filled with what must not be read."""
+    t = t if dtype is None else t.to(dtype)
+    wide = torch.full((t.shape[0], t.shape[1] + pad), float("nan") if t.is_floating_point() else 99, dtype=t.dtype, device=DEV)
+    wide[:, :t.shape[1]] = t.to(DEV)
+    return wide[:, :t.shape[1]]
+
+
+def held_exactly(y):
+    """What the definition says of float32 rows, in float32 operations: q = round(y * (127 / m)), scale = m / 127."""
+    m = y.abs().amax(dim=1)
+    top = torch.full_like(m, 127)            # a tensor: torch takes 127 / m as 127 times a rounded reciprocal
+    q = torch.round(y * torch.where(m > 0, top / m, torch.zeros(()))[:, None])
+    return q.to(torch.int8), m / top
+
+
+def check_held(rows, y, err):
+    """``rows`` against numbers y in 64 bits, of which the kernel's differ by at most ``err`` (relative, per element): the scale is
+    off by the largest number's error and one rounding; q lies within half of y / scale and what the errors of y and of the two
+    float32 roundings of y * (127 / m) add."""
+    q, s = rows.values.cpu().double(), rows.scales.cpu().double()
+    m = y.abs().amax(dim=1)
+    worst = (err * y.abs() / m[:, None]).amax(dim=1) + 2 * U       # of m, relative
+    assert ((s - m / 127).abs() <= (worst + U) * m / 127).all()
+    room = 0.5 + (y.abs() * 127 / m[:, None]) * (err + worst[:, None] + 3 * U)
+    off = (q - y * (127 / m)[:, None]).abs()
+    assert (off <= room).all(), (off - room).max()
+    assert int(q.abs().max()) <= 127
+
+
+# ------------------------------------------------------------------------------------------------------------ plain rows
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,width", [(1, 1), (3, 7), (5, 64), (2, 100), (7, 1000), (1, 4096), (130, 257), (3, 5001), (2, 12288), (1, 40000), (2, 70001)])
+def test_rows(int8, dtype, rows, width):
+    x = randn(rows, width, scale=3.0).to(dtype)
+    q, s = held_exactly(x.float())
+    for at in (x.to(DEV), strided(x, 3), strided(x, 8)):
+        held = int8.quantize_int8(at)
+        assert torch.equal(held.values.cpu(), q) and torch.equal(held.scales.cpu(), s)
+        assert held.values.data_ptr() % 16 == 0 and (rows == 1 or held.values.stride(0) % 16 == 0)
+    for to in DTYPES:
+        assert torch.equal(int8.dequantize_int8(held, to).cpu(), (q.float() * s[:, None]).to(to))
+    out = strided(torch.zeros(rows, width), 5)
+    int8.dequantize_int8(held, out=out)
+    assert torch.equal(out.cpu(), q.float() * s[:, None])
+    if rows > 1:
+        assert bool(torch.isnan(out.as_strided((rows - 1, 5), out.stride(), out.storage_offset() + width)).all())   # the room between rows
+
+
+@pytest.mark.parametrize("width", [33, 64, 512, 4096, 40000])
+def test_rows_of_extreme_numbers(int8, width):
+    big, small, sub = 3.0e38, 2.0e-36, 1.0e-41
+    x = randn(9, width)
+    x[0] = 0.0
+    x[1, -1] = float("inf")
+    x[2, width // 2] = float("nan")
+    x[3, 0], x[3, 1] = float("-inf"), float("nan")
+    x[4] *= big / x[4].abs().max()
+    x[5] *= small / x[5].abs().max()
+    x[6] = 0.0
+    x[6, 3] = -sub                       # below the normal numbers: 127 / m alone would be infinite
+    x[7, 5] = -0.0
+    held = int8.quantize_int8(x.to(DEV))
+    q, s = held.values.cpu(), held.scales.cpu()
+    assert not q[0].any() and s[0] == 0
+    for r in (1, 2, 3):
+        assert not q[r].any() and torch.isnan(s[r])
+    ref_q, ref_s = held_exactly(x)
+    for r in (4, 7, 8):                  # a row beside one that is not finite is what it is alone
+        assert torch.equal(q[r], ref_q[r]) and torch.equal(s[r], ref_s[r])
+    # row 5 is multiplied by a power of two first, which changes no rounding; its scale is normal
+    assert torch.equal(q[5], held_exactly((x[5:6].double() * 2.0 ** 80).float())[0][0]) and abs(float(s[5]) * 127 / small - 1) < 4 * U
+    # row 6: the integer is exact, the scale a subnormal number, off by half a step of those (2^-150) and the roundings
+    assert q[6, 3] == -127 and int(q[6].abs().sum()) == 127
+    assert abs(float(s[6]) - float(x[6, 3].abs()) / 127) <= 2.0 ** -149
+    back = int8.dequantize_int8(held, torch.float32).cpu()
+    assert torch.isnan(back[1:4]).all() and not torch.isnan(back[[0, 4, 5, 6, 7, 8]]).any()
+
+
+# ------------------------------------------------------------------------------------------------------------ norms
+def norm_error(width):
+    """Relative error of a norm's output in float32: squares added by at least 32 threads in turn and then in a tree (at most
+    width / 32 + 20 roundings, halved by the root), the root's 2 units, three products, an addition."""
+    return ((width / 32 + 20) / 2 + 12) * U
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("w_dtype", DTYPES)
+@pytest.mark.parametrize("rows,width", [(1, 1), (4, 24), (3, 100), (9, 512), (2, 1000), (1, 4096), (5, 4104), (130, 768), (3, 5001), (1, 16384), (2, 33000)])
+def test_norm(int8, dtype, w_dtype, rows, width):
+    x, d = (randn(rows, width, seed=s, scale=3.0).to(dtype) for s in (1, 2))
+    w = (1 + 0.1 * randn(width, seed=3)).to(w_dtype)
+
+    def ref(v, offset):
+        v = v.double()
+        return v / torch.sqrt(v.pow(2).mean(dim=1, keepdim=True) + 1e-5) * (offset + w.double())
+    for pad in (0, 3, 8):
+        at, dt = strided(x, pad), strided(d, pad)
+        held = int8.rmsnorm_int8(at, w.to(DEV), 1e-5)
+        check_held(held, ref(x, 0.0), norm_error(width))
+        assert torch.equal(at.cpu(), x)
+        held = int8.rmsnorm_int8(at, w.to(DEV), 1e-5, delta=dt, weight_offset=1.0)
+        total = (x.float() + d.float()).to(dtype)
+        assert torch.equal(at.cpu(), total) and torch.equal(dt.cpu(), d)           # the sum is stored, rounded once
+        check_held(held, ref(total, 1.0), norm_error(width))
+        if pad and rows > 1:                                                       # and nothing behind a row
+            assert bool(torch.isnan(at.as_strided((rows, pad), at.stride(), at.storage_offset() + width)).all())
+
+
+def test_norm_of_rows_that_are_zero_or_not_finite(int8):
+    for width in (40, 4096, 40000):
+        x = randn(4, width, dtype=torch.bfloat16)
+        x[0] = 0
+        x[1, 7] = float("inf")
+        x[2, 0] = float("nan")
+        held = int8.rmsnorm_int8(x.to(DEV), torch.ones(width, device=DEV), 1e-6)
+        alone = int8.rmsnorm_int8(x[3:].to(DEV), torch.ones(width, device=DEV), 1e-6)
+        s = held.scales.cpu()
+        assert s[0] == 0 and torch.isnan(s[1:3]).all() and not held.values[:3].any()
+        assert torch.equal(held.values[3:], alone.values) and torch.equal(held.scales[3:], alone.scales)
+
+
+def test_norm_takes_itself_as_the_residual_and_one_row_for_all(int8):
+    x, one, w = randn(6, 256).to(DEV), randn(1, 256, seed=4).to(DEV), torch.ones(256, device=DEV)
+    a, b = x.clone(), x.clone()
+    held = int8.rmsnorm_int8(a, w, 1e-6, delta=a)
+    assert torch.equal(a, x + x)
+    check_held(held, (a.cpu().double() / a.cpu().double().pow(2).mean(dim=1, keepdim=True).add(1e-6).sqrt()), norm_error(256))
+    int8.rmsnorm_int8(b, w, 1e-6, delta=one.expand(6, 256))
+    assert torch.equal(b, x + one)
+
+
+@pytest.mark.parametrize("width", [64, 256, 1024, 4096, 5001])
+def test_a_row_does_not_depend_on_the_rows_around_it(int8, width):
+    x = randn(3000, width, dtype=torch.bfloat16).to(DEV)
+    w = (1 + 0.1 * randn(width, seed=5)).to(DEV)
+    whole = int8.rmsnorm_int8(x, w, 1e-6)
+    gates = int8.silu_mul_int8(x[:, :width // 2 * 2])
+    for r in (0, 1777, 2999):
+        one = int8.rmsnorm_int8(x[r:r + 1], w, 1e-6)
+        assert torch.equal(one.values[0], whole.values[r]) and torch.equal(one.scales[0], whole.scales[r])
+        one = int8.silu_mul_int8(x[r:r + 1, :width // 2 * 2])
+        assert torch.equal(one.values[0], gates.values[r]) and torch.equal(one.scales[0], gates.scales[r])
+
+
+# ------------------------------------------------------------------------------------------------------------ gates
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("rows,inter,block", [(1, 1, 1), (3, 5, 5), (4, 64, 64), (2, 96, 32), (5, 1000, 8), (3, 1000, 4), (1, 12288, 64), (130, 640, 640), (2, 12288, 12288),
+                                              (1, 36000, 36000), (1, 36000, 16), (2, 5001, 5001)])
+def test_gate(int8, dtype, act, rows, inter, block):
+    gu = randn(rows, 2 * inter, scale=4.0).to(dtype)
+    pairs = gu.double().view(rows, inter // block, 2, block)
+    g, u = pairs[:, :, 0].reshape(rows, inter), pairs[:, :, 1].reshape(rows, inter)
+    t = 2 * (2 / torch.pi) ** 0.5 * (g + 0.044715 * g ** 3) if act == "gelu_tanh" else g
+    y = g * torch.sigmoid(t) * u
+    # t is off by at most 8 roundings; e^-t by that times |t|, and 2 units of its own; then a sum, a quotient, a product
+    err = (8 * t.abs() + 8) * U
+    for pad in (0, 3, 8):
+        check_held(int8.silu_mul_int8(strided(gu, pad), block=block, act=act), y, err)
+
+
+def test_gates_that_are_far_out_and_not_finite(int8):
+    g = torch.tensor([[-200.0, 200.0, 0.0, -88.8, 89.0, 1.0, -1e30, 1.0], [float("inf"), 1, 1, 1, 1, 1, 1, 1], [1, 1, float("nan"), 1, 1, 1, 1, 1]])
+    u = torch.ones(3, 8)
+    u[0, 7] = -3.0
+    held = int8.silu_mul_int8(torch.cat([g, u], dim=1).to(DEV))
+    y = g[:1].double() * torch.sigmoid(g[:1].double()) * u[:1].double()
+    check_held(int8.Int8Rows(held.values[:1], held.scales[:1]), y, (8 * g[:1].double().abs().clamp(max=200) + 8) * U)
+    assert torch.isnan(held.scales[1:].cpu()).all() and not held.values[1:].any()
+
+
+# ------------------------------------------------------------------------------------------------------------ products
+def product_exactly(x, sx, w, sw, bias, dtype):
+    total = (x.cuda().double() @ w.cuda().double().t()).cpu()          # whole numbers below 2^53: exact in any order
+    y = total.to(torch.int64).float() * sx[:, None] * sw
+    return (y if bias is None else y + bias).to(dtype)
+
+
+def integers(rows, width, seed):
+    g = torch.Generator().manual_seed(seed + rows + 7 * width)
+    return torch.randint(-128, 128, (rows, width), generator=g, dtype=torch.int8), torch.rand(rows, generator=g) * 0.02 + 1e-4
+
+
+def on_device(int8, x, sx):
+    held = int8.empty_rows(*x.shape, DEV)
+    room = -(-x.shape[1] // 16) * 16
+    held.values.as_strided((x.shape[0], room), (room, 1)).fill_(77)      # what lies behind an odd width must not count
+    held.values.copy_(x)
+    held.scales.copy_(sx)
+    return held
+
+
+# rows on both sides of every size at which another tile is taken; sums that fill a stage, miss it by one, and leave slices empty
+SHAPES = [(1, 1, 1), (1, 128, 128), (1, 5, 16), (2, 33, 31), (3, 130, 129), (8, 256, 127), (15, 1000, 64), (16, 128, 4096), (17, 256, 500), (31, 300, 1024), (32, 1536, 4096),
+          (33, 257, 2048), (48, 640, 1000), (64, 1024, 4096), (65, 384, 96), (100, 4096, 777), (127, 129, 8192), (128, 1024, 1024), (129, 999, 2048), (200, 128, 300),
+          (256, 512, 512), (257, 2049, 333), (300, 6144, 256), (512, 513, 1025), (777, 1000, 2001), (1024, 2048, 640), (2050, 300, 4100), (5000, 130, 72), (1, 9000, 14000), (4, 64, 60000)]
+
+
+@pytest.mark.parametrize("rows,channels,width", SHAPES)
+def test_product(int8, rows, channels, width):
+    (x, sx), (w, sw) = integers(rows, width, 1), integers(channels, width, 2)
+    bias = randn(channels, seed=3)
+    held, weight = on_device(int8, x, sx), int8.Int8Weight(w.to(DEV), sw.to(DEV))
+    for dtype in DTYPES:
+        assert torch.equal(int8.linear_int8(held, weight, out_dtype=dtype).cpu(), product_exactly(x, sx, w, sw, None, dtype))
+    want = product_exactly(x, sx, w, sw, bias, torch.bfloat16)
+    assert torch.equal(int8.linear_int8(held, weight, bias=bias.to(DEV)).cpu(), want)
+    for pad in (1, 8):                                    # result rows further apart, on and off 16-byte borders; nothing behind them
+        for dtype in DTYPES:
+            out = torch.full((rows, channels + pad), -7.0, dtype=dtype, device=DEV)
+            int8.linear_int8(held, weight, bias=bias.to(DEV), out=out[:, :channels])
+            assert torch.equal(out[:, :channels].cpu(), product_exactly(x, sx, w, sw, bias, dtype)) and bool((out[:, channels:] == -7.0).all())
+
+
+def test_the_longest_and_largest_sums(int8):
+    """131071 products of -128 and -128: the largest sum there is, one step below 2^31."""
+    width = int8.MAX_WIDTH
+    for rows in (1, 40):
+        x = torch.full((rows, width), -128, dtype=torch.int8)
+        w = torch.full((3, width), -128, dtype=torch.int8)
+        w[1] = 127
+        held, weight = on_device(int8, x, torch.ones(rows)), int8.Int8Weight(w.to(DEV), torch.ones(3, device=DEV))
+        got = int8.linear_int8(held, weight, out_dtype=torch.float32).cpu()
+        want = torch.tensor([128 * 128 * width, -128 * 127 * width, 128 * 128 * width], dtype=torch.int64).float()
+        assert torch.equal(got, want.expand(rows, 3))
+
+
+@pytest.mark.parametrize("rows", [2, 40, 300])
+def test_scales_that_are_zero_or_not_finite_stay_in_their_row_and_channel(int8, rows):
+    (x, sx), (w, sw) = integers(rows, 256, 5), integers(200, 256, 6)
+    sx[0], sx[1] = 0.0, float("nan")
+    sw[3], sw[150] = float("inf"), 0.0
+    got = int8.linear_int8(on_device(int8, x, sx), int8.Int8Weight(w.to(DEV), sw.to(DEV)), out_dtype=torch.float32).cpu()
+    want = product_exactly(x, sx, w, sw, None, torch.float32)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.nan_to_num(got, nan=1.0), torch.nan_to_num(want, nan=1.0))
+
+
+def test_no_rows_and_no_channels(int8):
+    weight = int8.Int8Weight(torch.ones(5, 32, dtype=torch.int8, device=DEV), torch.ones(5, device=DEV))
+    none = int8.quantize_int8(torch.empty(0, 32, device=DEV))
+    assert none.values.shape == (0, 32) and none.scales.shape == (0,)
+    assert int8.linear_int8(none, weight).shape == (0, 5)
+    assert int8.dequantize_int8(none).shape == (0, 32)
+    assert int8.silu_mul_int8(torch.empty(0, 32, device=DEV)).values.shape == (0, 16)
+    assert int8.rmsnorm_int8(torch.empty(0, 32, device=DEV), torch.ones(32, device=DEV), 1e-6).values.shape == (0, 32)
+    empty = int8.Int8Weight(torch.ones(0, 32, dtype=torch.int8, device=DEV), torch.ones(0, device=DEV))
+    assert int8.linear_int8(int8.quantize_int8(torch.ones(3, 32, device=DEV)), empty).shape == (3, 0)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 70, 700])
+def test_one_tensor_as_rows_and_as_weight(int8, rows):
+    """Rows that the kernel just ahead wrote may be a weight: the product waits for them."""
+    x = randn(rows, 512, dtype=torch.bfloat16).to(DEV)
+    for _ in range(20):
+        held = int8.quantize_int8(x)
+        got = int8.linear_int8(held, int8.Int8Weight(*held), out_dtype=torch.float32)
+        q, s = held_exactly(x.float().cpu())
+        assert torch.equal(got.cpu(), product_exactly(q, s, q, s, None, torch.float32))
+        x = x.roll(1, dims=0) * 1.5 if rows > 1 else -x * 1.5
+
+
+# ------------------------------------------------------------------------------------------------------------ together
+def layer(int8, h, branch, norm_w, gate_up, down, block):
+    """A feed-forward layer as a model runs it: norm of the sum, gate and up, activation, down."""
+    rows = int8.rmsnorm_int8(h, norm_w, 1e-6, delta=branch)
+    gu = int8.linear_int8(rows, gate_up)
+    act = int8.silu_mul_int8(gu, block=block)
+    return rows, gu, act, int8.linear_int8(act, down)
+
+
+@pytest.mark.parametrize("tokens", [1, 7, 40, 150, 600])
+def test_a_feed_forward_layer(int8, tokens):
+    width, inter, block = 512, 1536, 64
+    h, branch = (randn(tokens, width, seed=s, dtype=torch.bfloat16) for s in (1, 2))
+    norm_w = (1 + 0.1 * randn(width, seed=3)).bfloat16()
+    wgu, wd = randn(2 * inter, width, seed=4, scale=width ** -0.5), randn(width, inter, seed=5, scale=inter ** -0.5)
+    gate_up, down = int8.Int8Weight.quantize(wgu.to(DEV)), int8.Int8Weight.quantize(wd.to(DEV))
+    on = h.to(DEV)
+    rows, gu, act, out = layer(int8, on, branch.to(DEV), norm_w.to(DEV), gate_up, down, block)
+    # each link from what the one before it gave: products bit for bit, norm and gate within their bounds
+    total = (h.float() + branch.float()).bfloat16()
+    assert torch.equal(on.cpu(), total)
+    v = total.double()
+    y = v / torch.sqrt(v.pow(2).mean(dim=1, keepdim=True) + 1e-6) * norm_w.double()
+    check_held(rows, y, norm_error(width))
+    assert torch.equal(gu.cpu(), product_exactly(rows.values.cpu(), rows.scales.cpu(), *held_exactly(wgu), None, torch.bfloat16))
+    pairs = gu.cpu().double().view(tokens, inter // block, 2, block)
+    g, u = pairs[:, :, 0].reshape(tokens, inter), pairs[:, :, 1].reshape(tokens, inter)
+    check_held(act, g * torch.sigmoid(g) * u, (8 * g.abs() + 8) * U)
+    assert torch.equal(out.cpu(), product_exactly(act.values.cpu(), act.scales.cpu(), *held_exactly(wd), None, torch.bfloat16))
+    # and the whole against the layer without 8-bit integers. Rounding to steps of m / 127 is noise of m / 127 / sqrt(12) in each
+    # operand: 0.0023 m of a root mean square of m / 4 (normal numbers, widths near 500) or m / 8 (activations: products of two
+    # such) is 0.9 % and 1.8 %; weights 0.9 %. First product sqrt(2) * 0.9 = 1.3 %; the activation passes on the gate's and the up's
+    # share, about 1.3 * sqrt(2) = 1.8 %; with its own 1.8 % and the weights' 0.9 %: 2.7 %. Twice that is never reached.
+    full = y @ wgu.double().t()
+    pairs = full.view(tokens, inter // block, 2, block)
+    g, u = pairs[:, :, 0].reshape(tokens, inter), pairs[:, :, 1].reshape(tokens, inter)
+    full = (g * torch.sigmoid(g) * u) @ wd.double().t()
+    assert float((out.cpu().double() - full).norm() / full.norm()) < 0.054
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 300])
+def test_a_layer_in_a_recorded_graph_and_on_another_stream(int8, tokens):
+    width, inter = 256, 768
+    norm_w = torch.ones(width, device=DEV)
+    gate_up = int8.Int8Weight.quantize(randn(2 * inter, width, seed=4).to(DEV))
+    down = int8.Int8Weight.quantize(randn(width, inter, seed=5).to(DEV))
+    h, branch = (torch.zeros(tokens, width, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+
+    def fill(seed):
+        h.copy_(randn(tokens, width, seed=seed))
+        branch.copy_(randn(tokens, width, seed=seed + 50))
+
+    def eager(seed):
+        fill(seed)
+        return layer(int8, h, branch, norm_w, gate_up, down, 64)[3].clone(), h.clone()
+    want = [eager(s) for s in range(4)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for s in range(4):
+            got = eager(s)
+            assert torch.equal(got[0], want[s][0]) and torch.equal(got[1], want[s][1])
+    torch.cuda.current_stream().wait_stream(side)
+    fill(0)
+    graphs = []
+    for _ in range(2):                          # two graphs of the same layer, replayed in turn, eager calls between them
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = layer(int8, h, branch, norm_w, gate_up, down, 64)[3]
+        graphs.append((g, out))
+    for s in (3, 1, 2, 0, 3):
+        fill(s)
+        graphs[s % 2][0].replay()
+        assert torch.equal(graphs[s % 2][1], want[s][0]) and torch.equal(h, want[s][1])
+        assert torch.equal(eager(s)[0], want[s][0])
+
+
+def test_two_streams_at_once(int8):
+    width = 1024
+    weight = int8.Int8Weight.quantize(randn(2048, width, seed=1).to(DEV))
+    xs = [randn(r, width, seed=r, dtype=torch.bfloat16).to(DEV) for r in (5, 90, 400)]
+    want = [int8.linear_int8(int8.quantize_int8(x), weight) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[] for _ in xs]
+    for _ in range(10):
+        for i, (x, s) in enumerate(zip(xs, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(int8.linear_int8(int8.quantize_int8(x), weight))
+    torch.cuda.synchronize()
+    for w, several in zip(want, got):
+        assert all(torch.equal(w, g) for g in several)
+
+
+def test_results_that_lie_beyond_2_to_the_31(int8):
+    """70,000 rows of 32,768 results: the last ones begin 2.3e9 numbers behind the first."""
+    rows, channels = 70000, 32768
+    (x, sx), (w, sw) = integers(rows, 32, 1), integers(channels, 32, 2)
+    out = int8.linear_int8(on_device(int8, x, sx), int8.Int8Weight(w.to(DEV), sw.to(DEV)))
+    for at in (0, 65535, 69990):
+        assert torch.equal(out[at:at + 10].cpu(), product_exactly(x[at:at + 10], sx[at:at + 10], w, sw, None, torch.bfloat16))
+    held = int8.quantize_int8(out)
+    ref = held_exactly(out[-5:].float().cpu())
+    assert torch.equal(held.values[-5:].cpu(), ref[0]) and torch.equal(held.scales[-5:].cpu(), ref[1])
+    back = int8.dequantize_int8(held, out=out)
+    assert torch.equal(back[-5:].cpu(), (ref[0].float() * ref[1][:, None]).bfloat16())
+
+
+def test_refusals_on_the_device(int8):
+    from openinfer_b200.kernels.lib import KernelError
+    weight = int8.Int8Weight(torch.ones(5, 32, dtype=torch.int8, device=DEV), torch.ones(5, device=DEV))
+    held = int8.quantize_int8(torch.ones(3, 32, device=DEV))
+    for bad in (lambda: int8.linear_int8(held, int8.Int8Weight(torch.ones(5, 32, dtype=torch.int8), torch.ones(5))),
+                lambda: int8.linear_int8(held, weight, bias=torch.ones(5)),
+                lambda: int8.linear_int8(held, weight, out=torch.empty(3, 5)),
+                lambda: int8.linear_int8(int8.Int8Rows(held.values, held.scales.cpu()), weight),
+                lambda: int8.rmsnorm_int8(torch.ones(3, 32, device=DEV), torch.ones(32), 1e-6),
+                lambda: int8.rmsnorm_int8(torch.ones(3, 32, device=DEV), torch.ones(32, device=DEV), 1e-6, delta=torch.ones(3, 32)),
+                lambda: int8.quantize_int8(torch.ones(3, 32, device=DEV), out=int8.empty_rows(3, 31, DEV)),
+                lambda: int8.silu_mul_int8(torch.ones(3, 32, device=DEV), out=int8.empty_rows(3, 32, DEV))):
+        with pytest.raises(KernelError):
+            bad()
