@@ -238,6 +238,27 @@ __device__ __forceinline__ unsigned long long desc_mn_major_sw128(unsigned smem_
   d |= (unsigned long long)2 << 61;
   return d;
 }
+// The same products of 8-bit integers (K = 32 an instruction), summed exactly in 32-bit integers.
+__device__ __forceinline__ void umma_i8(unsigned tmem_c, unsigned long long desc_a, unsigned long long desc_b, unsigned idesc,
+                                        unsigned accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+      ::"r"(tmem_c), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(unsigned tmem_c, unsigned long long desc_a, unsigned long long desc_b, unsigned idesc,
+                                             unsigned accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+      ::"r"(tmem_c), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Instruction descriptor of kind::i8 with signed 8-bit A and B (both K-major), 32-bit integer D, shape M x N.
+__host__ __device__ constexpr unsigned idesc_i8_s32(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
+}
 // Instruction descriptor of kind::f16 with bfloat16 A and B (both K-major), float32 D, shape M x N.
 __host__ __device__ constexpr unsigned idesc_bf16_f32(int m, int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
@@ -269,6 +290,18 @@ inline int make_map_2d_bf16(CUtensorMap* map, const void* base, long long rows, 
   return (int)fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+// rows x K 8-bit matrix with row stride ld (bytes, a multiple of 16); boxes of box_rows x 128 bytes, 128-byte swizzle, zeros
+// outside the matrix (K need not be a multiple of anything).
+inline int make_map_2d_i8(CUtensorMap* map, const void* base, long long rows, long long K, long long ld, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return (int)fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 }  // namespace tc

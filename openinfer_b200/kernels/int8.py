@@ -94,6 +94,12 @@ def _on(device: torch.device):
 _HERE = nullcontext()
 
 
+def _done(L, out: Optional[Int8Rows]) -> None:
+    """Rows written into given memory may be those of a weight, which products fetch ahead: the next launch starts behind this one."""
+    if out is not None:
+        L.oi_launch_fence()
+
+
 def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
     """The rows of ``x`` [rows, width] (float32 or bfloat16, row stride free) as 8-bit integers."""
     code = _float_rows(x, "quantize_int8")
@@ -105,6 +111,7 @@ def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
             L = _lib.load()
             _lib.check(L.oi_quantize_int8(held.values.data_ptr(), _stride(held.values), held.scales.data_ptr(), x.data_ptr(), code,
                                           x.stride(0), rows, width, _lib.current_stream()), "quantize_int8")
+            _done(L, out)
     return held
 
 
@@ -135,6 +142,7 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, delta: Op
                                          0 if delta is None else delta.data_ptr(), 0 if delta is None else delta.stride(0), code,
                                          weight.data_ptr(), w_code, rows, width, float(eps), float(weight_offset),
                                          _lib.current_stream()), "rmsnorm_int8")
+            _done(L, out)
     return held
 
 
@@ -155,6 +163,7 @@ def silu_mul_int8(gate_up: torch.Tensor, block: Optional[int] = None, act: str =
             L = _lib.load()
             _lib.check(L.oi_silu_mul_int8(held.values.data_ptr(), _stride(held.values), held.scales.data_ptr(), gate_up.data_ptr(), code,
                                           gate_up.stride(0), rows, inter, block, act_c, _lib.current_stream()), "silu_mul_int8")
+            _done(L, out)
     return held
 
 
@@ -180,11 +189,11 @@ def dequantize_int8(rows: Int8Rows, dtype: torch.dtype = torch.bfloat16, out: Op
 class Int8Weight:
     """A weight [channels, width] for ``linear_int8``: int8 values with a float32 scale for each output channel, laid out once.
 
-    Values whose rows do not start on 16-byte borders are copied into rows that do; others are kept as they are. A product may
-    fetch the weight while the kernel ahead of it on the stream still runs: its contents are not changed by this package's
-    kernels once the object exists (a later copy by torch into its tensors is fine)."""
+    Values whose rows do not start on 16-byte borders are copied into rows that do; others are kept as they are. A product
+    fetches its weight while the kernel ahead of it on the stream still runs, but for the first one on each stream. Later
+    changes of the weight's tensors (by torch, or through ``out`` of the functions above) are ordered by the stream as ever."""
 
-    __slots__ = ("values", "scales", "channels", "width", "device")
+    __slots__ = ("values", "scales", "channels", "width", "device", "stream")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor) -> None:
         if values.dim() != 2 or values.dtype != torch.int8 or scales.shape != values.shape[:1]:
@@ -201,6 +210,7 @@ class Int8Weight:
         _check_rows(values, scales, "Int8Weight")
         self.values, self.scales, self.device = values, scales, values.device
         self.channels, self.width = values.shape
+        self.stream = None          # the stream of the last product: what wrote the weight is known to be done there
 
     @classmethod
     def quantize(cls, w: torch.Tensor) -> "Int8Weight":
@@ -229,12 +239,22 @@ def linear_int8(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = 
     _cuda(values, "linear_int8")
     if rows and weight.channels:
         with _on(values.device):
-            L = _lib.load()
+            L, stream = _lib.load(), _lib.current_stream()
+            if weight.stream != stream:
+                L.oi_launch_fence()          # the first product on a stream starts when all that is ahead of it has finished
+                weight.stream = stream
             _lib.check(L.oi_linear_int8(out.data_ptr(), _DT[out.dtype], out.stride(0), values.data_ptr(), _stride(values), scales.data_ptr(),
                                         weight.values.data_ptr(), _stride(weight.values), weight.scales.data_ptr(),
-                                        0 if bias is None else bias.data_ptr(), rows, weight.channels, width, _lib.current_stream()),
-                       "linear_int8")
+                                        0 if bias is None else bias.data_ptr(), rows, weight.channels, width, stream), "linear_int8")
     return out
+
+
+def status() -> int:
+    """0, or which bounded wait of a product ran out since the last call (synchronises the device)."""
+    from ctypes import byref, c_int
+    v = c_int(0)
+    _lib.check(_lib.load().oi_linear_int8_status(byref(v)), "linear_int8_status")
+    return v.value
 
 
 def _check_out(out: torch.Tensor, rows: int, width: int, device: torch.device, what: str) -> None:

@@ -18,7 +18,8 @@ DTYPES = [torch.float32, torch.bfloat16]
 def int8():
     from openinfer_b200.kernels import int8, lib
     lib.load()
-    return int8
+    yield int8
+    assert int8.status() == 0          # no bounded wait has run out
 
 
 def randn(*shape, seed=0, scale=1.0, dtype=torch.float32):
@@ -286,6 +287,27 @@ def test_one_tensor_as_rows_and_as_weight(int8, rows):
         q, s = held_exactly(x.float().cpu())
         assert torch.equal(got.cpu(), product_exactly(q, s, q, s, None, torch.float32))
         x = x.roll(1, dims=0) * 1.5 if rows > 1 else -x * 1.5
+
+
+@pytest.mark.parametrize("rows", [1, 100])
+def test_a_weight_that_is_written_again(int8, rows):
+    """New values in a weight's own memory, by torch and through ``out``, between products that follow at once."""
+    big = [randn(2048, 1024, seed=s).to(DEV) for s in range(3)]
+    x = int8.quantize_int8(randn(rows, 1024).to(DEV))
+    want = [int8.linear_int8(x, int8.Int8Weight.quantize(w)) for w in big]
+    weight = int8.Int8Weight.quantize(big[0])
+    held = int8.Int8Rows(weight.values, weight.scales)
+    got = []
+    for i in range(30):
+        if i % 2:
+            fresh = int8.quantize_int8(big[i % 3])
+            weight.values.copy_(fresh.values)
+            weight.scales.copy_(fresh.scales)
+        else:
+            int8.quantize_int8(big[i % 3], out=held)
+        got.append(int8.linear_int8(x, weight))
+    for i, g in enumerate(got):
+        assert torch.equal(g, want[i % 3])
 
 
 # ------------------------------------------------------------------------------------------------------------ together
