@@ -440,11 +440,10 @@ constexpr int kSmemOfTwo = 110 * 1024, kSmemOfOne = 208 * 1024;      // two CTAs
 
 template <typename TOut>
 int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
-                int c, cudaStream_t s) {
-  const int z = ceil_div(M, 256);                                      // tiles of x, of equal size
+                int c, int z, cudaStream_t s) {
   Shape g = {};
   g.M = M, g.N = N;
-  g.bn = ceil_div(ceil_div(M, z), 16) * 16;
+  g.bn = ceil_div(ceil_div(M, z), 16) * 16;                            // z tiles of x, of equal size
   g.num_kb = ceil_div(K, BK);
   g.kb_per_rank = ceil_div(g.num_kb, c);
   g.cols_per_owner = ceil_div(g.bn, c);
@@ -502,7 +501,7 @@ int launch(TOut* out, long long ldo, const void* x, long long ldx, const void* w
   int c = 1;
   while (c < 8 && tiles * c < oi_sm_count() && tiles * 2 * c <= at_once && num_kb / (2 * c) >= 2) c *= 2;
   while (c > 1 && (c - 1) * ((num_kb + c - 1) / c) >= num_kb) c /= 2;
-  return launch_rows(out, ldo, x, ldx, w, ldw, scales, M, N, K, c, s);
+  return launch_rows(out, ldo, x, ldx, w, ldw, scales, M, N, K, c, ceil_div(M, 256), s);
 }
 
 }  // namespace

@@ -12,117 +12,355 @@ namespace {
 // |y| as bits: ordered like the numbers, infinities above all finite ones and NaNs above those
 __device__ __forceinline__ unsigned magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
 
+// What a row is multiplied by, from the largest magnitude of its numbers. A norm's rows come without the reciprocal root mean
+// square `common`, which all of a row shares: q does not depend on it, the scale takes it up.
 struct RowScale {
-  float pre, inv, scale;
-  // `m`: the largest magnitude of the row. Below 2^-100 the row is taken times 2^80 first, or 127 / m would overflow.
-  __device__ __forceinline__ explicit RowScale(unsigned m) {
-    const float most = __uint_as_float(m);
-    if (m >= 0x7f800000u) {
-      pre = inv = 0.f;
-      scale = __uint_as_float(0x7fffffffu);
-    } else if (m == 0u) {
-      pre = inv = scale = 0.f;
-    } else {
-      const bool tiny = most < 7.888609e-31f;
-      pre = tiny ? 1.2089258e24f : 1.f;
-      inv = 127.f / (most * pre);
-      scale = tiny ? most * pre / 127.f / pre : most / 127.f;
-    }
+  float inv, scale;
+  bool tiny;            // m below 2^-100: the row is taken times 2^80 first, or 127 / m would overflow
+  unsigned keep;        // a row with an infinity or a NaN: all its bytes become zeros
+  __device__ __forceinline__ RowScale(unsigned m, float common) {
+    float most = __uint_as_float(m);
+    keep = m < 0x7f800000u ? ~0u : 0u;
+    tiny = most < 0x1p-100f;
+    if (tiny) most *= 0x1p80f;
+    inv = m ? 127.f / most : 0.f;
+    scale = keep ? (most * common) / 127.f : __uint_as_float(0x7fffffffu);
+    if (tiny) scale *= 0x1p-80f;
   }
-  __device__ __forceinline__ int quantise(float y) const { return __float2int_rn(y * pre * inv); }   // (NaN: 0)
+  // round(y * inv) in the low byte: added to 1.5 * 2^23, the sum's last bit stands for one (ties to even, as the sum is rounded)
+  __device__ __forceinline__ unsigned byte(float y) const {
+    if (tiny) y *= 0x1p80f;
+    return __float_as_uint(__fadd_rn(__fmul_rn(y, inv), 12582912.f));
+  }
+  __device__ __forceinline__ unsigned four(float a, float b, float c, float d) const {
+    return __byte_perm(__byte_perm(byte(a), byte(b), 0x0040), __byte_perm(byte(c), byte(d), 0x0040), 0x5410) & keep;
+  }
 };
 
-// What a row's numbers are made of. get(d) may be called more than once for the same d by the same thread.
+// Eight numbers of a row as they lie in memory, 16 bytes a load
+template <typename T>
+struct Eight {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = v[i];
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(reinterpret_cast<const unsigned*>(v)[e]);
+    } else {
+      const unsigned w = reinterpret_cast<const unsigned*>(v)[e >> 1];
+      return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+    }
+  }
+  __device__ __forceinline__ void set(int e, T x) {
+    if constexpr (sizeof(T) == 4) reinterpret_cast<unsigned*>(v)[e] = __float_as_uint(x);
+    else {
+      unsigned& w = reinterpret_cast<unsigned*>(v)[e >> 1];
+      const unsigned b = __bfloat16_as_ushort(x);
+      w = e & 1 ? (w & 0xffffu) | b << 16 : (w & 0xffff0000u) | b;
+    }
+  }
+};
+
+// What a row's numbers are made of. fetch(d) asks for eight of them (d a multiple of 8, aligned, all within the row), make() turns them
+// into numbers; one(d) is one number anywhere. Both add up in `squares` what a norm needs; again(d) is the number without.
 template <typename T>
 struct PlainRow {
   const T* x;
   long long ldx;
   static constexpr bool kNorm = false;
+  struct Raw { Eight<T> x; };
   __device__ __forceinline__ void begin(long long r) { x += r * ldx; }
-  __device__ __forceinline__ float get(int d) const { return to_f32(x[d]); }
+  __device__ __forceinline__ void fetch(int d, Raw& raw) const { raw.x.load(x + d); }
+  __device__ __forceinline__ void make(int d, Raw& raw, float (&y)[8], float& squares) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = raw.x.get(e);
+  }
+  __device__ __forceinline__ float one(int d, float& squares) const { return to_f32(x[d]); }
+  __device__ __forceinline__ float again(int d) const { return to_f32(x[d]); }
 };
 
+// x <- round(x + delta) is stored where there is a delta; the numbers are x * (w_offset + w), without the reciprocal root mean square
 template <typename T>
 struct NormRow {
-  T* x;                 // x <- round(x + delta) is stored where there is a delta
+  T* x;
   const T* delta;
   const void* w;
   long long ldx, ldd;
   int w_dtype;
-  float eps, w_offset, inv;
+  float eps, w_offset;
   static constexpr bool kNorm = true;
+  struct Raw { Eight<T> x, delta; Eight<float> w; };
   __device__ __forceinline__ void begin(long long r) {
     x += r * ldx;
     if (delta) delta += r * ldd;
   }
-  __device__ __forceinline__ float add(int d) {
+  __device__ __forceinline__ void fetch(int d, Raw& raw) const {
+    raw.x.load(x + d);
+    if (delta) raw.delta.load(delta + d);
+    if (w_dtype == OI_F32) raw.w.load(reinterpret_cast<const float*>(w) + d);
+    else raw.w.v[0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(w) + d);
+  }
+  __device__ __forceinline__ void make(int d, Raw& raw, float (&y)[8], float& squares) const {
+    if (delta) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) raw.x.set(e, from_f32<T>(raw.x.get(e) + raw.delta.get(e)));
+      raw.x.store(x + d);
+    }
+    float wv[8];
+    if (w_dtype == OI_F32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wv[e] = raw.w.get(e);
+    } else {
+      Eight<bf16> wb;
+      wb.v[0] = raw.w.v[0];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wv[e] = wb.get(e);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = raw.x.get(e);
+      squares += v * v;
+      y[e] = v * (w_offset + wv[e]);
+    }
+  }
+  __device__ __forceinline__ float one(int d, float& squares) const {
     float v = to_f32(x[d]);
     if (delta) {
       const T sum = from_f32<T>(v + to_f32(delta[d]));
       x[d] = sum;
       v = to_f32(sum);
     }
-    return v;
+    squares += v * v;
+    return v * (w_offset + load_as_f32(w, w_dtype, d));
   }
-  __device__ __forceinline__ float get(int d) const { return to_f32(x[d]) * inv * (w_offset + load_as_f32(w, w_dtype, d)); }
+  __device__ __forceinline__ float again(int d) const { return to_f32(x[d]) * (w_offset + load_as_f32(w, w_dtype, d)); }
 };
 
+// The activation by the special-function unit's exponential and reciprocal (2 ulp each): what follows is a rounding to 8 bits
 template <typename T>
 struct GateRow {
   const T* x;
   long long ldx;
-  int block, act;
+  int block, act, whole;     // whole: all gates, then all ups
   static constexpr bool kNorm = false;
+  struct Raw { Eight<T> gate, up; };
   __device__ __forceinline__ void begin(long long r) { x += r * ldx; }
-  __device__ __forceinline__ float get(int d) const {
-    const int at = d / block * (2 * block) + d % block;
-    return glu_act<false>(to_f32(x[at]), to_f32(x[at + block]), act, 0.f);
+  __device__ __forceinline__ const T* at(int d) const { return x + (whole ? d : d / block * block + d); }
+  __device__ __forceinline__ void fetch(int d, Raw& raw) const {
+    raw.gate.load(at(d));
+    raw.up.load(at(d) + block);
   }
+  __device__ __forceinline__ void make(int d, Raw& raw, float (&y)[8], float& squares) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = glu_act<true>(raw.gate.get(e), raw.up.get(e), act, 0.f);
+  }
+  __device__ __forceinline__ float one(int d, float& squares) const { return again(d); }
+  __device__ __forceinline__ float again(int d) const { return glu_act<true>(to_f32(at(d)[0]), to_f32(at(d)[block]), act, 0.f); }
 };
 
-// One block a row, any length and any alignment: the row is read once for each thing that is asked of all of it.
-template <typename Row>
-__global__ void rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int cols) {
+// A row in registers, UNITS times eight numbers a thread, read once: by a warp (kWarps: rows of up to 1,024 numbers, eight rows a
+// block) or by a block. kVec: 16 bytes a load, eight neighbours a thread; else neighbours lie in neighbouring threads and the bytes
+// are put together in shared memory. One exchange between the warps: the largest magnitude and a norm's sum of squares at
+// once. How a row is shared out goes by its length alone, so that a row's result does not depend on how many there are.
+template <typename Row, bool kVec, int UNITS, bool kWarps>
+__global__ void __launch_bounds__(kWarps || UNITS == 1 ? 256 : 512)
+rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows, int cols) {
   pdl_start();
-  __shared__ float sums[32];
-  __shared__ unsigned most;
+  extern __shared__ __align__(16) unsigned char bytes[];
+  __shared__ float part_squares[32];
+  __shared__ unsigned part_most[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long r = kWarps ? (long long)blockIdx.x * 8 + warp : blockIdx.x;
+  if (kWarps && r >= rows) return;
+  const int me = kWarps ? lane : threadIdx.x, step = kWarps ? 32 : blockDim.x;
+  row.begin(r);
+  q += r * ldq;
+
+  float y[UNITS][8], squares = 0.f;
+  unsigned most = 0u;
+  if constexpr (kVec) {
+    constexpr int kAhead = UNITS < 2 ? UNITS : 2;      // units asked for before the first is used
+#pragma unroll
+    for (int u0 = 0; u0 < UNITS; u0 += kAhead) {
+      typename Row::Raw raw[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int d = (me + (u0 + u) * step) * 8;
+        if (d + 8 <= cols) row.fetch(d, raw[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int d = (me + (u0 + u) * step) * 8;
+        if (d + 8 <= cols) row.make(d, raw[u], y[u0 + u], squares);
+        else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[u0 + u][e] = d + e < cols ? row.one(d + e, squares) : 0.f;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < UNITS * 8; ++i) {
+      const int d = me + i * step;
+      y[i / 8][i % 8] = d < cols ? row.one(d, squares) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < UNITS * 8; ++i) most = max(most, magnitude(y[i / 8][i % 8]));
+  most = __reduce_max_sync(0xffffffffu, most);
+  if constexpr (Row::kNorm) squares = warp_sum(squares);
+  if constexpr (!kWarps) {
+    if (lane == 0) {
+      part_most[warp] = most;
+      part_squares[warp] = squares;
+    }
+    __syncthreads();
+    const int warps = blockDim.x >> 5;
+    most = __reduce_max_sync(0xffffffffu, lane < warps ? part_most[lane] : 0u);
+    if constexpr (Row::kNorm) squares = warp_sum(lane < warps ? part_squares[lane] : 0.f);
+  }
+  float common = 1.f;
+  if constexpr (Row::kNorm) common = rsqrtf(squares / (float)cols + row.eps);
+  const RowScale s(most, common);
+  if (me == 0) scales[r] = s.scale;
+  if constexpr (kVec) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int d = (me + u * step) * 8;
+      const uint2 o = {s.four(y[u][0], y[u][1], y[u][2], y[u][3]), s.four(y[u][4], y[u][5], y[u][6], y[u][7])};
+      if (d + 8 <= cols) *reinterpret_cast<uint2*>(q + d) = o;
+      else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (d + e < cols) q[d + e] = (signed char)((e < 4 ? o.x : o.y) >> 8 * (e & 3));
+      }
+    }
+  } else {
+    unsigned char* mine = bytes + (kWarps ? warp * 1024 : 0);
+#pragma unroll
+    for (int i = 0; i < UNITS * 8; ++i) {
+      const int d = me + i * step;
+      if (d < cols) mine[d] = (unsigned char)(s.byte(y[i / 8][i % 8]) & s.keep);
+    }
+    if constexpr (kWarps) __syncwarp();
+    else __syncthreads();
+    for (int d = me * 16; d < cols; d += step * 16) {
+      if (d + 16 <= cols) *reinterpret_cast<uint4*>(q + d) = *reinterpret_cast<const uint4*>(mine + d);
+      else
+        for (int e = d; e < cols; ++e) q[e] = (signed char)mine[e];
+    }
+  }
+}
+
+// Rows longer than 512 threads hold in registers: one block a row, read once for each thing that is asked of all of it.
+template <typename Row>
+__global__ void __launch_bounds__(1024) long_rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int cols) {
+  pdl_start();
+  __shared__ float part_squares[32];
+  __shared__ unsigned part_most[32];
   const long long r = blockIdx.x;
   row.begin(r);
   q += r * ldq;
-  if (threadIdx.x == 0) most = 0u;
-  if constexpr (Row::kNorm) {
-    float ss = 0.f;
-    for (int d = threadIdx.x; d < cols; d += blockDim.x) {
-      const float v = row.add(d);
-      ss += v * v;
-    }
-    ss = block_sum(ss, sums);
-    row.inv = rsqrtf(ss / (float)cols + row.eps);
+  float squares = 0.f;
+  unsigned most = 0u;
+  for (int d = threadIdx.x; d < cols; d += 1024) most = max(most, magnitude(row.one(d, squares)));
+  most = __reduce_max_sync(0xffffffffu, most);
+  if constexpr (Row::kNorm) squares = warp_sum(squares);
+  if ((threadIdx.x & 31) == 0) {
+    part_most[threadIdx.x >> 5] = most;
+    part_squares[threadIdx.x >> 5] = squares;
   }
-  unsigned m = 0u;
-  for (int d = threadIdx.x; d < cols; d += blockDim.x) m = max(m, magnitude(row.get(d)));
-  m = __reduce_max_sync(0xffffffffu, m);
-  __syncthreads();                       // `most` is zero
-  if ((threadIdx.x & 31) == 0) atomicMax(&most, m);
   __syncthreads();
-  const RowScale s(most);
-  for (int d = threadIdx.x; d < cols; d += blockDim.x) q[d] = (signed char)s.quantise(row.get(d));
+  most = __reduce_max_sync(0xffffffffu, part_most[threadIdx.x & 31]);
+  float common = 1.f;
+  if constexpr (Row::kNorm) common = rsqrtf(warp_sum(part_squares[threadIdx.x & 31]) / (float)cols + row.eps);
+  const RowScale s(most, common);
+  for (int d = threadIdx.x; d < cols; d += 1024) q[d] = (signed char)(s.byte(row.again(d)) & s.keep);
   if (threadIdx.x == 0) scales[r] = s.scale;
 }
 
+template <typename Row, bool kVec>
+void launch_rows(const Row& row, signed char* q, long long ldq, float* scales, int rows, int cols, cudaStream_t s) {
+  const int units = ceil_div(cols, 8);
+  if (units <= 128) {                                  // a warp a row
+    const int grid = ceil_div(rows, 8), smem = kVec ? 0 : 8 * 1024;
+    if (units <= 32) oi_launch(rows_int8_kernel<Row, kVec, 1, true>, grid, 256, smem, s, row, q, ldq, scales, rows, cols);
+    else if (units <= 64) oi_launch(rows_int8_kernel<Row, kVec, 2, true>, grid, 256, smem, s, row, q, ldq, scales, rows, cols);
+    else oi_launch(rows_int8_kernel<Row, kVec, 4, true>, grid, 256, smem, s, row, q, ldq, scales, rows, cols);
+    return;
+  }
+  const int smem = kVec ? 0 : ceil_div(cols, 16) * 16;
+  auto threads = [&](int each) { return ceil_div(ceil_div(units, each), 32) * 32; };
+  if (units <= 256) oi_launch(rows_int8_kernel<Row, kVec, 1, false>, rows, threads(1), smem, s, row, q, ldq, scales, rows, cols);
+  else if (units <= 1024) oi_launch(rows_int8_kernel<Row, kVec, 2, false>, rows, threads(2), smem, s, row, q, ldq, scales, rows, cols);
+  else if (units <= 2048) oi_launch(rows_int8_kernel<Row, kVec, 4, false>, rows, threads(4), smem, s, row, q, ldq, scales, rows, cols);
+  else if (units <= 4096) oi_launch(rows_int8_kernel<Row, kVec, 8, false>, rows, threads(8), smem, s, row, q, ldq, scales, rows, cols);
+  else oi_launch(long_rows_int8_kernel<Row>, rows, 1024, 0, s, row, q, ldq, scales, cols);
+}
+
+// vec: everything that a row is read from starts on 16-byte borders, and the next row's too, whether there is one or not: one row
+// of a matrix is shared out among the threads as it is among others
 template <typename Row>
-int launch_rows(const Row& row, void* q, long long ldq, float* scales, int rows, int cols, cudaStream_t s) {
-  oi_launch(rows_int8_kernel<Row>, rows, 256, 0, s, row, (signed char*)q, ldq, scales, cols);
+int launch(const Row& row, bool vec, void* q, long long ldq, float* scales, int rows, int cols, cudaStream_t s) {
+  if (vec) launch_rows<Row, true>(row, (signed char*)q, ldq, scales, rows, cols, s);
+  else launch_rows<Row, false>(row, (signed char*)q, ldq, scales, rows, cols, s);
   OI_CHECK_LAUNCH();
   return OI_OK;
 }
 
-template <typename T>
-__global__ void dequantize_kernel(T* out, long long ldo, const signed char* q, long long ldq, const float* scales, int cols) {
+bool on_borders(const void* p, long long ld, int esize) { return (uintptr_t)p % 16 == 0 && ld * esize % 16 == 0; }
+
+// Sixteen numbers a thread: neighbours where rows start on 16-byte borders, else every 256th. A byte becomes a number without a
+// conversion: with its sign turned it is the last byte of 2^23 + 128 + q.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(256) dequantize_kernel(T* out, long long ldo, const signed char* q, long long ldq, const float* scales, int cols) {
   pdl_start();
-  const long long r = blockIdx.x;
+  const long long r = blockIdx.y;
+  const int first = blockIdx.x * (256 * 16), d = kVec ? first + threadIdx.x * 16 : first + threadIdx.x;
+  if (d >= cols) return;
   const float scale = scales[r];
-  for (int d = threadIdx.x; d < cols; d += blockDim.x) out[r * ldo + d] = from_f32<T>((float)q[r * ldq + d] * scale);
+  out += r * ldo;
+  q += r * ldq;
+  if (kVec && d + 16 <= cols) {
+    const uint4 v = *reinterpret_cast<const uint4*>(q + d);
+    const unsigned words[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      Eight<T> o;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float f = __uint_as_float(__byte_perm(words[2 * h + e / 4], 0x4b000000u, 0x7650 + e % 4)) - 8388736.f;
+        o.set(e, from_f32<T>(f * scale));
+      }
+      o.store(out + d + 8 * h);
+    }
+  } else {
+    constexpr int kStep = kVec ? 1 : 256;
+    signed char v[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = d + e * kStep < cols ? q[d + e * kStep] : 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (d + e * kStep < cols) out[d + e * kStep] = from_f32<T>((float)v[e] * scale);
+  }
+}
+
+template <typename T>
+int launch_dequantize(T* out, long long ldo, const signed char* q, long long ldq, const float* scales, int rows, int cols, cudaStream_t s) {
+  const bool vec = on_borders(out, rows > 1 ? ldo : 0, sizeof(T));
+  for (long long r = 0; r < rows; r += 65535) {        // one launch, but for more rows than a grid has
+    const dim3 grid(ceil_div(cols, 256 * 16), (unsigned)(rows - r < 65535 ? rows - r : 65535));
+    if (vec) oi_launch(dequantize_kernel<T, true>, grid, 256, 0, s, out + r * ldo, ldo, q + r * ldq, ldq, scales + r, cols);
+    else oi_launch(dequantize_kernel<T, false>, grid, 256, 0, s, out + r * ldo, ldo, q + r * ldq, ldq, scales + r, cols);
+  }
+  OI_CHECK_LAUNCH();
+  return OI_OK;
 }
 
 int check_rows(const char* what, const void* q, long long ldq, const float* scales, int rows, int cols) {
@@ -140,8 +378,9 @@ OI_API int oi_quantize_int8(void* q, long long ldq, float* scales, const void* x
   OI_REQUIRE(dtype == OI_F32 || dtype == OI_BF16, "quantize_int8: unknown dtype code %d", dtype);
   if (rows == 0) return OI_OK;
   cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == OI_F32) return launch_rows(PlainRow<float>{(const float*)x, ldx}, q, ldq, scales, rows, cols, s);
-  return launch_rows(PlainRow<bf16>{(const bf16*)x, ldx}, q, ldq, scales, rows, cols, s);
+  const bool vec = on_borders(x, ldx, dtype == OI_F32 ? 4 : 2);
+  if (dtype == OI_F32) return launch(PlainRow<float>{(const float*)x, ldx}, vec, q, ldq, scales, rows, cols, s);
+  return launch(PlainRow<bf16>{(const bf16*)x, ldx}, vec, q, ldq, scales, rows, cols, s);
 }
 
 // The rows of oi_rmsnorm's output, not rounded: x <- round(x + delta) (stored; delta may be null), then
@@ -154,9 +393,11 @@ OI_API int oi_rmsnorm_int8(void* q, long long ldq, float* scales, void* x, long 
   OI_REQUIRE(!delta || rows <= 1 || ldx >= cols, "rmsnorm_int8: rows of %d that start %lld apart cannot take a sum", cols, ldx);
   if (rows == 0) return OI_OK;
   cudaStream_t s = (cudaStream_t)stream;
+  const int esize = dtype == OI_F32 ? 4 : 2;
+  const bool vec = on_borders(x, ldx, esize) && (!delta || on_borders(delta, ldd, esize)) && (uintptr_t)w % 16 == 0;
   if (dtype == OI_F32)
-    return launch_rows(NormRow<float>{(float*)x, (const float*)delta, w, ldx, ldd, w_dtype, eps, w_offset, 0.f}, q, ldq, scales, rows, cols, s);
-  return launch_rows(NormRow<bf16>{(bf16*)x, (const bf16*)delta, w, ldx, ldd, w_dtype, eps, w_offset, 0.f}, q, ldq, scales, rows, cols, s);
+    return launch(NormRow<float>{(float*)x, (const float*)delta, w, ldx, ldd, w_dtype, eps, w_offset}, vec, q, ldq, scales, rows, cols, s);
+  return launch(NormRow<bf16>{(bf16*)x, (const bf16*)delta, w, ldx, ldd, w_dtype, eps, w_offset}, vec, q, ldq, scales, rows, cols, s);
 }
 
 // The rows of oi_silu_mul's output, not rounded: act(gate) * up of gate_up [rows, 2 inter] (row stride ldx elements), which lies
@@ -169,8 +410,9 @@ OI_API int oi_silu_mul_int8(void* q, long long ldq, float* scales, const void* g
   OI_REQUIRE(act == OI_ACT_SILU || act == OI_ACT_GELU_TANH, "silu_mul_int8: unknown activation code %d", act);
   if (rows == 0) return OI_OK;
   cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == OI_F32) return launch_rows(GateRow<float>{(const float*)gate_up, ldx, block, act}, q, ldq, scales, rows, inter, s);
-  return launch_rows(GateRow<bf16>{(const bf16*)gate_up, ldx, block, act}, q, ldq, scales, rows, inter, s);
+  const bool vec = block % 8 == 0 && on_borders(gate_up, ldx, dtype == OI_F32 ? 4 : 2);
+  if (dtype == OI_F32) return launch(GateRow<float>{(const float*)gate_up, ldx, block, act, block == inter}, vec, q, ldq, scales, rows, inter, s);
+  return launch(GateRow<bf16>{(const bf16*)gate_up, ldx, block, act, block == inter}, vec, q, ldq, scales, rows, inter, s);
 }
 
 // out[r, :] = round(q[r, :] * scales[r]) (row stride ldo elements)
@@ -181,8 +423,6 @@ OI_API int oi_dequantize_int8(void* out, int dtype, long long ldo, const void* q
   OI_REQUIRE(rows <= 1 || ldo >= cols, "dequantize_int8: rows of %d that start %lld apart", cols, ldo);
   if (rows == 0) return OI_OK;
   cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == OI_F32) oi_launch(dequantize_kernel<float>, rows, 256, 0, s, (float*)out, ldo, (const signed char*)q, ldq, scales, cols);
-  else oi_launch(dequantize_kernel<bf16>, rows, 256, 0, s, (bf16*)out, ldo, (const signed char*)q, ldq, scales, cols);
-  OI_CHECK_LAUNCH();
-  return OI_OK;
+  if (dtype == OI_F32) return launch_dequantize((float*)out, ldo, (const signed char*)q, ldq, scales, rows, cols, s);
+  return launch_dequantize((bf16*)out, ldo, (const signed char*)q, ldq, scales, rows, cols, s);
 }

@@ -15,8 +15,7 @@ Every function launches on the current stream of its tensors' device. Results th
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -36,82 +35,90 @@ class Int8Rows(NamedTuple):
     scales: torch.Tensor
 
 
-def _float_rows(t: torch.Tensor, what: str) -> int:
-    """The dtype code of a matrix of floating rows (any row stride, neighbours next to each other)."""
+# The checks below ask a tensor for each thing once and hand on what they found: at a few rows a call's time is the host's.
+
+def _float_rows(t: torch.Tensor, what: str) -> Tuple[int, int, int, int]:
+    """(dtype code, rows, width, row stride) of a matrix of floating rows (any row stride, neighbours next to each other)."""
     code = _DT.get(t.dtype)
     if code is None:
         raise KernelError(f"{what}: dtype {t.dtype} is not supported (float32 or bfloat16)")
-    if t.dim() != 2 or t.shape[1] < 1 or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise KernelError(f"{what}: expected rows of at least one number, neighbours next to each other: shape {tuple(t.shape)}, strides {t.stride()}")
-    return code
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or shape[1] < 1 or (strides[1] != 1 and shape[1] > 1):
+        raise KernelError(f"{what}: expected rows of at least one number, neighbours next to each other: shape {tuple(shape)}, strides {strides}")
+    return code, shape[0], shape[1], strides[0]
 
 
-def _cuda(t: torch.Tensor, what: str) -> None:
-    if not t.is_cuda:
-        raise KernelError(f"{what}: the tensor is not on a CUDA device; this package has no CPU path")
-
-
-def _stride(t: torch.Tensor) -> int:
-    """The row stride; where there is one row, its width rounded up to what 8-bit rows start on (the stride then means nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // ALIGN) * ALIGN
-
-
-def _check_rows(values: torch.Tensor, scales: torch.Tensor, what: str) -> None:
+def _int8_rows(held: Int8Rows, what: str) -> Tuple[int, int, int, int, int, int]:
+    """(address, row stride, rows, width, address of the scales, device index) of 8-bit rows. The stride of one row is its width
+    rounded up to what rows start on (it means nothing then)."""
+    values, scales = held
     if values.dtype != torch.int8 or scales.dtype != torch.float32:
         raise KernelError(f"{what}: 8-bit rows are int8 with float32 scales: {values.dtype}, {scales.dtype}")
-    if values.dim() != 2 or values.shape[1] < 1 or (values.stride(1) != 1 and values.shape[1] > 1):
-        raise KernelError(f"{what}: expected rows of at least one integer, neighbours next to each other: shape {tuple(values.shape)}, strides {values.stride()}")
-    rows, width = values.shape
-    if values.data_ptr() % ALIGN or (rows > 1 and (values.stride(0) % ALIGN or values.stride(0) < width)):
-        raise KernelError(f"{what}: 8-bit rows must start on {ALIGN}-byte borders and not overlap (row stride {values.stride(0)}, width {width})")
+    shape, strides = values.shape, values.stride()
+    if len(shape) != 2 or shape[1] < 1 or (strides[1] != 1 and shape[1] > 1):
+        raise KernelError(f"{what}: expected rows of at least one integer, neighbours next to each other: shape {tuple(shape)}, strides {strides}")
+    rows, width = shape
+    address, stride = values.data_ptr(), strides[0] if rows > 1 else -(-width // ALIGN) * ALIGN
+    if address % ALIGN or stride % ALIGN or stride < width:
+        raise KernelError(f"{what}: 8-bit rows must start on {ALIGN}-byte borders and not overlap (row stride {stride}, width {width})")
     if scales.shape != (rows,) or not scales.is_contiguous():
         raise KernelError(f"{what}: expected {rows} scales in a row: shape {tuple(scales.shape)}")
-    if values.device != scales.device:
+    device = values.get_device()
+    if device != scales.get_device():
         raise KernelError(f"{what}: values and scales must be on one device: {values.device}, {scales.device}")
+    return address, stride, rows, width, scales.data_ptr(), device
+
+
+def _cuda(device: int, what: str) -> None:
+    if device < 0:
+        raise KernelError(f"{what}: the tensor is not on a CUDA device; this package has no CPU path")
 
 
 def empty_rows(rows: int, width: int, device) -> Int8Rows:
     """Room for rows of 8-bit integers."""
     room = -(-width // ALIGN) * ALIGN
-    values = torch.empty((rows, room), dtype=torch.int8, device=device)
-    return Int8Rows(values if room == width else values[:, :width], torch.empty(rows, dtype=torch.float32, device=device))
+    return Int8Rows(torch.empty_strided((rows, width), (room, 1), dtype=torch.int8, device=device),
+                    torch.empty(rows, dtype=torch.float32, device=device))
 
 
-def _room(out: Optional[Int8Rows], x: torch.Tensor, width: int, what: str) -> Int8Rows:
+def _room(out: Optional[Int8Rows], x: torch.Tensor, rows: int, width: int, device: int, what: str):
+    """(8-bit rows, their address, row stride, address of the scales)"""
     if out is None:
-        return empty_rows(x.shape[0], width, x.device)
-    _check_rows(*out, what)
-    if out.values.shape != (x.shape[0], width) or out.values.device != x.device:
-        raise KernelError(f"{what}: room for {tuple(out.values.shape)} on {out.values.device}, needed {(x.shape[0], width)} on {x.device}")
-    return out
+        out = empty_rows(rows, width, x.device)
+        return out, out.values.data_ptr(), -(-width // ALIGN) * ALIGN, out.scales.data_ptr()
+    address, stride, has_rows, has_width, scales, on = _int8_rows(out, what)
+    if (has_rows, has_width, on) != (rows, width, device):
+        raise KernelError(f"{what}: room for {(has_rows, has_width)} on {out.values.device}, needed {(rows, width)} on {x.device}")
+    return out, address, stride, scales
 
 
-def _on(device: torch.device):
-    """The tensors' own device for the launch, whatever the calling thread's current one is."""
-    return _HERE if _lib.current_device() == device.index else torch.cuda.device(device)
+def _launch(device: int, what: str, entry, *args) -> None:
+    """Calls an entry point with the current stream of the tensors' own device, whatever the calling thread's current one is."""
+    if device == _lib.current_device():
+        code = entry(*args, _lib.current_stream())
+    else:
+        with torch.cuda.device(device):
+            code = entry(*args, _lib.current_stream())
+    if code:
+        _lib.check(code, what)
 
 
-_HERE = nullcontext()
-
-
-def _done(L, out: Optional[Int8Rows]) -> None:
+def _done(L, given: Optional[Int8Rows]) -> None:
     """Rows written into given memory may be those of a weight, which products fetch ahead: the next launch starts behind this one."""
-    if out is not None:
+    if given is not None:
         L.oi_launch_fence()
 
 
 def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
     """The rows of ``x`` [rows, width] (float32 or bfloat16, row stride free) as 8-bit integers."""
-    code = _float_rows(x, "quantize_int8")
-    rows, width = x.shape
-    _cuda(x, "quantize_int8")
-    held = _room(out, x, width, "quantize_int8")
+    code, rows, width, stride = _float_rows(x, "quantize_int8")
+    device = x.get_device()
+    _cuda(device, "quantize_int8")
+    held, q, ldq, scales = _room(out, x, rows, width, device, "quantize_int8")
     if rows:
-        with _on(x.device):
-            L = _lib.load()
-            _lib.check(L.oi_quantize_int8(held.values.data_ptr(), _stride(held.values), held.scales.data_ptr(), x.data_ptr(), code,
-                                          x.stride(0), rows, width, _lib.current_stream()), "quantize_int8")
-            _done(L, out)
+        L = _lib.load()
+        _launch(device, "quantize_int8", L.oi_quantize_int8, q, ldq, scales, x.data_ptr(), code, stride, rows, width)
+        _done(L, out)
     return held
 
 
@@ -120,69 +127,75 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, delta: Op
     """x * rsqrt(mean(x^2) + eps) * (weight_offset + weight), row by row, as 8-bit integers.
 
     ``delta``: x <- x + delta first (rounded, stored in x), the norm is of the sum as it is stored."""
-    code = _float_rows(x, "rmsnorm_int8")
-    rows, width = x.shape
+    code, rows, width, stride = _float_rows(x, "rmsnorm_int8")
+    device, address = x.get_device(), x.data_ptr()
     w_code = _DT.get(weight.dtype)
-    if w_code is None or weight.shape != (width,) or not weight.is_contiguous() or weight.device != x.device:
+    if w_code is None or weight.shape != (width,) or not weight.is_contiguous() or weight.get_device() != device:
         raise KernelError(f"rmsnorm_int8: expected a float32 or bfloat16 weight of {width} numbers on {x.device}: {weight.dtype} {tuple(weight.shape)} on {weight.device}")
+    d_address = d_stride = 0
     if delta is not None:
-        _float_rows(delta, "rmsnorm_int8 delta")
-        if delta.dtype != x.dtype or delta.shape != x.shape or delta.device != x.device:
-            raise KernelError(f"rmsnorm_int8: x and delta must share a dtype, a shape and a device: {x.dtype} {tuple(x.shape)}, {delta.dtype} {tuple(delta.shape)}")
-        if rows > 1 and x.stride(0) < width:
-            raise KernelError(f"rmsnorm_int8: rows that overlap (row stride {x.stride(0)}, width {width}) cannot take a sum")
-        if (delta.data_ptr(), delta.stride(0)) != (x.data_ptr(), x.stride(0)) and _overlap(x, delta):
+        d_code, d_rows, d_width, d_stride = _float_rows(delta, "rmsnorm_int8 delta")
+        if (d_code, d_rows, d_width, delta.get_device()) != (code, rows, width, device):
+            raise KernelError(f"rmsnorm_int8: x and delta must share a dtype, a shape and a device: {x.dtype} {tuple(x.shape)} on {x.device}, {delta.dtype} {tuple(delta.shape)} on {delta.device}")
+        if rows > 1 and stride < width:
+            raise KernelError(f"rmsnorm_int8: rows that overlap (row stride {stride}, width {width}) cannot take a sum")
+        d_address = delta.data_ptr()
+        size = 2 if code else 4
+        if (d_address < address + ((rows - 1) * stride + width) * size and address < d_address + ((rows - 1) * d_stride + width) * size
+                and rows and (d_address, d_stride) != (address, stride)):
             raise KernelError("rmsnorm_int8: x and delta must be the same rows or not overlap")
-    _cuda(x, "rmsnorm_int8")
-    held = _room(out, x, width, "rmsnorm_int8")
+    _cuda(device, "rmsnorm_int8")
+    held, q, ldq, scales = _room(out, x, rows, width, device, "rmsnorm_int8")
     if rows:
-        with _on(x.device):
-            L = _lib.load()
-            _lib.check(L.oi_rmsnorm_int8(held.values.data_ptr(), _stride(held.values), held.scales.data_ptr(), x.data_ptr(), x.stride(0),
-                                         0 if delta is None else delta.data_ptr(), 0 if delta is None else delta.stride(0), code,
-                                         weight.data_ptr(), w_code, rows, width, float(eps), float(weight_offset),
-                                         _lib.current_stream()), "rmsnorm_int8")
-            _done(L, out)
+        L = _lib.load()
+        _launch(device, "rmsnorm_int8", L.oi_rmsnorm_int8, q, ldq, scales, address, stride, d_address, d_stride, code, weight.data_ptr(),
+                w_code, rows, width, eps, weight_offset)
+        _done(L, out)
     return held
 
 
 def silu_mul_int8(gate_up: torch.Tensor, block: Optional[int] = None, act: str = "silu", out: Optional[Int8Rows] = None) -> Int8Rows:
     """act(gate_i) * up_i of a fused gate|up buffer [rows, 2 * inter] as 8-bit integers [rows, inter]; the buffer is laid out in
-    blocks of ``block`` gate values followed by their up values (default: all gates, then all ups)."""
-    code = _float_rows(gate_up, "silu_mul_int8")
-    rows, both = gate_up.shape
+    blocks of ``block`` gate values followed by their up values (default: all gates, then all ups). ``act``: "silu" or "gelu_tanh"."""
+    code, rows, both, stride = _float_rows(gate_up, "silu_mul_int8")
     inter = both // 2
     block = inter if block is None else int(block)
     if both % 2 or block < 1 or inter % block:
         raise KernelError(f"silu_mul_int8: gate_up of {both} numbers in blocks of {block} gates and {block} ups")
     act_c = act_code(act)
-    _cuda(gate_up, "silu_mul_int8")
-    held = _room(out, gate_up, inter, "silu_mul_int8")
+    device = gate_up.get_device()
+    _cuda(device, "silu_mul_int8")
+    held, q, ldq, scales = _room(out, gate_up, rows, inter, device, "silu_mul_int8")
     if rows:
-        with _on(gate_up.device):
-            L = _lib.load()
-            _lib.check(L.oi_silu_mul_int8(held.values.data_ptr(), _stride(held.values), held.scales.data_ptr(), gate_up.data_ptr(), code,
-                                          gate_up.stride(0), rows, inter, block, act_c, _lib.current_stream()), "silu_mul_int8")
-            _done(L, out)
+        L = _lib.load()
+        _launch(device, "silu_mul_int8", L.oi_silu_mul_int8, q, ldq, scales, gate_up.data_ptr(), code, stride, rows, inter, block, act_c)
+        _done(L, out)
     return held
 
 
-def dequantize_int8(rows: Int8Rows, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The numbers that 8-bit rows stand for, rounded once to ``dtype`` (float32 or bfloat16)."""
-    values, scales = rows
-    _check_rows(values, scales, "dequantize_int8")
+def _results(out: Optional[torch.Tensor], dtype: torch.dtype, rows: int, width: int, like: torch.Tensor, device: int, what: str):
+    """(results [rows, width], their dtype code, row stride)"""
     if out is None:
-        if dtype not in _DT:
-            raise KernelError(f"dequantize_int8: dtype {dtype} is not supported (float32 or bfloat16)")
-        out = torch.empty(values.shape, dtype=dtype, device=values.device)
-    else:
-        _check_out(out, values.shape[0], values.shape[1], values.device, "dequantize_int8")
-    _cuda(values, "dequantize_int8")
-    if values.shape[0]:
-        with _on(values.device):
-            L = _lib.load()
-            _lib.check(L.oi_dequantize_int8(out.data_ptr(), _DT[out.dtype], out.stride(0), values.data_ptr(), _stride(values),
-                                            scales.data_ptr(), values.shape[0], values.shape[1], _lib.current_stream()), "dequantize_int8")
+        code = _DT.get(dtype)
+        if code is None:
+            raise KernelError(f"{what}: output dtype {dtype} is not supported (float32 or bfloat16)")
+        _cuda(device, what)
+        return torch.empty(rows, width, dtype=dtype, device=like.device), code, width
+    code, shape, strides = _DT.get(out.dtype), out.shape, out.stride()
+    if code is None or shape != (rows, width) or out.get_device() != device:
+        raise KernelError(f"{what}: expected float32 or bfloat16 results [{rows}, {width}] on {like.device}: {out.dtype} {tuple(shape)} on {out.device}")
+    if (width > 1 and strides[1] != 1) or (rows > 1 and strides[0] < width):
+        raise KernelError(f"{what}: result rows must not overlap, neighbours next to each other: strides {strides}")
+    _cuda(device, what)
+    return out, code, strides[0]
+
+
+def dequantize_int8(rows: Int8Rows, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The numbers that 8-bit rows stand for, rounded once to ``dtype`` (float32 or bfloat16) or to that of ``out`` (row stride free)."""
+    q, ldq, count, width, scales, device = _int8_rows(rows, "dequantize_int8")
+    out, code, stride = _results(out, dtype, count, width, rows[0], device, "dequantize_int8")
+    if count:
+        _launch(device, "dequantize_int8", _lib.load().oi_dequantize_int8, out.data_ptr(), code, stride, q, ldq, scales, count, width)
     return out
 
 
@@ -193,24 +206,24 @@ class Int8Weight:
     fetches its weight while the kernel ahead of it on the stream still runs, but for the first one on each stream. Later
     changes of the weight's tensors (by torch, or through ``out`` of the functions above) are ordered by the stream as ever."""
 
-    __slots__ = ("values", "scales", "channels", "width", "device", "stream")
+    __slots__ = ("values", "scales", "channels", "width", "device", "operands", "stream")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor) -> None:
         if values.dim() != 2 or values.dtype != torch.int8 or scales.shape != values.shape[:1]:
             raise KernelError(f"Int8Weight: expected int8 [channels, width] and a scale for each channel: {values.dtype} {tuple(values.shape)}, {tuple(scales.shape)}")
-        if not 1 <= values.shape[1] <= MAX_WIDTH:
-            raise KernelError(f"Int8Weight: sums of {values.shape[1]} products (1 to {MAX_WIDTH} are exact in 32 bits)")
-        if values.shape[1] > 1 and values.stride(1) != 1 or values.data_ptr() % ALIGN or values.shape[0] > 1 and (
-                values.stride(0) % ALIGN or values.stride(0) < values.shape[1]):
-            held = empty_rows(*values.shape, values.device).values
+        rows, width = values.shape
+        if not 1 <= width <= MAX_WIDTH:
+            raise KernelError(f"Int8Weight: sums of {width} products (1 to {MAX_WIDTH} are exact in 32 bits)")
+        strides = values.stride()
+        if (width > 1 and strides[1] != 1) or values.data_ptr() % ALIGN or (rows > 1 and (strides[0] % ALIGN or strides[0] < width)):
+            held = empty_rows(rows, width, values.device).values
             held.copy_(values)
             values = held
-        if not scales.is_contiguous():
-            scales = scales.contiguous()
-        _check_rows(values, scales, "Int8Weight")
-        self.values, self.scales, self.device = values, scales, values.device
-        self.channels, self.width = values.shape
-        self.stream = None          # the stream of the last product: what wrote the weight is known to be done there
+        self.values, self.scales, self.device = values, scales.contiguous(), values.device
+        self.channels, self.width = rows, width
+        q, ldq, _, _, scale, device = _int8_rows(Int8Rows(self.values, self.scales), "Int8Weight")
+        self.operands = (q, ldq, scale, device)
+        self.stream = None          # of the last product: what wrote the weight is known to be done there
 
     @classmethod
     def quantize(cls, w: torch.Tensor) -> "Int8Weight":
@@ -223,30 +236,34 @@ def linear_int8(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = 
     """x [rows, width] times the weight [channels, width], transposed: sums of 8-bit products exact in 32-bit integers, then
     float32(sum) * x's scale * the channel's scale (+ the channel's ``bias``, float32) and one rounding to ``out_dtype``
     (float32 or bfloat16, or that of ``out`` [rows, channels], whose row stride is free)."""
-    values, scales = x
-    _check_rows(values, scales, "linear_int8")
-    rows, width = values.shape
-    if width != weight.width or values.device != weight.device:
-        raise KernelError(f"linear_int8: rows of {width} on {values.device} and a weight of {weight.channels} x {weight.width} on {weight.device}")
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (weight.channels,) or not bias.is_contiguous() or bias.device != values.device):
-        raise KernelError(f"linear_int8: expected {weight.channels} float32 numbers of bias on {values.device}: {bias.dtype} {tuple(bias.shape)} on {bias.device}")
-    if out is None:
-        if out_dtype not in _DT:
-            raise KernelError(f"linear_int8: output dtype {out_dtype} is not supported (float32 or bfloat16)")
-        out = torch.empty((rows, weight.channels), dtype=out_dtype, device=values.device)
-    else:
-        _check_out(out, rows, weight.channels, values.device, "linear_int8")
-    _cuda(values, "linear_int8")
-    if rows and weight.channels:
-        with _on(values.device):
-            L, stream = _lib.load(), _lib.current_stream()
-            if weight.stream != stream:
-                L.oi_launch_fence()          # the first product on a stream starts when all that is ahead of it has finished
-                weight.stream = stream
-            _lib.check(L.oi_linear_int8(out.data_ptr(), _DT[out.dtype], out.stride(0), values.data_ptr(), _stride(values), scales.data_ptr(),
-                                        weight.values.data_ptr(), _stride(weight.values), weight.scales.data_ptr(),
-                                        0 if bias is None else bias.data_ptr(), rows, weight.channels, width, stream), "linear_int8")
+    q, ldq, rows, width, scales, device = _int8_rows(x, "linear_int8")
+    w, ldw, w_scales, w_device = weight.operands
+    channels = weight.channels
+    if width != weight.width or device != w_device:
+        raise KernelError(f"linear_int8: rows of {width} on {x[0].device} and a weight of {channels} x {weight.width} on {weight.device}")
+    b = 0
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.shape != (channels,) or not bias.is_contiguous() or bias.get_device() != device:
+            raise KernelError(f"linear_int8: expected {channels} float32 numbers of bias on {x[0].device}: {bias.dtype} {tuple(bias.shape)} on {bias.device}")
+        b = bias.data_ptr()
+    out, code, stride = _results(out, out_dtype, rows, channels, x[0], device, "linear_int8")
+    if rows and channels:
+        if device == _lib.current_device():
+            _product(weight, out.data_ptr(), code, stride, q, ldq, scales, w, ldw, w_scales, b, rows, channels, width)
+        else:
+            with torch.cuda.device(device):
+                _product(weight, out.data_ptr(), code, stride, q, ldq, scales, w, ldw, w_scales, b, rows, channels, width)
     return out
+
+
+def _product(weight: Int8Weight, *args) -> None:
+    L, stream = _lib.load(), _lib.current_stream()
+    if weight.stream != stream:
+        L.oi_launch_fence()          # the first product on a stream starts when all that is ahead of it has finished
+        weight.stream = stream
+    code = L.oi_linear_int8(*args, stream)
+    if code:
+        _lib.check(code, "linear_int8")
 
 
 def status() -> int:
@@ -255,20 +272,3 @@ def status() -> int:
     v = c_int(0)
     _lib.check(_lib.load().oi_linear_int8_status(byref(v)), "linear_int8_status")
     return v.value
-
-
-def _check_out(out: torch.Tensor, rows: int, width: int, device: torch.device, what: str) -> None:
-    if out.dtype not in _DT or out.shape != (rows, width) or out.device != device:
-        raise KernelError(f"{what}: expected float32 or bfloat16 results [{rows}, {width}] on {device}: {out.dtype} {tuple(out.shape)} on {out.device}")
-    if (width > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < width):
-        raise KernelError(f"{what}: result rows must not overlap, neighbours next to each other: strides {out.stride()}")
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two matrices of rows share bytes (or may)."""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
-    if not a.numel() or not b.numel():
-        return False
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1

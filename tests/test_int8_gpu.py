@@ -212,9 +212,9 @@ def integers(rows, width, seed):
 
 
 def on_device(int8, x, sx):
-    held = int8.empty_rows(*x.shape, DEV)
     room = -(-x.shape[1] // 16) * 16
-    held.values.as_strided((x.shape[0], room), (room, 1)).fill_(77)      # what lies behind an odd width must not count
+    wide = torch.full((x.shape[0], room), 77, dtype=torch.int8, device=DEV)      # what lies behind an odd width must not count
+    held = int8.Int8Rows(wide[:, :x.shape[1]], torch.empty(x.shape[0], device=DEV))
     held.values.copy_(x)
     held.scales.copy_(sx)
     return held
