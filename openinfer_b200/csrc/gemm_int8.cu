@@ -20,7 +20,20 @@ __device__ int g_int8_error = 0;            // set to a non-zero code when a bou
 __device__ __forceinline__ bool wait_on(unsigned bar, unsigned parity, volatile int* abort_flag, int code) {
   return tc::mbar_wait(bar, parity, abort_flag, &g_int8_error, code);
 }
-__device__ __forceinline__ float finish(int sum, float sx, float sw) { return __fmul_rn(__fmul_rn((float)sum, sx), sw); }
+__device__ __forceinline__ float finish(int sum, float sx, float sw, float b, bool biased) {
+  const float y = __fmul_rn(__fmul_rn((float)sum, sx), sw);
+  return biased ? __fadd_rn(y, b) : y;
+}
+
+// A place in a ring of stages and the parity of its turn. (A division a stage by each of the threads that issue copies and products
+// is on the path of every stage.)
+struct Ring {
+  int stage = 0;
+  unsigned parity = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++stage == stages) stage = 0, parity ^= 1;
+  }
+};
 
 struct Scales {
   const float *sx, *sw, *bias;
@@ -29,46 +42,32 @@ struct Scales {
 // ------------------------------------------------------------------------------------------------
 // Few rows. The product is formed transposed: 128 rows of w are the M side of tcgen05.mma, up to 256 rows of x (a multiple of
 // 16, `bn`) its N side, so a weight byte goes HBM -> TMA -> shared memory -> tensor core, and the accumulator [128 rows of
-// w x bn] lies in tensor memory. Grid (c, tiles of w, tiles of x): a cluster of c CTAs shares one tile, CTA r streaming k blocks
-// [r * kb_per_rank, ...) of it, and adds up: column j of the accumulator (a row of x) belongs to CTA j / cols_per_owner, into
-// whose shared memory every CTA deposits its partial sums of it.
+// w x bn] lies in tensor memory. Grid (c, tiles of w, tiles of x): a cluster of c CTAs (a power of two) shares one tile, CTA r
+// streaming k blocks [r * kb_per_rank, ...) of it, and adds up: row i of the accumulator (a row of w) belongs to CTA i / (128 / c),
+// into whose shared memory every CTA deposits its partial sums of it.
 //   warp 0     one thread issues the copies; the first ring-full of WEIGHT boxes is requested before the wait for the kernel
 //              ahead (programmatic dependent launch), which may still be writing x
 //   warp 1     allocates tensor memory (behind that wait: a kernel ahead that needs all of it may not have taken its own
 //              yet), one thread issues four products (K = 32) a stage
-//   warps 2-5  read the accumulator (one weight row a thread) and deposit; then all six warps add up, scale and store.
-constexpr int kThreads = 192;
+//   the others (four, or eight) read the accumulator (one row of w a thread) and deposit, or with c = 1 scale and store; then
+//              all warps add up, scale and store.
+// What the results cost shows in the instructions per column: with a column at a time, a branch and a cluster address each, and
+// six warps, 128 columns took 8,000 cycles to deposit and 8,700 to store (N 1024, K 1024, c 1).
+constexpr int kFewColumns = 32;             // up to so many rows of x a tile four warps read results, else eight
 
 struct Shape {
-  int M, N, num_kb, kb_per_rank, bn, stages, cols_per_owner, tmem_cols;
+  int M, N, num_kb, kb_per_rank, bn, stages, tmem_cols;
   int recv_offset;          // where deposits go: behind the ring, or over the drained ring (0)
+  int scale_offset;         // scales of the tile's rows of x [bn]
   int bar_offset;
-  int vec;                  // result rows may be stored four numbers at a time
 };
 
-template <typename TOut>
-__device__ __forceinline__ void store4(TOut* dst, const float (&y)[4], int valid, int vec) {
-  if (vec && valid >= 4) {
-    if constexpr (sizeof(TOut) == 2) {
-      uint2 o;
-      reinterpret_cast<__nv_bfloat162*>(&o)[0] = __floats2bfloat162_rn(y[0], y[1]);
-      reinterpret_cast<__nv_bfloat162*>(&o)[1] = __floats2bfloat162_rn(y[2], y[3]);
-      *reinterpret_cast<uint2*>(dst) = o;
-    } else {
-      *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < valid) dst[e] = from_f32<TOut>(y[e]);
-  }
-}
-
-template <typename TOut>
-__global__ void __launch_bounds__(kThreads)
+template <typename TOut, int kReaders>
+__global__ void __launch_bounds__(64 + 32 * kReaders)
 linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, TOut* out, long long ldo,
                         const Scales scales, const Shape g) {
   pdl_trigger();
+  constexpr int kThreads = 64 + 32 * kReaders;
   extern __shared__ __align__(1024) unsigned char smem[];
   const unsigned smem_base = tc::smem_u32(smem);
   const bool misaligned = (smem_base & 1023u) != 0;   // never seen; refuse rather than compute garbage
@@ -109,6 +108,12 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
       tc::tma_load_2d(smem_base + s * stage_bytes, &map_w, (kb0 + s) * BK, n0, full_bar(s));
     }
   }
+  // what the sums are multiplied by is fetched under the copies: a channel's scale in its thread, later every row's in shared memory
+  const int cols = min(g.bn, g.M - m0);  // rows of x in this tile
+  const int quarter = warp & 3;          // a warp may only touch lanes [32 * (warp % 4), +32) of tensor memory
+  const int rows_mine = BM / csize;      // channels that this CTA adds up
+  const int n = n0 + (csize > 1 ? rank * rows_mine + (int)threadIdx.x % rows_mine : quarter * 32 + lane);
+  const float sw = n < g.N ? scales.sw[n] : 0.f;
   pdl_wait();
   if (warp == 1) {
     tc::tmem_alloc(tc::smem_u32(tmem_slot), g.tmem_cols);
@@ -125,35 +130,48 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
   const unsigned tmem_base = *tmem_slot;
   if (csize > 1) tc::cluster_arrive();   // phase 0: "this CTA runs"; waited for before anyone writes into it
 
+  float* sx_s = reinterpret_cast<float*>(smem + g.scale_offset);
+  if (warp >= 2) {
+    for (int c = threadIdx.x - 64; c < g.bn; c += 32 * kReaders) sx_s[c] = c < cols ? scales.sx[m0 + c] : 0.f;
+    asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kReaders) : "memory");      // the warps that read results
+  }
+  const float b = scales.bias && n < g.N ? scales.bias[n] : 0.f;
+
   bool ok = true;
   if (warp == 0) {
-    if (lane == 0) {
-      for (int kb = g.stages; kb < nkb; ++kb) {
-        const int s = kb % g.stages;
-        if (!wait_on(empty_bar(s), (unsigned)((kb / g.stages) - 1) & 1, abort_flag, 1)) break;
+    const bool leader = tc::elect_one();
+    Ring at;
+    for (int kb = g.stages; kb < nkb; ++kb, at.next(g.stages)) {
+      const int s = at.stage;
+      if (!wait_on(empty_bar(s), at.parity, abort_flag, 1)) break;
+      if (leader) {
         tc::mbar_expect_tx(full_bar(s), stage_bytes);
         const unsigned dst = smem_base + s * stage_bytes;
         tc::tma_load_2d(dst, &map_w, (kb0 + kb) * BK, n0, full_bar(s));
         tc::tma_load_2d(dst + kBoxBytes, &map_x, (kb0 + kb) * BK, m0, full_bar(s));
       }
+      __syncwarp();
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const unsigned idesc = tc::idesc_i8_s32(BM, g.bn);
-      for (int kb = 0; kb < nkb; ++kb) {
-        const int s = kb % g.stages;
-        ok = wait_on(full_bar(s), (unsigned)(kb / g.stages) & 1, abort_flag, 2);
-        if (!ok) break;
-        tc::fence_after();
-        const unsigned a_addr = smem_base + s * stage_bytes;
-        const unsigned long long da = tc::desc_k_major_sw128(a_addr), db = tc::desc_k_major_sw128(a_addr + kBoxBytes);
+    const bool leader = tc::elect_one();
+    const unsigned idesc = tc::idesc_i8_s32(BM, g.bn);
+    Ring at;
+    for (int kb = 0; kb < nkb; ++kb, at.next(g.stages)) {
+      const int s = at.stage;
+      ok = wait_on(full_bar(s), at.parity, abort_flag, 2);
+      if (!ok) break;
+      tc::fence_after();
+      const unsigned a_addr = smem_base + s * stage_bytes;
+      const unsigned long long da = tc::desc_k_major_sw128(a_addr), db = tc::desc_k_major_sw128(a_addr + kBoxBytes);
+      if (leader) {
 #pragma unroll
         for (int k = 0; k < BK / 32; ++k)   // 32 bytes further along K inside the swizzle row: +2 in the address field
           tc::umma_i8(tmem_base, da + 2ull * k, db + 2ull * k, idesc, (kb | k) != 0 ? 1u : 0u);
         tc::umma_commit(empty_bar(s));
       }
-      if (ok && nkb > 0) tc::umma_commit(acc_full);
+      __syncwarp();
     }
+    if (leader && ok && nkb > 0) tc::umma_commit(acc_full);
   } else if (nkb > 0) {
     ok = wait_on(acc_full, 0, abort_flag, 3);
     tc::fence_after();
@@ -162,23 +180,20 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     __syncwarp();
     tc::cluster_wait();                  // phase 0
     if (g.recv_offset == 0) {            // deposits go over the ring: every CTA's products have read theirs first
-      __syncthreads();                   // (warps 0 and 1 come here before the products are done, warps 2-5 after)
+      __syncthreads();                   // (warps 0 and 1 come here before the products are done, the others after)
       tc::cluster_arrive();
       tc::cluster_wait();
     }
-  } else if (g.recv_offset == 0) {
-    __syncthreads();
   }
-  const int cols = min(g.bn, g.M - m0);  // rows of x in this tile
-  const unsigned recv = smem_base + g.recv_offset;
+  const int ld = g.bn + 4;               // words of a row of deposits: eight lanes' 16 bytes then lie in different banks
   if (warp >= 2) {
-    const int quarter = warp & 3;        // a warp may only touch lanes [32 * (warp % 4), +32)
     const unsigned tmem_row = tmem_base + ((unsigned)(quarter * 32) << 16);
-    const unsigned mine = (unsigned)(rank * g.cols_per_owner) * (BM * 4) + (quarter * 32 + lane) * 4;
-    int owner = 0, local = 0;
-    unsigned dst = csize > 1 ? tc::map_to_rank(recv, 0) : recv;
+    const int row = quarter * 32 + lane;
+    unsigned dst = 0;
+    if (csize > 1)
+      dst = tc::map_to_rank(smem_base + g.recv_offset, row / rows_mine) + (unsigned)((rank * rows_mine + row % rows_mine) * ld) * 4;
 #pragma unroll 1
-    for (int c0 = 0; c0 < cols; c0 += 16) {
+    for (int c0 = 16 * ((warp - 2) >> 2); c0 < cols; c0 += 4 * kReaders) {
       unsigned v[16];
       if (nkb > 0 && ok) {
         tc::tmem_ld16(tmem_row + (unsigned)c0, v);
@@ -187,14 +202,17 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = 0u;
       }
+      if (csize > 1) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if (c0 + e >= cols) break;
-        asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(dst + mine + (unsigned)local * (BM * 4)), "r"(v[e]) : "memory");
-        if (++local == g.cols_per_owner) {
-          local = 0;
-          ++owner;
-          if (owner < csize) dst = tc::map_to_rank(recv, owner);
+        for (int e = 0; e < 16; e += 4)
+          if (c0 + e < cols) asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};\n"
+                       ::"r"(dst + (unsigned)(c0 + e) * 4), "r"(v[e]), "r"(v[e + 1]), "r"(v[e + 2]), "r"(v[e + 3]) : "memory");
+      } else if (n < g.N) {
+        TOut* at = out + (size_t)(m0 + c0) * ldo + n;
+#pragma unroll
+        for (int e = 0; e < 16; ++e, at += ldo) {
+          const float y = finish((int)v[e], sx_s[c0 + e], sw, b, scales.bias != nullptr);
+          if (c0 + e < cols) *at = from_f32<TOut>(y);
         }
       }
     }
@@ -204,32 +222,25 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     __syncwarp();
     tc::cluster_arrive();                // this CTA's deposits are made ...
     tc::cluster_wait();                  // ... and so are everybody's; nothing remote is touched after this
-  } else {
-    __syncthreads();
-  }
-  // a warp a column, four rows of w a lane
-  const int n = n0 + 4 * lane, valid = g.N - n;
-  if (valid > 0) {
-    float sw[4], b[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      sw[e] = e < valid ? scales.sw[n + e] : 0.f;
-      b[e] = scales.bias && e < valid ? scales.bias[n + e] : 0.f;
-    }
-    const int first = rank * g.cols_per_owner, last = min(first + g.cols_per_owner, cols);
-    for (int c = first + warp; c < last; c += kThreads / 32) {
-      int4 sum = make_int4(0, 0, 0, 0);
-      for (int q = 0; q < csize; ++q) {
-        const int4 part = *reinterpret_cast<const int4*>(smem + g.recv_offset + (size_t)(q * g.cols_per_owner + c - first) * (BM * 4) + 16 * lane);
-        sum.x += part.x, sum.y += part.y, sum.z += part.z, sum.w += part.w;
+    // a channel and four rows of x a thread (rows_mine divides the threads: its channel stays)
+    const int local = (int)threadIdx.x % rows_mine, step = kThreads / rows_mine;
+    const unsigned char* mine = smem + g.recv_offset + (size_t)local * ld * 4;
+    if (n < g.N) {
+#pragma unroll 2
+      for (int c = (int)threadIdx.x / rows_mine * 4; c < cols; c += step * 4) {
+        int4 sum = make_int4(0, 0, 0, 0);
+        for (int q = 0; q < csize; ++q) {
+          const int4 part = *reinterpret_cast<const int4*>(mine + ((size_t)q * rows_mine * ld + c) * 4);
+          sum.x += part.x, sum.y += part.y, sum.z += part.z, sum.w += part.w;
+        }
+        const float4 sx = *reinterpret_cast<const float4*>(sx_s + c);
+        TOut* at = out + (size_t)(m0 + c) * ldo + n;
+        const bool biased = scales.bias != nullptr;
+        *at = from_f32<TOut>(finish(sum.x, sx.x, sw, b, biased));
+        if (c + 1 < cols) at[ldo] = from_f32<TOut>(finish(sum.y, sx.y, sw, b, biased));
+        if (c + 2 < cols) at[2 * ldo] = from_f32<TOut>(finish(sum.z, sx.z, sw, b, biased));
+        if (c + 3 < cols) at[3 * ldo] = from_f32<TOut>(finish(sum.w, sx.w, sw, b, biased));
       }
-      const float sx = scales.sx[m0 + c];
-      float y[4] = {finish(sum.x, sx, sw[0]), finish(sum.y, sx, sw[1]), finish(sum.z, sx, sw[2]), finish(sum.w, sx, sw[3])};
-      if (scales.bias) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = __fadd_rn(y[e], b[e]);
-      }
-      store4(out + (size_t)(m0 + c) * ldo + n, y, valid, g.vec);
     }
   }
   if (*abort_flag && threadIdx.x == 0) {
@@ -253,38 +264,19 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 //   warps 2-9  of both CTAs drain their own tensor memory and arrive on the even CTA's "drained" barrier
 constexpr int kEpilogueWarps = 8;
 constexpr int kPairThreads = 64 + 32 * kEpilogueWarps;
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 5;
 constexpr int kPairStageBytes = 2 * kBoxBytes;
-constexpr int kPairBarOffset = kPairStages * kPairStageBytes;       // full, empty, acc_full[2], acc_empty[2], tmem slot, abort
+constexpr int kBufferBytes = 32 * 128;                              // a warp's results on their way out: 32 rows of 128 bytes
+constexpr int kPairBufferOffset = kPairStages * kPairStageBytes;
+constexpr int kPairScaleOffset = kPairBufferOffset + kEpilogueWarps * kBufferBytes;      // per warp 128 channels' scales, then biases
+constexpr int kPairBarOffset = kPairScaleOffset + kEpilogueWarps * 2 * 128 * 4;  // full, empty, acc_full[2], acc_empty[2], tmem slot, abort
 constexpr int kPairSmem = kPairBarOffset + (2 * kPairStages + 4) * 8 + 16 + 1024;
 
 template <typename TOut>
-__device__ __forceinline__ void store32(TOut* dst, const float (&a)[32], int valid) {
-  if (valid >= 32 && (((uintptr_t)dst) & 15) == 0) {
-    if constexpr (sizeof(TOut) == 2) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint4 o;
-        __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o2[e] = __floats2bfloat162_rn(a[q * 8 + 2 * e], a[q * 8 + 2 * e + 1]);
-        reinterpret_cast<uint4*>(dst)[q] = o;
-      }
-    } else {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) reinterpret_cast<float4*>(dst)[q] = make_float4(a[q * 4], a[q * 4 + 1], a[q * 4 + 2], a[q * 4 + 3]);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (e < valid) dst[e] = from_f32<TOut>(a[e]);
-  }
-}
-
-template <typename TOut>
 __global__ void __launch_bounds__(kPairThreads)
-linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, TOut* out, long long ldo,
-                        const Scales scales, int M, int N, int num_kb) {
+linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                        const __grid_constant__ CUtensorMap map_out, TOut* out, long long ldo, const Scales scales, int M, int N, int num_kb,
+                        int tma_out) {
   pdl_start();
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -325,26 +317,31 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
   const unsigned tmem_base = *tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0) {
-      long long it = 0;
-      bool ok = true;
-      for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
-        const int m0 = (tile % m_tiles) * 256 + (int)rank * 128, n0 = (tile / m_tiles) * 256 + (int)rank * 128;
-        for (int kb = 0; kb < num_kb; ++kb, ++it) {
-          const int s = (int)(it % kPairStages);
-          if (it >= kPairStages && !wait_on(empty_bar(s), (unsigned)((it / kPairStages) - 1) & 1, abort_flag, 11)) { ok = false; break; }
+    const bool leader = tc::elect_one();
+    Ring at;
+    int ahead = kPairStages;                         // stages that have not been used yet
+    bool ok = true;
+    for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+      const int m0 = (tile % m_tiles) * 256 + (int)rank * 128, n0 = (tile / m_tiles) * 256 + (int)rank * 128;
+      for (int kb = 0; kb < num_kb; ++kb, at.next(kPairStages)) {
+        const int s = at.stage;
+        if (ahead > 0) --ahead;
+        else if (!wait_on(empty_bar(s), at.parity ^ 1, abort_flag, 11)) { ok = false; break; }
+        if (leader) {
           if (rank == 0) tc::mbar_expect_tx(full_bar(s), 2 * kPairStageBytes);
           const unsigned counted_on = tc::map_to_rank(full_bar(s), 0);
           const unsigned dst = smem_base + s * kPairStageBytes;
           tc::tma_load_2d_pair(dst, &map_x, kb * BK, m0, counted_on);
           tc::tma_load_2d_pair(dst + kBoxBytes, &map_w, kb * BK, n0, counted_on);
         }
+        __syncwarp();
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      const bool leader = tc::elect_one();
       constexpr unsigned idesc = tc::idesc_i8_s32(256, 256);
-      long long it = 0;
+      Ring at;
       int local = 0;
       bool ok = true;
       for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local) {
@@ -355,59 +352,118 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
           tc::fence_after();
         }
         const unsigned tmem_acc = tmem_base + (unsigned)(a * 256);
-        for (int kb = 0; kb < num_kb; ++kb, ++it) {
-          const int s = (int)(it % kPairStages);
-          ok = wait_on(full_bar(s), (unsigned)(it / kPairStages) & 1, abort_flag, 12);
+        for (int kb = 0; kb < num_kb; ++kb, at.next(kPairStages)) {
+          const int s = at.stage;
+          ok = wait_on(full_bar(s), at.parity, abort_flag, 12);
           if (!ok) break;
           tc::fence_after();
           const unsigned a_addr = smem_base + s * kPairStageBytes;
           const unsigned long long da = tc::desc_k_major_sw128(a_addr), db = tc::desc_k_major_sw128(a_addr + kBoxBytes);
+          if (leader) {
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k)
-            tc::umma_i8_pair(tmem_acc, da + 2ull * k, db + 2ull * k, idesc, (kb | k) != 0 ? 1u : 0u);
-          tc::umma_commit_pair(empty_bar(s), 3);
+            for (int k = 0; k < BK / 32; ++k)
+              tc::umma_i8_pair(tmem_acc, da + 2ull * k, db + 2ull * k, idesc, (kb | k) != 0 ? 1u : 0u);
+            tc::umma_commit_pair(empty_bar(s), 3);
+          }
+          __syncwarp();
         }
-        if (ok) tc::umma_commit_pair(acc_full_bar(a), 3);
+        if (leader && ok) tc::umma_commit_pair(acc_full_bar(a), 3);
+        __syncwarp();
       }
     }
   } else {
     const int quarter = warp & 3;            // a warp may only touch lanes [32 * (warp % 4), +32)
     const int part = (warp - 2) >> 2;        // the two warps of a quarter take half of the columns each
+    constexpr int kCols = 128 / (int)sizeof(TOut);             // columns of a row of the buffer
+    unsigned char* buffer = smem + kPairBufferOffset + (warp - 2) * kBufferBytes;
+    float* sw_s = reinterpret_cast<float*>(smem + kPairScaleOffset) + (warp - 2) * 256;
+    float* b_s = sw_s + 128;
+    const bool biased = scales.bias != nullptr;
     int local = 0;
+    // the next tile's scales are asked for a tile ahead: where sums are short the results, not the products, take the time
+    float next_sx, next_sw[4], next_b[4];
+    auto ask = [&](int tile) {
+      const int m = (tile % m_tiles) * 256 + (int)rank * 128 + quarter * 32 + lane, n0 = (tile / m_tiles) * 256 + part * 128 + lane;
+      next_sx = tile < num_tiles && m < M ? scales.sx[m] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool there = tile < num_tiles && n0 + 32 * i < N;
+        next_sw[i] = there ? scales.sw[n0 + 32 * i] : 0.f;
+        next_b[i] = there && scales.bias ? scales.bias[n0 + 32 * i] : 0.f;
+      }
+    };
+    ask(pair);
     for (int tile = pair; tile < num_tiles; tile += num_pairs, ++local) {
       const int a = local & 1;
-      const int row = (tile % m_tiles) * 256 + (int)rank * 128 + quarter * 32 + lane, n0 = (tile / m_tiles) * 256 + part * 128;
-      const float sx = row < M ? scales.sx[row] : 0.f;
+      const int m0 = (tile % m_tiles) * 256 + (int)rank * 128 + quarter * 32, n0 = (tile / m_tiles) * 256 + part * 128;
+      const float sx = next_sx;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sw_s[32 * i + lane] = next_sw[i];
+        b_s[32 * i + lane] = next_b[i];
+      }
+      __syncwarp();
+      ask(tile + num_pairs);
       if (!wait_on(acc_full_bar(a), (unsigned)(local >> 1) & 1, abort_flag, 13)) break;
       tc::fence_after();
       const unsigned tmem_acc = tmem_base + (unsigned)(a * 256 + part * 128) + ((unsigned)(quarter * 32) << 16);
 #pragma unroll 1
-      for (int c = 0; c < 128; c += 32) {
-        if (n0 + c >= N) break;                      // the same for the whole warp
-        unsigned v[32];
-        float y[32];
-        tc::tmem_ld32(tmem_acc + (unsigned)c, v);
+      for (int c = 0; c < 128; c += kCols) {
+        unsigned v[kCols];
+#pragma unroll
+        for (int h = 0; h < kCols; h += 32) tc::tmem_ld32(tmem_acc + (unsigned)(c + h), *reinterpret_cast<unsigned(*)[32]>(v + h));
         tc::tmem_ld_wait();
-        if (n0 + c + 32 <= N) {
+        if (c + kCols == 128) {                      // all of this warp's part is read: the products may fill it again
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive_cluster(tc::map_to_rank(acc_empty_bar(a), 0));
+        }
+        if (n0 + c >= N || m0 >= M) continue;        // the same for the whole warp
+        uint4 row[8];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            y[e] = finish((int)v[e], sx, scales.sw[n0 + c + e]);
-            if (scales.bias) y[e] = __fadd_rn(y[e], scales.bias[n0 + c + e]);
-          }
-        } else {
+        for (int j = 0; j < 8; ++j) {
+          constexpr int kEach = 16 / (int)sizeof(TOut);
+          uint4& o = row[j];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int n = n0 + c + e < N ? n0 + c + e : N - 1;
-            y[e] = finish((int)v[e], sx, scales.sw[n]);
-            if (scales.bias) y[e] = __fadd_rn(y[e], scales.bias[n]);
+          for (int e = 0; e < kEach; e += 2) {
+            const int at = j * kEach + e;
+            const float2 sw = *reinterpret_cast<const float2*>(sw_s + c + at);
+            const float2 b = *reinterpret_cast<const float2*>(b_s + c + at);
+            const float y0 = finish((int)v[at], sx, sw.x, b.x, biased), y1 = finish((int)v[at + 1], sx, sw.y, b.y, biased);
+            if constexpr (sizeof(TOut) == 2) reinterpret_cast<__nv_bfloat162*>(&o)[e / 2] = __floats2bfloat162_rn(y0, y1);
+            else reinterpret_cast<float2*>(&o)[e / 2] = make_float2(y0, y1);
           }
         }
-        if (row < M) store32(out + (size_t)row * ldo + n0 + c, y, N - (n0 + c));
+        if (lane == 0) tc::bulk_wait<0>();           // the buffer's last contents are on their way
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)                  // 16 bytes at a time, their place turned by the row (the copy's swizzle)
+          *reinterpret_cast<uint4*>(buffer + lane * 128 + ((j ^ (lane & 7)) << 4)) = row[j];
+        if (tma_out) {
+          tc::fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tc::tma_store_2d(&map_out, tc::smem_u32(buffer), n0 + c, m0);
+            tc::bulk_commit();
+          }
+        } else {                                     // rows that do not start on 16-byte borders: a row at a time
+          __syncwarp();
+          const int rows = min(32, M - m0);
+#pragma unroll 4
+          for (int r = 0; r < rows; ++r) {
+            TOut* dst = out + (size_t)(m0 + r) * ldo + n0 + c;
+#pragma unroll
+            for (int h = 0; h < kCols; h += 32) {
+              const int at = h + lane, byte = at * (int)sizeof(TOut);
+              if (n0 + c + at < N)
+                dst[at] = *reinterpret_cast<const TOut*>(buffer + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
+            }
+          }
+          __syncwarp();
+        }
       }
-      tc::fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive_cluster(tc::map_to_rank(acc_empty_bar(a), 0));
     }
+    if (lane == 0) tc::bulk_wait<0, true>();
   }
 
   tc::fence_before();
@@ -436,7 +492,7 @@ int allow_smem(Kernel kernel, int bytes, bool (&done)[64]) {
   return OI_OK;
 }
 
-constexpr int kSmemOfTwo = 110 * 1024, kSmemOfOne = 208 * 1024;      // two CTAs on an SM, or one
+constexpr int kMostStages = 12, kSmemOfTwo = 110 * 1024, kSmemOfOne = 208 * 1024;
 
 template <typename TOut>
 int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
@@ -446,15 +502,17 @@ int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const vo
   g.bn = ceil_div(ceil_div(M, z), 16) * 16;                            // z tiles of x, of equal size
   g.num_kb = ceil_div(K, BK);
   g.kb_per_rank = ceil_div(g.num_kb, c);
-  g.cols_per_owner = ceil_div(g.bn, c);
   g.tmem_cols = g.bn <= 32 ? 32 : g.bn <= 64 ? 64 : g.bn <= 128 ? 128 : 256;
-  const int stage = kBoxBytes + g.bn * BK, recv = c * g.cols_per_owner * BM * 4, budget = g.bn <= 128 ? kSmemOfTwo : kSmemOfOne;
-  const bool own_room = g.bn <= 64;                                    // deposits beside the ring, or over it when it is drained
-  g.stages = (budget - 256 - (own_room ? recv : 0)) / stage;
-  if (g.stages > 8) g.stages = 8;
+  const int stage = kBoxBytes + g.bn * BK, recv = c > 1 ? BM * (g.bn + 4) * 4 : 0;
+  // two CTAs on an SM, where there are more than SMs: one streams while the other ends, the next kernel's included
+  const int budget = (long long)c * z * ceil_div(N, BM) <= oi_sm_count() || g.bn > 128 ? kSmemOfOne : kSmemOfTwo;
+  // deposits beside the ring, or over it when it is drained (a cluster's barrier more) where a ring beside them would be short
+  const bool own_room = recv <= budget - 256 - g.bn * 4 - 3 * stage;
+  g.stages = (budget - 256 - g.bn * 4 - (own_room ? recv : 0)) / stage;
+  if (g.stages > kMostStages) g.stages = kMostStages;
   g.recv_offset = own_room ? g.stages * stage : 0;
-  g.bar_offset = own_room ? g.recv_offset + recv : (g.stages * stage > recv ? g.stages * stage : recv);
-  g.vec = (uintptr_t)out % (4 * sizeof(TOut)) == 0 && (M == 1 || ldo % 4 == 0);
+  g.scale_offset = own_room ? g.recv_offset + recv : (g.stages * stage > recv ? g.stages * stage : recv);
+  g.bar_offset = g.scale_offset + g.bn * 4;
   const int smem = g.bar_offset + 8 * (2 * g.stages + 1) + 16;
   OI_REQUIRE(ceil_div(N, BM) <= 65535, "linear_int8: %d channels are too many for %d rows", N, M);
   CUtensorMap mw, mx;
@@ -462,10 +520,14 @@ int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const vo
   OI_REQUIRE(rc == 0, "linear_int8: tensor map for the weight failed (%d; -1: cuTensorMapEncodeTiled is not available)", rc);
   rc = tc::make_map_2d_i8(&mx, x, M, K, ldx, g.bn);
   OI_REQUIRE(rc == 0, "linear_int8: tensor map for x failed (%d)", rc);
-  auto kernel = linear_int8_rows_kernel<TOut>;
-  static bool allowed[64];
-  if ((rc = allow_smem(kernel, 227 * 1024, allowed))) return rc;
-  oi_launch_cluster(kernel, dim3(c, ceil_div(N, BM), z), kThreads, smem, s, c, mw, mx, out, ldo, scales, g);
+  auto go = [&](auto kernel, int threads, bool (&allowed)[64]) {
+    if (int bad = allow_smem(kernel, 227 * 1024, allowed)) return bad;
+    oi_launch_cluster(kernel, dim3(c, ceil_div(N, BM), z), threads, smem, s, c, mw, mx, out, ldo, scales, g);
+    return (int)OI_OK;
+  };
+  static bool few[64], more[64];
+  rc = g.bn <= kFewColumns ? go(linear_int8_rows_kernel<TOut, 4>, 192, few) : go(linear_int8_rows_kernel<TOut, 8>, 320, more);
+  if (rc) return rc;
   OI_CHECK_LAUNCH();
   return OI_OK;
 }
@@ -478,30 +540,52 @@ int launch_pair(TOut* out, long long ldo, const void* x, long long ldx, const vo
   OI_REQUIRE(rc == 0, "linear_int8: tensor map for x failed (%d; -1: cuTensorMapEncodeTiled is not available)", rc);
   rc = tc::make_map_2d_i8(&mw, w, N, K, ldw, BM);
   OI_REQUIRE(rc == 0, "linear_int8: tensor map for the weight failed (%d)", rc);
+  const bool tma_out = (uintptr_t)out % 16 == 0 && ldo * sizeof(TOut) % 16 == 0;
+  CUtensorMap mo = mx;
+  if (tma_out && (rc = tc::make_map_2d_out(&mo, out, sizeof(TOut) == 4, M, N, ldo, 32))) OI_REQUIRE(false, "linear_int8: tensor map for the result failed (%d)", rc);
   auto kernel = linear_int8_pair_kernel<TOut>;
   static bool allowed[64];
   if ((rc = allow_smem(kernel, kPairSmem, allowed))) return rc;
   const long long tiles = (long long)ceil_div(M, 256) * ceil_div(N, 256);
   OI_REQUIRE(tiles < (1LL << 31), "linear_int8: %d rows of %d results are too many", M, N);
   const int most = oi_sm_count() / 2, pairs = tiles < most ? (int)tiles : most;
-  oi_launch_cluster(kernel, 2 * pairs, kPairThreads, kPairSmem, s, 2, mx, mw, out, ldo, scales, M, N, ceil_div(K, BK));
+  oi_launch_cluster(kernel, 2 * pairs, kPairThreads, kPairSmem, s, 2, mx, mw, mo, out, ldo, scales, M, N, ceil_div(K, BK), (int)tma_out);
   OI_CHECK_LAUNCH();
   return OI_OK;
 }
 
-constexpr int kRowsMost = 512;
+// What a product takes in us, from what was measured (B200; N 1024 to 24576, K 512 to 12288, 1 to 2,048 rows), to choose a kernel, the
+// tiles of x and the slices of K. Few rows: 2.3 for the launch and what is ahead of the first copy; a stage of 128 bytes of K is 16 KB
+// of w and `cols` rows of x at what one SM takes in; the weight's bytes from memory; results 0.012 a column of the accumulator, or
+// added up over a cluster 0.7 and 0.028 a column. Many rows: 4.5, and for each round of tiles 0.33 a stage, or the 3.2 that a
+// tile's results take.
+float few_rows_us(int M, int N, int num_kb, int c, int z, int sms) {
+  const int cols = ceil_div(M, z), bn = ceil_div(cols, 16) * 16, kb = ceil_div(num_kb, c);
+  const float rounds = (float)(((long long)ceil_div(N, BM) * z * c + sms - 1) / sms);
+  const float stream = rounds * kb * (0.17f + 0.0006f * cols), memory = (float)N * num_kb * BK / 6.4e6f;
+  const float results = c == 1 ? 0.012f * bn : 0.7f + 0.028f * (cols < bn - 12 ? cols : bn);
+  return 2.3f + (stream > memory ? stream : memory) + results * (rounds > 2.f ? rounds - 1.f : 1.f);
+}
+float many_rows_us(int M, int N, int num_kb, int sms) {
+  const long long tiles = (long long)ceil_div(M, 256) * ceil_div(N, 256);
+  const float a_round = 0.33f * num_kb > 3.2f ? 0.33f * num_kb : 3.2f;
+  return 4.5f + (float)((tiles + sms / 2 - 1) / (sms / 2)) * a_round;
+}
 
 template <typename TOut>
 int launch(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
            cudaStream_t s) {
-  if (M > kRowsMost) return launch_pair(out, ldo, x, ldx, w, ldw, scales, M, N, K, s);
-  // slices of K: as many as run at once, each of two stages at least, none empty
-  const int num_kb = ceil_div(K, BK), tiles = ceil_div(N, BM) * ceil_div(M, 256);
-  const int at_once = ceil_div(M, ceil_div(M, 256)) <= 128 ? 264 : 132;     // two CTAs on an SM, or one
-  int c = 1;
-  while (c < 8 && tiles * c < oi_sm_count() && tiles * 2 * c <= at_once && num_kb / (2 * c) >= 2) c *= 2;
-  while (c > 1 && (c - 1) * ((num_kb + c - 1) / c) >= num_kb) c /= 2;
-  return launch_rows(out, ldo, x, ldx, w, ldw, scales, M, N, K, c, ceil_div(M, 256), s);
+  const int num_kb = ceil_div(K, BK), sms = oi_sm_count(), least = ceil_div(M, 256);
+  int best_c = 0, best_z = 0;
+  float best = many_rows_us(M, N, num_kb, sms);
+  if (least <= 16 && ceil_div(N, BM) <= 65535) {
+    for (int z = least; z <= 4 * least + 4 && z <= ceil_div(M, 16); ++z)
+      for (int c = 1; c <= 8 && (c == 1 || (c - 1) * ceil_div(num_kb, c) < num_kb); c *= 2) {     // no slice without a stage
+        const float us = few_rows_us(M, N, num_kb, c, z, sms);
+        if (us < best) best = us, best_c = c, best_z = z;
+      }
+  }
+  return best_c ? launch_rows(out, ldo, x, ldx, w, ldw, scales, M, N, K, best_c, best_z, s) : launch_pair(out, ldo, x, ldx, w, ldw, scales, M, N, K, s);
 }
 
 }  // namespace

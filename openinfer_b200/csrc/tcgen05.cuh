@@ -50,6 +50,14 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, volatil
   return false;
 }
 
+// One lane of a converged warp, chosen by the hardware. Copies and products issued under this, from a loop that the whole warp runs,
+// take their operands from uniform registers as they are; under a test of the lane number each is moved there first.
+__device__ __forceinline__ bool elect_one() {
+  unsigned one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(one));
+  return one != 0;
+}
+
 // the descriptor of a map that a later copy uses: its fetch from memory is on the way before that copy is issued
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
@@ -76,6 +84,20 @@ __device__ __forceinline__ void tma_load_2d_hint(unsigned dst, const CUtensorMap
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;\n"
       ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar), "l"(policy) : "memory");
 }
+// A tile from shared memory to global memory; what lies outside the map is not written. The thread that issues it commits and waits.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, unsigned src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n"
+               ::"l"(map), "r"(c0), "r"(c1), "r"(src) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
+// until at most N of this thread's committed groups still read shared memory (kDone: until their writes are made, too)
+template <int N, bool kDone = false>
+__device__ __forceinline__ void bulk_wait() {
+  if constexpr (kDone) asm volatile("cp.async.bulk.wait_group %0;\n" ::"n"(N) : "memory");
+  else asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory");
+}
+// what this thread wrote to shared memory by plain stores is there for copies issued later
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 __device__ __forceinline__ unsigned long long policy_evict_first() {
   unsigned long long p;
   asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(p));
@@ -290,6 +312,17 @@ inline int make_map_2d_bf16(CUtensorMap* map, const void* base, long long rows, 
   return (int)fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+// rows x cols result matrix (float32 or bfloat16, row stride ld in elements) for stores of box_rows rows of 128 bytes, 128-byte swizzle.
+inline int make_map_2d_out(CUtensorMap* map, void* base, bool f32, long long rows, long long cols, long long ld, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * (f32 ? 4 : 2)};
+  cuuint32_t box[2] = {f32 ? 32u : 64u, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return (int)fn(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr,
+                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 // rows x K 8-bit matrix with row stride ld (bytes, a multiple of 16); boxes of box_rows x 128 bytes, 128-byte swizzle, zeros
 // outside the matrix (K need not be a multiple of anything).
