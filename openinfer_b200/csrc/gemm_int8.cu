@@ -42,7 +42,7 @@ struct Scales {
 // ------------------------------------------------------------------------------------------------
 // Few rows. The product is formed transposed: 128 rows of w are the M side of tcgen05.mma, up to 256 rows of x (a multiple of
 // 16, `bn`) its N side, so a weight byte goes HBM -> TMA -> shared memory -> tensor core, and the accumulator [128 rows of
-// w x bn] lies in tensor memory. Grid (c, tiles of w, tiles of x): a cluster of c CTAs (a power of two) shares one tile, CTA r
+// w x bn] lies in tensor memory. Grid (c, tiles of x, tiles of w; those that share a tile of w run together): a cluster of c CTAs (a power of two) shares one tile, CTA r
 // streaming k blocks [r * kb_per_rank, ...) of it, and adds up: row i of the accumulator (a row of w) belongs to CTA i / (128 / c),
 // into whose shared memory every CTA deposits its partial sums of it.
 //   warp 0     one thread issues the copies; the first ring-full of WEIGHT boxes is requested before the wait for the kernel
@@ -81,7 +81,7 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x, csize = gridDim.x;
-  const int n0 = blockIdx.y * BM, m0 = blockIdx.z * g.bn;
+  const int n0 = blockIdx.z * BM, m0 = blockIdx.y * g.bn;
   const int kb0 = rank * g.kb_per_rank;
   int nkb = min(g.num_kb - kb0, g.kb_per_rank);
   nkb = nkb > 0 ? nkb : 0;
@@ -261,16 +261,19 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 // in its tensor memory, double buffered (512 columns): while the epilogue warps drain one tile the next is formed.
 //   warp 0     of both CTAs loads its own halves, counted on the even CTA's "full" barrier
 //   warp 1     of the even CTA issues the products (M = 256, N = 256, K = 32) for both
-//   warps 2-9  of both CTAs drain their own tensor memory and arrive on the even CTA's "drained" barrier
-constexpr int kEpilogueWarps = 8;
+//   warps 2-17 of both CTAs drain their own tensor memory and arrive on the even CTA's "drained" barrier
+constexpr int kEpilogueWarps = 16;
+constexpr int kParts = kEpilogueWarps / 4;                          // the warps of a quarter of the lanes share its columns
+constexpr int kPartCols = 256 / kParts;
 constexpr int kPairThreads = 64 + 32 * kEpilogueWarps;
 constexpr int kPairStages = 5;
 constexpr int kPairStageBytes = 2 * kBoxBytes;
-constexpr int kBufferBytes = 32 * 128;                              // a warp's results on their way out: 32 rows of 128 bytes
+constexpr int kBufferBytes = 32 * 64;                               // a warp's results on their way out: 32 rows of 64 bytes
 constexpr int kPairBufferOffset = kPairStages * kPairStageBytes;
-constexpr int kPairScaleOffset = kPairBufferOffset + kEpilogueWarps * kBufferBytes;      // per warp 128 channels' scales, then biases
-constexpr int kPairBarOffset = kPairScaleOffset + kEpilogueWarps * 2 * 128 * 4;  // full, empty, acc_full[2], acc_empty[2], tmem slot, abort
+constexpr int kPairScaleOffset = kPairBufferOffset + kEpilogueWarps * kBufferBytes;      // per warp its channels' scales, then biases
+constexpr int kPairBarOffset = kPairScaleOffset + kEpilogueWarps * 2 * kPartCols * 4;  // full, empty, acc_full[2], acc_empty[2], tmem slot, abort
 constexpr int kPairSmem = kPairBarOffset + (2 * kPairStages + 4) * 8 + 16 + 1024;
+static_assert(kPairSmem <= 227 * 1024, "more shared memory than a CTA may have");
 
 template <typename TOut>
 __global__ void __launch_bounds__(kPairThreads)
@@ -373,32 +376,32 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
     }
   } else {
     const int quarter = warp & 3;            // a warp may only touch lanes [32 * (warp % 4), +32)
-    const int part = (warp - 2) >> 2;        // the two warps of a quarter take half of the columns each
-    constexpr int kCols = 128 / (int)sizeof(TOut);             // columns of a row of the buffer
+    const int part = (warp - 2) >> 2;
+    constexpr int kCols = 64 / (int)sizeof(TOut);             // columns of a row of the buffer
     unsigned char* buffer = smem + kPairBufferOffset + (warp - 2) * kBufferBytes;
-    float* sw_s = reinterpret_cast<float*>(smem + kPairScaleOffset) + (warp - 2) * 256;
-    float* b_s = sw_s + 128;
+    float* sw_s = reinterpret_cast<float*>(smem + kPairScaleOffset) + (warp - 2) * 2 * kPartCols;
+    float* b_s = sw_s + kPartCols;
     const bool biased = scales.bias != nullptr;
     int local = 0;
     // the next tile's scales are asked for a tile ahead: where sums are short the results, not the products, take the time
-    float next_sx, next_sw[4], next_b[4];
+    float next_sx, next_sw[kPartCols / 32], next_b[kPartCols / 32];
     auto ask = [&](int tile) {
-      const int m = (tile % m_tiles) * 256 + (int)rank * 128 + quarter * 32 + lane, n0 = (tile / m_tiles) * 256 + part * 128 + lane;
+      const int m = (tile % m_tiles) * 256 + (int)rank * 128 + quarter * 32 + lane, n0 = (tile / m_tiles) * 256 + part * kPartCols + lane;
       next_sx = tile < num_tiles && m < M ? scales.sx[m] : 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kPartCols / 32; ++i) {
         const bool there = tile < num_tiles && n0 + 32 * i < N;
         next_sw[i] = there ? scales.sw[n0 + 32 * i] : 0.f;
-        next_b[i] = there && scales.bias ? scales.bias[n0 + 32 * i] : 0.f;
+        next_b[i] = there && biased ? scales.bias[n0 + 32 * i] : 0.f;
       }
     };
     ask(pair);
     for (int tile = pair; tile < num_tiles; tile += num_pairs, ++local) {
       const int a = local & 1;
-      const int m0 = (tile % m_tiles) * 256 + (int)rank * 128 + quarter * 32, n0 = (tile / m_tiles) * 256 + part * 128;
+      const int m0 = (tile % m_tiles) * 256 + (int)rank * 128 + quarter * 32, n0 = (tile / m_tiles) * 256 + part * kPartCols;
       const float sx = next_sx;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kPartCols / 32; ++i) {
         sw_s[32 * i + lane] = next_sw[i];
         b_s[32 * i + lane] = next_b[i];
       }
@@ -406,39 +409,46 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
       ask(tile + num_pairs);
       if (!wait_on(acc_full_bar(a), (unsigned)(local >> 1) & 1, abort_flag, 13)) break;
       tc::fence_after();
-      const unsigned tmem_acc = tmem_base + (unsigned)(a * 256 + part * 128) + ((unsigned)(quarter * 32) << 16);
+      const unsigned tmem_acc = tmem_base + (unsigned)(a * 256 + part * kPartCols) + ((unsigned)(quarter * 32) << 16);
 #pragma unroll 1
-      for (int c = 0; c < 128; c += kCols) {
+      for (int c = 0; c < kPartCols; c += kCols) {
         unsigned v[kCols];
-#pragma unroll
-        for (int h = 0; h < kCols; h += 32) tc::tmem_ld32(tmem_acc + (unsigned)(c + h), *reinterpret_cast<unsigned(*)[32]>(v + h));
+        if constexpr (kCols == 32) tc::tmem_ld32(tmem_acc + (unsigned)c, v);
+        else tc::tmem_ld16(tmem_acc + (unsigned)c, v);
         tc::tmem_ld_wait();
-        if (c + kCols == 128) {                      // all of this warp's part is read: the products may fill it again
+        if (c + kCols == kPartCols) {                // all of this warp's part is read: the products may fill it again
           tc::fence_before();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive_cluster(tc::map_to_rank(acc_empty_bar(a), 0));
         }
         if (n0 + c >= N || m0 >= M) continue;        // the same for the whole warp
-        uint4 row[8];
+        float y[kCols];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          constexpr int kEach = 16 / (int)sizeof(TOut);
-          uint4& o = row[j];
+        for (int e = 0; e < kCols; e += 4) {
+          const float4 sw = *reinterpret_cast<const float4*>(sw_s + c + e);
+          y[e] = __fmul_rn(__fmul_rn((float)(int)v[e], sx), sw.x), y[e + 1] = __fmul_rn(__fmul_rn((float)(int)v[e + 1], sx), sw.y);
+          y[e + 2] = __fmul_rn(__fmul_rn((float)(int)v[e + 2], sx), sw.z), y[e + 3] = __fmul_rn(__fmul_rn((float)(int)v[e + 3], sx), sw.w);
+        }
+        if (biased) {
 #pragma unroll
-          for (int e = 0; e < kEach; e += 2) {
-            const int at = j * kEach + e;
-            const float2 sw = *reinterpret_cast<const float2*>(sw_s + c + at);
-            const float2 b = *reinterpret_cast<const float2*>(b_s + c + at);
-            const float y0 = finish((int)v[at], sx, sw.x, b.x, biased), y1 = finish((int)v[at + 1], sx, sw.y, b.y, biased);
-            if constexpr (sizeof(TOut) == 2) reinterpret_cast<__nv_bfloat162*>(&o)[e / 2] = __floats2bfloat162_rn(y0, y1);
-            else reinterpret_cast<float2*>(&o)[e / 2] = make_float2(y0, y1);
+          for (int e = 0; e < kCols; e += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(b_s + c + e);
+            y[e] = __fadd_rn(y[e], b.x), y[e + 1] = __fadd_rn(y[e + 1], b.y), y[e + 2] = __fadd_rn(y[e + 2], b.z), y[e + 3] = __fadd_rn(y[e + 3], b.w);
           }
         }
         if (lane == 0) tc::bulk_wait<0>();           // the buffer's last contents are on their way
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 8; ++j)                  // 16 bytes at a time, their place turned by the row (the copy's swizzle)
-          *reinterpret_cast<uint4*>(buffer + lane * 128 + ((j ^ (lane & 7)) << 4)) = row[j];
+        for (int j = 0; j < 4; ++j) {                // 16 bytes at a time, their place turned by the row (the copy's swizzle)
+          uint4 o;
+          if constexpr (sizeof(TOut) == 2) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) reinterpret_cast<__nv_bfloat162*>(&o)[e] = __floats2bfloat162_rn(y[8 * j + 2 * e], y[8 * j + 2 * e + 1]);
+          } else {
+            o = make_uint4(__float_as_uint(y[4 * j]), __float_as_uint(y[4 * j + 1]), __float_as_uint(y[4 * j + 2]), __float_as_uint(y[4 * j + 3]));
+          }
+          *reinterpret_cast<uint4*>(buffer + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = o;
+        }
         if (tma_out) {
           tc::fence_async_smem();
           __syncwarp();
@@ -446,17 +456,26 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
             tc::tma_store_2d(&map_out, tc::smem_u32(buffer), n0 + c, m0);
             tc::bulk_commit();
           }
-        } else {                                     // rows that do not start on 16-byte borders: a row at a time
+        } else {
+          // Rows that do not start on 16-byte borders: two rows at a time, four bytes a lane. A row of bfloat16 may start between two
+          // four-byte borders: its pairs are then put together from neighbours' words, its first and last number stored alone.
           __syncwarp();
-          const int rows = min(32, M - m0);
+          const int half = lane >> 4, word = lane & 15, left = min(kCols, N - (n0 + c));
+          const unsigned char* from = buffer + half * 64 + (word & 3) * 4;
+          TOut* dst = out + (size_t)(m0 + half) * ldo + n0 + c;
 #pragma unroll 4
-          for (int r = 0; r < rows; ++r) {
-            TOut* dst = out + (size_t)(m0 + r) * ldo + n0 + c;
-#pragma unroll
-            for (int h = 0; h < kCols; h += 32) {
-              const int at = h + lane, byte = at * (int)sizeof(TOut);
-              if (n0 + c + at < N)
-                dst[at] = *reinterpret_cast<const TOut*>(buffer + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
+          for (int i = 0; i < 16; ++i, dst += 2 * ldo) {
+            const unsigned own = *reinterpret_cast<const unsigned*>(from + i * 128 + (((word >> 2) ^ (i & 3)) << 4));
+            const bool live = m0 + 2 * i + half < M;
+            if constexpr (sizeof(TOut) == 4) {
+              if (live && word < left) dst[word] = __uint_as_float(own);
+            } else {
+              const unsigned next = __shfl_down_sync(0xffffffffu, own, 1);
+              const int odd = (int)((uintptr_t)dst >> 1) & 1, at = 2 * word + odd;
+              const unsigned two = odd ? __byte_perm(own, next, 0x5432) : own;
+              if (live && at + 1 < left) *reinterpret_cast<unsigned*>(dst + at) = two;
+              else if (live && at < left) dst[at] = __ushort_as_bfloat16((unsigned short)two);
+              if (live && odd && word == 0) dst[0] = __ushort_as_bfloat16((unsigned short)own);
             }
           }
           __syncwarp();
@@ -494,6 +513,10 @@ int allow_smem(Kernel kernel, int bytes, bool (&done)[64]) {
 
 constexpr int kMostStages = 12, kSmemOfTwo = 110 * 1024, kSmemOfOne = 208 * 1024;
 
+// result rows that start on 16-byte borders can be copied out by TMA
+template <typename TOut>
+bool rows_on_borders(const TOut* out, long long ldo) { return (uintptr_t)out % 16 == 0 && ldo * sizeof(TOut) % 16 == 0; }
+
 template <typename TOut>
 int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
                 int c, int z, cudaStream_t s) {
@@ -505,7 +528,7 @@ int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const vo
   g.tmem_cols = g.bn <= 32 ? 32 : g.bn <= 64 ? 64 : g.bn <= 128 ? 128 : 256;
   const int stage = kBoxBytes + g.bn * BK, recv = c > 1 ? BM * (g.bn + 4) * 4 : 0;
   // two CTAs on an SM, where there are more than SMs: one streams while the other ends, the next kernel's included
-  const int budget = (long long)c * z * ceil_div(N, BM) <= oi_sm_count() || g.bn > 128 ? kSmemOfOne : kSmemOfTwo;
+  const int budget = (long long)c * z * ceil_div(N, BM) <= (c == 8 ? 96 : oi_sm_count()) || g.bn > 128 ? kSmemOfOne : kSmemOfTwo;
   // deposits beside the ring, or over it when it is drained (a cluster's barrier more) where a ring beside them would be short
   const bool own_room = recv <= budget - 256 - g.bn * 4 - 3 * stage;
   g.stages = (budget - 256 - g.bn * 4 - (own_room ? recv : 0)) / stage;
@@ -522,7 +545,7 @@ int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const vo
   OI_REQUIRE(rc == 0, "linear_int8: tensor map for x failed (%d)", rc);
   auto go = [&](auto kernel, int threads, bool (&allowed)[64]) {
     if (int bad = allow_smem(kernel, 227 * 1024, allowed)) return bad;
-    oi_launch_cluster(kernel, dim3(c, ceil_div(N, BM), z), threads, smem, s, c, mw, mx, out, ldo, scales, g);
+    oi_launch_cluster(kernel, dim3(c, z, ceil_div(N, BM)), threads, smem, s, c, mw, mx, out, ldo, scales, g);
     return (int)OI_OK;
   };
   static bool few[64], more[64];
@@ -540,7 +563,7 @@ int launch_pair(TOut* out, long long ldo, const void* x, long long ldx, const vo
   OI_REQUIRE(rc == 0, "linear_int8: tensor map for x failed (%d; -1: cuTensorMapEncodeTiled is not available)", rc);
   rc = tc::make_map_2d_i8(&mw, w, N, K, ldw, BM);
   OI_REQUIRE(rc == 0, "linear_int8: tensor map for the weight failed (%d)", rc);
-  const bool tma_out = (uintptr_t)out % 16 == 0 && ldo * sizeof(TOut) % 16 == 0;
+  const bool tma_out = rows_on_borders(out, ldo);
   CUtensorMap mo = mx;
   if (tma_out && (rc = tc::make_map_2d_out(&mo, out, sizeof(TOut) == 4, M, N, ldo, 32))) OI_REQUIRE(false, "linear_int8: tensor map for the result failed (%d)", rc);
   auto kernel = linear_int8_pair_kernel<TOut>;
@@ -554,21 +577,25 @@ int launch_pair(TOut* out, long long ldo, const void* x, long long ldx, const vo
   return OI_OK;
 }
 
-// What a product takes in us, from what was measured (B200; N 1024 to 24576, K 512 to 12288, 1 to 2,048 rows), to choose a kernel, the
-// tiles of x and the slices of K. Few rows: 2.3 for the launch and what is ahead of the first copy; a stage of 128 bytes of K is 16 KB
-// of w and `cols` rows of x at what one SM takes in; the weight's bytes from memory; results 0.012 a column of the accumulator, or
-// added up over a cluster 0.7 and 0.028 a column. Many rows: 4.5, and for each round of tiles 0.33 a stage, or the 3.2 that a
-// tile's results take.
+// What a product takes in us, from what was measured (B200; N 128 to 32,000, K 128 to 16,000, 1 to 4,096 rows), to choose a kernel, the
+// tiles of x and the slices of K.
+// Few rows: a stage of 128 bytes of K is 16 KB of w and `cols` rows of x at what one SM takes in, for as many CTAs as an SM has to
+// run; the weight's bytes come from memory; every round of CTAs costs 2.3 around its first copy and its results, 0.012 a column of
+// the accumulator, or added up over a cluster 0.7 and 0.028 a column. Clusters of four and eight do not fill the SMs (35 of four: two
+// rounds). Many rows: 4.5, and for each round of tiles 0.33 a stage, or what a tile's results take: 3.2, and 5.5 where result rows do
+// not start on 16-byte borders.
 float few_rows_us(int M, int N, int num_kb, int c, int z, int sms) {
-  const int cols = ceil_div(M, z), bn = ceil_div(cols, 16) * 16, kb = ceil_div(num_kb, c);
-  const float rounds = (float)(((long long)ceil_div(N, BM) * z * c + sms - 1) / sms);
-  const float stream = rounds * kb * (0.17f + 0.0006f * cols), memory = (float)N * num_kb * BK / 6.4e6f;
-  const float results = c == 1 ? 0.012f * bn : 0.7f + 0.028f * (cols < bn - 12 ? cols : bn);
-  return 2.3f + (stream > memory ? stream : memory) + results * (rounds > 2.f ? rounds - 1.f : 1.f);
+  const int cols = ceil_div(M, z), bn = ceil_div(cols, 16) * 16, kb = ceil_div(num_kb, c), at_once = c == 8 ? sms * 2 / 3 : c == 4 ? sms - 20 : sms;
+  const long long ctas = (long long)ceil_div(N, BM) * z * c;
+  const int on_an_sm = ctas <= at_once || bn > 128 ? 1 : 2;
+  const float rounds = (float)((ctas + at_once * on_an_sm - 1) / (at_once * on_an_sm));
+  const float stream = (float)((ctas + at_once - 1) / at_once) * kb * (0.185f + 0.0005f * cols), memory = (float)N * num_kb * BK / 6.4e6f;
+  const float results = c > 1 ? 0.7f + 0.028f * (cols < bn - 12 ? cols : bn) : (bn > 128 ? 0.02f : 0.012f) * bn;
+  return rounds * (2.3f + results * on_an_sm) + (stream > memory ? stream : memory);
 }
-float many_rows_us(int M, int N, int num_kb, int sms) {
+float many_rows_us(int M, int N, int num_kb, bool on_borders, int sms) {
   const long long tiles = (long long)ceil_div(M, 256) * ceil_div(N, 256);
-  const float a_round = 0.33f * num_kb > 3.2f ? 0.33f * num_kb : 3.2f;
+  const float products = 0.33f * num_kb, results = on_borders ? 3.2f : 5.5f, a_round = products > results ? products : results;
   return 4.5f + (float)((tiles + sms / 2 - 1) / (sms / 2)) * a_round;
 }
 
@@ -577,7 +604,7 @@ int launch(TOut* out, long long ldo, const void* x, long long ldx, const void* w
            cudaStream_t s) {
   const int num_kb = ceil_div(K, BK), sms = oi_sm_count(), least = ceil_div(M, 256);
   int best_c = 0, best_z = 0;
-  float best = many_rows_us(M, N, num_kb, sms);
+  float best = many_rows_us(M, N, num_kb, rows_on_borders(out, ldo), sms);
   if (least <= 16 && ceil_div(N, BM) <= 65535) {
     for (int z = least; z <= 4 * least + 4 && z <= ceil_div(M, 16); ++z)
       for (int c = 1; c <= 8 && (c == 1 || (c - 1) * ceil_div(num_kb, c) < num_kb); c *= 2) {     // no slice without a stage
