@@ -147,11 +147,11 @@ template <typename T>
 struct GateRow {
   const T* x;
   long long ldx;
-  int block, act, whole;     // whole: all gates, then all ups
+  int block, act, shift;     // shift: of a block that is a power of two; -1: all gates, then all ups; -2: any other
   static constexpr bool kNorm = false;
   struct Raw { Eight<T> gate, up; };
   __device__ __forceinline__ void begin(long long r) { x += r * ldx; }
-  __device__ __forceinline__ const T* at(int d) const { return x + (whole ? d : d / block * block + d); }
+  __device__ __forceinline__ const T* at(int d) const { return x + d + (shift >= 0 ? d >> shift << shift : shift == -1 ? 0 : d / block * block); }
   __device__ __forceinline__ void fetch(int d, Raw& raw) const {
     raw.gate.load(at(d));
     raw.up.load(at(d) + block);
@@ -164,21 +164,25 @@ struct GateRow {
   __device__ __forceinline__ float again(int d) const { return glu_act<true>(to_f32(at(d)[0]), to_f32(at(d)[block]), act, 0.f); }
 };
 
-// A row in registers, UNITS times eight numbers a thread, read once: by a warp (kWarps: rows of up to 1,024 numbers, eight rows a
-// block) or by a block. kVec: 16 bytes a load, eight neighbours a thread; else neighbours lie in neighbouring threads and the bytes
+// A row in registers, UNITS times eight numbers a thread, read once: by LANES of a warp (rows of up to 1,024 numbers, several rows a
+// block) or, LANES 0, by a block. kVec: 16 bytes a load, eight neighbours a thread; else neighbours lie in neighbouring threads and the bytes
 // are put together in shared memory. One exchange between the warps: the largest magnitude and a norm's sum of squares at
 // once. How a row is shared out goes by its length alone, so that a row's result does not depend on how many there are.
-template <typename Row, bool kVec, int UNITS, bool kWarps>
-__global__ void __launch_bounds__(kWarps || UNITS == 1 ? 256 : 512)
+template <typename Row, bool kVec, int UNITS, int LANES>
+__global__ void __launch_bounds__(LANES || UNITS == 1 ? 256 : UNITS == 2 ? 768 : 512)
 rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows, int cols) {
   pdl_start();
   extern __shared__ __align__(16) unsigned char bytes[];
   __shared__ float part_squares[32];
   __shared__ unsigned part_most[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long r = kWarps ? (long long)blockIdx.x * 8 + warp : blockIdx.x;
-  if (kWarps && r >= rows) return;
-  const int me = kWarps ? lane : threadIdx.x, step = kWarps ? 32 : blockDim.x;
+  constexpr int kRows = LANES ? 256 / LANES : 1;
+  long long r = (long long)blockIdx.x * kRows + (LANES ? threadIdx.x / (LANES ? LANES : 1) : 0);
+  const bool live = r < rows;
+  if (LANES && !live) r = rows - 1;                  // reads and writes nothing, but takes part in what its warp does together
+  const int me = LANES ? threadIdx.x % (LANES ? LANES : 1) : threadIdx.x, step = LANES ? LANES : blockDim.x;
+  const int row_cols = cols;
+  if (LANES && !live) cols = 0;
   row.begin(r);
   q += r * ldq;
 
@@ -213,9 +217,17 @@ rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows
   }
 #pragma unroll
   for (int i = 0; i < UNITS * 8; ++i) most = max(most, magnitude(y[i / 8][i % 8]));
-  most = __reduce_max_sync(0xffffffffu, most);
-  if constexpr (Row::kNorm) squares = warp_sum(squares);
-  if constexpr (!kWarps) {
+  if constexpr (LANES > 0 && LANES < 32) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if constexpr (Row::kNorm) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+    }
+  } else {
+    most = __reduce_max_sync(0xffffffffu, most);
+    if constexpr (Row::kNorm) squares = warp_sum(squares);
+  }
+  if constexpr (LANES == 0) {
     if (lane == 0) {
       part_most[warp] = most;
       part_squares[warp] = squares;
@@ -226,9 +238,9 @@ rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows
     if constexpr (Row::kNorm) squares = warp_sum(lane < warps ? part_squares[lane] : 0.f);
   }
   float common = 1.f;
-  if constexpr (Row::kNorm) common = rsqrtf(squares / (float)cols + row.eps);
+  if constexpr (Row::kNorm) common = rsqrtf(squares / (float)row_cols + row.eps);
   const RowScale s(most, common);
-  if (me == 0) scales[r] = s.scale;
+  if (me == 0 && (!LANES || live)) scales[r] = s.scale;
   if constexpr (kVec) {
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
@@ -242,13 +254,13 @@ rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows
       }
     }
   } else {
-    unsigned char* mine = bytes + (kWarps ? warp * 1024 : 0);
+    unsigned char* mine = bytes + (LANES ? threadIdx.x / (LANES ? LANES : 1) * (LANES * UNITS * 8) : 0);
 #pragma unroll
     for (int i = 0; i < UNITS * 8; ++i) {
       const int d = me + i * step;
       if (d < cols) mine[d] = (unsigned char)(s.byte(y[i / 8][i % 8]) & s.keep);
     }
-    if constexpr (kWarps) __syncwarp();
+    if constexpr (LANES > 0) __syncwarp();
     else __syncthreads();
     for (int d = me * 16; d < cols; d += step * 16) {
       if (d + 16 <= cols) *reinterpret_cast<uint4*>(q + d) = *reinterpret_cast<const uint4*>(mine + d);
@@ -288,19 +300,21 @@ __global__ void __launch_bounds__(1024) long_rows_int8_kernel(Row row, signed ch
 template <typename Row, bool kVec>
 void launch_rows(const Row& row, signed char* q, long long ldq, float* scales, int rows, int cols, cudaStream_t s) {
   const int units = ceil_div(cols, 8);
-  if (units <= 128) {                                  // a warp a row
-    const int grid = ceil_div(rows, 8), smem = kVec ? 0 : 8 * 1024;
-    if (units <= 32) oi_launch(rows_int8_kernel<Row, kVec, 1, true>, grid, 256, smem, s, row, q, ldq, scales, rows, cols);
-    else if (units <= 64) oi_launch(rows_int8_kernel<Row, kVec, 2, true>, grid, 256, smem, s, row, q, ldq, scales, rows, cols);
-    else oi_launch(rows_int8_kernel<Row, kVec, 4, true>, grid, 256, smem, s, row, q, ldq, scales, rows, cols);
+  if (units <= 128) {
+    auto go = [&](auto kernel, int lanes) { oi_launch(kernel, ceil_div(rows, 256 / lanes), 256, kVec ? 0 : 8 * 1024, s, row, q, ldq, scales, rows, cols); };
+    if (units <= 16) go(rows_int8_kernel<Row, kVec, 1, 16>, 16);
+    else if (units <= 32) go(rows_int8_kernel<Row, kVec, 1, 32>, 32);
+    else if (units <= 64) go(rows_int8_kernel<Row, kVec, 2, 32>, 32);
+    else go(rows_int8_kernel<Row, kVec, 4, 32>, 32);
     return;
   }
-  const int smem = kVec ? 0 : ceil_div(cols, 16) * 16;
-  auto threads = [&](int each) { return ceil_div(ceil_div(units, each), 32) * 32; };
-  if (units <= 256) oi_launch(rows_int8_kernel<Row, kVec, 1, false>, rows, threads(1), smem, s, row, q, ldq, scales, rows, cols);
-  else if (units <= 1024) oi_launch(rows_int8_kernel<Row, kVec, 2, false>, rows, threads(2), smem, s, row, q, ldq, scales, rows, cols);
-  else if (units <= 2048) oi_launch(rows_int8_kernel<Row, kVec, 4, false>, rows, threads(4), smem, s, row, q, ldq, scales, rows, cols);
-  else if (units <= 4096) oi_launch(rows_int8_kernel<Row, kVec, 8, false>, rows, threads(8), smem, s, row, q, ldq, scales, rows, cols);
+  auto go = [&](auto kernel, int each) {
+    oi_launch(kernel, rows, ceil_div(ceil_div(units, each), 32) * 32, kVec ? 0 : ceil_div(cols, 16) * 16, s, row, q, ldq, scales, rows, cols);
+  };
+  if (units <= 256) go(rows_int8_kernel<Row, kVec, 1, 0>, 1);
+  else if (units <= (Row::kNorm ? 1024 : 1536)) go(rows_int8_kernel<Row, kVec, 2, 0>, 2);
+  else if (units <= 2048) go(rows_int8_kernel<Row, kVec, 4, 0>, 4);
+  else if (units <= 4096) go(rows_int8_kernel<Row, kVec, 8, 0>, 8);
   else oi_launch(long_rows_int8_kernel<Row>, rows, 1024, 0, s, row, q, ldq, scales, cols);
 }
 
@@ -316,14 +330,17 @@ int launch(const Row& row, bool vec, void* q, long long ldq, float* scales, int 
 
 bool on_borders(const void* p, long long ld, int esize) { return (uintptr_t)p % 16 == 0 && ld * esize % 16 == 0; }
 
-// Sixteen numbers a thread: neighbours where rows start on 16-byte borders, else every 256th. A byte becomes a number without a
-// conversion: with its sign turned it is the last byte of 2^23 + 128 + q.
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(256) dequantize_kernel(T* out, long long ldo, const signed char* q, long long ldq, const float* scales, int cols) {
+// Sixteen numbers a thread: neighbours where rows start on 16-byte borders, else one of each 1 << lanes_log; 256 >> lanes_log rows a
+// block. A byte becomes a number without a conversion: with its sign turned it is the last byte of 2^23 + 128 + q.
+template <typename T, bool kVec, bool kWide>
+__global__ void __launch_bounds__(256) dequantize_kernel(T* out, long long ldo, const signed char* q, long long ldq, const float* scales, int rows,
+                                                         int cols, int lanes_log) {
   pdl_start();
-  const long long r = blockIdx.y;
-  const int first = blockIdx.x * (256 * 16), d = kVec ? first + threadIdx.x * 16 : first + threadIdx.x;
-  if (d >= cols) return;
+  if constexpr (kWide) lanes_log = 8;
+  const int lanes = 1 << lanes_log, lane = threadIdx.x & (lanes - 1), step = kVec ? 1 : lanes;
+  const long long r = ((long long)blockIdx.x << (8 - lanes_log)) + (threadIdx.x >> lanes_log);
+  const int d = blockIdx.y * (lanes * 16) + (kVec ? lane * 16 : lane);
+  if (r >= rows || d >= cols) return;
   const float scale = scales[r];
   out += r * ldo;
   q += r * ldq;
@@ -341,24 +358,25 @@ __global__ void __launch_bounds__(256) dequantize_kernel(T* out, long long ldo, 
       o.store(out + d + 8 * h);
     }
   } else {
-    constexpr int kStep = kVec ? 1 : 256;
     signed char v[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = d + e * kStep < cols ? q[d + e * kStep] : 0;
+    for (int e = 0; e < 16; ++e) v[e] = d + e * step < cols ? q[d + e * step] : 0;
 #pragma unroll
     for (int e = 0; e < 16; ++e)
-      if (d + e * kStep < cols) out[d + e * kStep] = from_f32<T>((float)v[e] * scale);
+      if (d + e * step < cols) out[d + e * step] = from_f32<T>((float)v[e] * scale);
   }
 }
 
 template <typename T>
 int launch_dequantize(T* out, long long ldo, const signed char* q, long long ldq, const float* scales, int rows, int cols, cudaStream_t s) {
-  const bool vec = on_borders(out, rows > 1 ? ldo : 0, sizeof(T));
-  for (long long r = 0; r < rows; r += 65535) {        // one launch, but for more rows than a grid has
-    const dim3 grid(ceil_div(cols, 256 * 16), (unsigned)(rows - r < 65535 ? rows - r : 65535));
-    if (vec) oi_launch(dequantize_kernel<T, true>, grid, 256, 0, s, out + r * ldo, ldo, q + r * ldq, ldq, scales + r, cols);
-    else oi_launch(dequantize_kernel<T, false>, grid, 256, 0, s, out + r * ldo, ldo, q + r * ldq, ldq, scales + r, cols);
-  }
+  int lanes_log = 0;
+  while (lanes_log < 8 && 16 << lanes_log < cols) ++lanes_log;
+  const dim3 grid(ceil_div(rows, 256 >> lanes_log), ceil_div(cols, 16 << lanes_log));
+  OI_REQUIRE(grid.y <= 65535, "dequantize_int8: rows of %d numbers are too long", cols);
+  const bool vec = on_borders(out, rows > 1 ? ldo : 0, sizeof(T)), wide = lanes_log == 8;
+  auto go = [&](auto kernel) { oi_launch(kernel, grid, 256, 0, s, out, ldo, q, ldq, scales, rows, cols, lanes_log); };
+  if (vec) wide ? go(dequantize_kernel<T, true, true>) : go(dequantize_kernel<T, true, false>);
+  else wide ? go(dequantize_kernel<T, false, true>) : go(dequantize_kernel<T, false, false>);
   OI_CHECK_LAUNCH();
   return OI_OK;
 }
@@ -410,9 +428,12 @@ OI_API int oi_silu_mul_int8(void* q, long long ldq, float* scales, const void* g
   OI_REQUIRE(act == OI_ACT_SILU || act == OI_ACT_GELU_TANH, "silu_mul_int8: unknown activation code %d", act);
   if (rows == 0) return OI_OK;
   cudaStream_t s = (cudaStream_t)stream;
+  int shift = block == inter ? -1 : -2;
+  if (shift == -2 && (block & (block - 1)) == 0)
+    for (shift = 0; 1 << shift < block; ++shift) {}
   const bool vec = block % 8 == 0 && on_borders(gate_up, ldx, dtype == OI_F32 ? 4 : 2);
-  if (dtype == OI_F32) return launch(GateRow<float>{(const float*)gate_up, ldx, block, act, block == inter}, vec, q, ldq, scales, rows, inter, s);
-  return launch(GateRow<bf16>{(const bf16*)gate_up, ldx, block, act, block == inter}, vec, q, ldq, scales, rows, inter, s);
+  if (dtype == OI_F32) return launch(GateRow<float>{(const float*)gate_up, ldx, block, act, shift}, vec, q, ldq, scales, rows, inter, s);
+  return launch(GateRow<bf16>{(const bf16*)gate_up, ldx, block, act, shift}, vec, q, ldq, scales, rows, inter, s);
 }
 
 // out[r, :] = round(q[r, :] * scales[r]) (row stride ldo elements)
