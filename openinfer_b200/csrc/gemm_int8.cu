@@ -529,8 +529,9 @@ int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const vo
   const int stage = kBoxBytes + g.bn * BK, recv = c > 1 ? BM * (g.bn + 4) * 4 : 0;
   // two CTAs on an SM, where there are more than SMs: one streams while the other ends, the next kernel's included
   const int budget = (long long)c * z * ceil_div(N, BM) <= (c == 8 ? 96 : oi_sm_count()) || g.bn > 128 ? kSmemOfOne : kSmemOfTwo;
-  // deposits beside the ring, or over it when it is drained (a cluster's barrier more) where a ring beside them would be short
-  const bool own_room = recv <= budget - 256 - g.bn * 4 - 3 * stage;
+  // deposits beside the ring, or over it when it is drained (a cluster's barrier more) where a ring beside them would be short (264 rows, N
+  // 4096, K 12288, c 2: three stages beside them 23.4 us, six under them 19.7)
+  const bool own_room = recv <= budget - 256 - g.bn * 4 - (g.kb_per_rank < 5 ? g.kb_per_rank : 5) * stage;
   g.stages = (budget - 256 - g.bn * 4 - (own_room ? recv : 0)) / stage;
   if (g.stages > kMostStages) g.stages = kMostStages;
   g.recv_offset = own_room ? g.stages * stage : 0;
@@ -570,7 +571,7 @@ int launch_pair(TOut* out, long long ldo, const void* x, long long ldx, const vo
   static bool allowed[64];
   if ((rc = allow_smem(kernel, kPairSmem, allowed))) return rc;
   const long long tiles = (long long)ceil_div(M, 256) * ceil_div(N, 256);
-  OI_REQUIRE(tiles < (1LL << 31), "linear_int8: %d rows of %d results are too many", M, N);
+  OI_REQUIRE(tiles < (1LL << 30), "linear_int8: %d rows of %d results are too many", M, N);
   const int most = oi_sm_count() / 2, pairs = tiles < most ? (int)tiles : most;
   oi_launch_cluster(kernel, 2 * pairs, kPairThreads, kPairSmem, s, 2, mx, mw, mo, out, ldo, scales, M, N, ceil_div(K, BK), (int)tma_out);
   OI_CHECK_LAUNCH();
@@ -622,12 +623,14 @@ int launch(TOut* out, long long ldo, const void* x, long long ldx, const void* w
 // launch in plain stream order (oi_launch_fence).
 OI_API int oi_linear_int8(void* out, int out_dtype, long long ldo, const void* x, long long ldx, const float* sx, const void* w,
                           long long ldw, const float* sw, const float* bias, int M, int N, int K, void* stream) {
-  OI_REQUIRE(M >= 0 && N >= 0 && K >= 1 && K <= 131071, "linear_int8: bad sizes M=%d N=%d K=%d (K: 1 to 131071)", M, N, K);
+  constexpr int kMost = (1 << 30);
+  OI_REQUIRE(M >= 0 && M <= kMost && N >= 0 && N <= kMost && K >= 1 && K <= 131071, "linear_int8: bad sizes M=%d N=%d K=%d (K: 1 to 131071)", M, N, K);
   OI_REQUIRE(out_dtype == OI_F32 || out_dtype == OI_BF16, "linear_int8: unknown output dtype code %d", out_dtype);
   if (M == 0 || N == 0) return OI_OK;
   OI_REQUIRE(ldx % 16 == 0 && ldw % 16 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0 && ldx >= K && ldw >= K,
              "linear_int8: rows of x and w must start on 16-byte borders");
   OI_REQUIRE(M == 1 || ldo >= N, "linear_int8: result rows of %d that start %lld apart", N, ldo);
+  if (M == 1) ldo = ceil_div(N, 16) * 16LL;      // one row's stride means nothing
   const Scales scales = {sx, sw, bias};
   cudaStream_t s = (cudaStream_t)stream;
   if (out_dtype == OI_F32) return launch((float*)out, ldo, x, ldx, w, ldw, scales, M, N, K, s);

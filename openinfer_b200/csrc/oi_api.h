@@ -312,11 +312,11 @@ OI_API int oi_gemm_few_status(int* status);
 
 // rows_int8.cu: rows as 8-bit integers with a float32 scale each (q = round(y * (127 / max |y|)), scale = max |y| / 127)
 OI_API int oi_quantize_int8(void* q, long long ldq, float* scales, const void* x, int dtype, long long ldx, int rows, int cols,
-                            void* stream);
+                            int early, void* stream);
 OI_API int oi_rmsnorm_int8(void* q, long long ldq, float* scales, void* x, long long ldx, const void* delta, long long ldd, int dtype,
-                           const void* w, int w_dtype, int rows, int cols, float eps, float w_offset, void* stream);
+                           const void* w, int w_dtype, int rows, int cols, float eps, float w_offset, int early, void* stream);
 OI_API int oi_silu_mul_int8(void* q, long long ldq, float* scales, const void* gate_up, int dtype, long long ldx, int rows, int inter,
-                            int block, int act, void* stream);
+                            int block, int act, int early, void* stream);
 OI_API int oi_dequantize_int8(void* out, int dtype, long long ldo, const void* q, long long ldq, const float* scales, int rows, int cols,
                               void* stream);
 

@@ -165,13 +165,15 @@ struct GateRow {
 };
 
 // A row in registers, UNITS times eight numbers a thread, read once: by LANES of a warp (rows of up to 1,024 numbers, several rows a
-// block) or, LANES 0, by a block. kVec: 16 bytes a load, eight neighbours a thread; else neighbours lie in neighbouring threads and the bytes
+// block) or, LANES 0, by a block. early: the next kernel may be scheduled while this one runs (not where the rows may be those of a
+// weight: a product fetches its weight before it waits). kVec: 16 bytes a load, eight neighbours a thread; else neighbours lie in neighbouring threads and the bytes
 // are put together in shared memory. One exchange between the warps: the largest magnitude and a norm's sum of squares at
 // once. How a row is shared out goes by its length alone, so that a row's result does not depend on how many there are.
 template <typename Row, bool kVec, int UNITS, int LANES>
 __global__ void __launch_bounds__(LANES || UNITS == 1 ? 256 : UNITS == 2 ? 768 : 512)
-rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows, int cols) {
-  pdl_start();
+rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows, int cols, int early) {
+  if (early) pdl_trigger();
+  pdl_wait();
   extern __shared__ __align__(16) unsigned char bytes[];
   __shared__ float part_squares[32];
   __shared__ unsigned part_most[32];
@@ -272,8 +274,9 @@ rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows
 
 // Rows longer than 512 threads hold in registers: one block a row, read once for each thing that is asked of all of it.
 template <typename Row>
-__global__ void __launch_bounds__(1024) long_rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int cols) {
-  pdl_start();
+__global__ void __launch_bounds__(1024) long_rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int cols, int early) {
+  if (early) pdl_trigger();
+  pdl_wait();
   __shared__ float part_squares[32];
   __shared__ unsigned part_most[32];
   const long long r = blockIdx.x;
@@ -298,10 +301,10 @@ __global__ void __launch_bounds__(1024) long_rows_int8_kernel(Row row, signed ch
 }
 
 template <typename Row, bool kVec>
-void launch_rows(const Row& row, signed char* q, long long ldq, float* scales, int rows, int cols, cudaStream_t s) {
+void launch_rows(const Row& row, signed char* q, long long ldq, float* scales, int rows, int cols, int early, cudaStream_t s) {
   const int units = ceil_div(cols, 8);
   if (units <= 128) {
-    auto go = [&](auto kernel, int lanes) { oi_launch(kernel, ceil_div(rows, 256 / lanes), 256, kVec ? 0 : 8 * 1024, s, row, q, ldq, scales, rows, cols); };
+    auto go = [&](auto kernel, int lanes) { oi_launch(kernel, ceil_div(rows, 256 / lanes), 256, kVec ? 0 : 8 * 1024, s, row, q, ldq, scales, rows, cols, early); };
     if (units <= 16) go(rows_int8_kernel<Row, kVec, 1, 16>, 16);
     else if (units <= 32) go(rows_int8_kernel<Row, kVec, 1, 32>, 32);
     else if (units <= 64) go(rows_int8_kernel<Row, kVec, 2, 32>, 32);
@@ -309,21 +312,21 @@ void launch_rows(const Row& row, signed char* q, long long ldq, float* scales, i
     return;
   }
   auto go = [&](auto kernel, int each) {
-    oi_launch(kernel, rows, ceil_div(ceil_div(units, each), 32) * 32, kVec ? 0 : ceil_div(cols, 16) * 16, s, row, q, ldq, scales, rows, cols);
+    oi_launch(kernel, rows, ceil_div(ceil_div(units, each), 32) * 32, kVec ? 0 : ceil_div(cols, 16) * 16, s, row, q, ldq, scales, rows, cols, early);
   };
   if (units <= 256) go(rows_int8_kernel<Row, kVec, 1, 0>, 1);
   else if (units <= (Row::kNorm ? 1024 : 1536)) go(rows_int8_kernel<Row, kVec, 2, 0>, 2);
   else if (units <= 2048) go(rows_int8_kernel<Row, kVec, 4, 0>, 4);
   else if (units <= 4096) go(rows_int8_kernel<Row, kVec, 8, 0>, 8);
-  else oi_launch(long_rows_int8_kernel<Row>, rows, 1024, 0, s, row, q, ldq, scales, cols);
+  else oi_launch(long_rows_int8_kernel<Row>, rows, 1024, 0, s, row, q, ldq, scales, cols, early);
 }
 
 // vec: everything that a row is read from starts on 16-byte borders, and the next row's too, whether there is one or not: one row
 // of a matrix is shared out among the threads as it is among others
 template <typename Row>
-int launch(const Row& row, bool vec, void* q, long long ldq, float* scales, int rows, int cols, cudaStream_t s) {
-  if (vec) launch_rows<Row, true>(row, (signed char*)q, ldq, scales, rows, cols, s);
-  else launch_rows<Row, false>(row, (signed char*)q, ldq, scales, rows, cols, s);
+int launch(const Row& row, bool vec, void* q, long long ldq, float* scales, int rows, int cols, int early, cudaStream_t s) {
+  if (vec) launch_rows<Row, true>(row, (signed char*)q, ldq, scales, rows, cols, early, s);
+  else launch_rows<Row, false>(row, (signed char*)q, ldq, scales, rows, cols, early, s);
   OI_CHECK_LAUNCH();
   return OI_OK;
 }
@@ -372,7 +375,7 @@ int launch_dequantize(T* out, long long ldo, const signed char* q, long long ldq
   int lanes_log = 0;
   while (lanes_log < 8 && 16 << lanes_log < cols) ++lanes_log;
   const dim3 grid(ceil_div(rows, 256 >> lanes_log), ceil_div(cols, 16 << lanes_log));
-  OI_REQUIRE(grid.y <= 65535, "dequantize_int8: rows of %d numbers are too long", cols);
+  OI_REQUIRE(grid.y <= 65535, "dequantize_int8: bad sizes rows=%d cols=%d", rows, cols);
   const bool vec = on_borders(out, rows > 1 ? ldo : 0, sizeof(T)), wide = lanes_log == 8;
   auto go = [&](auto kernel) { oi_launch(kernel, grid, 256, 0, s, out, ldo, q, ldq, scales, rows, cols, lanes_log); };
   if (vec) wide ? go(dequantize_kernel<T, true, true>) : go(dequantize_kernel<T, true, false>);
@@ -382,7 +385,7 @@ int launch_dequantize(T* out, long long ldo, const signed char* q, long long ldq
 }
 
 int check_rows(const char* what, const void* q, long long ldq, const float* scales, int rows, int cols) {
-  OI_REQUIRE(rows >= 0 && cols >= 1, "%s: bad sizes rows=%d cols=%d", what, rows, cols);
+  OI_REQUIRE(rows >= 0 && cols >= 1 && cols <= (1 << 30), "%s: bad sizes rows=%d cols=%d", what, rows, cols);
   OI_REQUIRE(rows == 0 || (q && scales), "%s: a pointer is missing", what);
   OI_REQUIRE(rows <= 1 || ldq >= cols, "%s: rows of %d that start %lld apart", what, cols, ldq);
   return OI_OK;
@@ -390,21 +393,23 @@ int check_rows(const char* what, const void* q, long long ldq, const float* scal
 
 }  // namespace
 
-// q[r, :] (row stride ldq bytes) and scales[r] of x[r, :] (row stride ldx elements)
-OI_API int oi_quantize_int8(void* q, long long ldq, float* scales, const void* x, int dtype, long long ldx, int rows, int cols, void* stream) {
+// q[r, :] (row stride ldq bytes) and scales[r] of x[r, :] (row stride ldx elements). early 0: what is written may be a weight, which
+// kernels behind this one read before their wait.
+OI_API int oi_quantize_int8(void* q, long long ldq, float* scales, const void* x, int dtype, long long ldx, int rows, int cols, int early,
+                            void* stream) {
   if (int rc = check_rows("quantize_int8", q, ldq, scales, rows, cols)) return rc;
   OI_REQUIRE(dtype == OI_F32 || dtype == OI_BF16, "quantize_int8: unknown dtype code %d", dtype);
   if (rows == 0) return OI_OK;
   cudaStream_t s = (cudaStream_t)stream;
   const bool vec = on_borders(x, ldx, dtype == OI_F32 ? 4 : 2);
-  if (dtype == OI_F32) return launch(PlainRow<float>{(const float*)x, ldx}, vec, q, ldq, scales, rows, cols, s);
-  return launch(PlainRow<bf16>{(const bf16*)x, ldx}, vec, q, ldq, scales, rows, cols, s);
+  if (dtype == OI_F32) return launch(PlainRow<float>{(const float*)x, ldx}, vec, q, ldq, scales, rows, cols, early, s);
+  return launch(PlainRow<bf16>{(const bf16*)x, ldx}, vec, q, ldq, scales, rows, cols, early, s);
 }
 
 // The rows of oi_rmsnorm's output, not rounded: x <- round(x + delta) (stored; delta may be null), then
 // x * rsqrt(mean(x^2) + eps) * (w_offset + w). Row strides ldx, ldd in elements.
 OI_API int oi_rmsnorm_int8(void* q, long long ldq, float* scales, void* x, long long ldx, const void* delta, long long ldd, int dtype,
-                           const void* w, int w_dtype, int rows, int cols, float eps, float w_offset, void* stream) {
+                           const void* w, int w_dtype, int rows, int cols, float eps, float w_offset, int early, void* stream) {
   if (int rc = check_rows("rmsnorm_int8", q, ldq, scales, rows, cols)) return rc;
   OI_REQUIRE(dtype == OI_F32 || dtype == OI_BF16, "rmsnorm_int8: unknown dtype code %d", dtype);
   OI_REQUIRE(w_dtype == OI_F32 || w_dtype == OI_BF16, "rmsnorm_int8: unknown weight dtype code %d", w_dtype);
@@ -414,17 +419,17 @@ OI_API int oi_rmsnorm_int8(void* q, long long ldq, float* scales, void* x, long 
   const int esize = dtype == OI_F32 ? 4 : 2;
   const bool vec = on_borders(x, ldx, esize) && (!delta || on_borders(delta, ldd, esize)) && (uintptr_t)w % 16 == 0;
   if (dtype == OI_F32)
-    return launch(NormRow<float>{(float*)x, (const float*)delta, w, ldx, ldd, w_dtype, eps, w_offset}, vec, q, ldq, scales, rows, cols, s);
-  return launch(NormRow<bf16>{(bf16*)x, (const bf16*)delta, w, ldx, ldd, w_dtype, eps, w_offset}, vec, q, ldq, scales, rows, cols, s);
+    return launch(NormRow<float>{(float*)x, (const float*)delta, w, ldx, ldd, w_dtype, eps, w_offset}, vec, q, ldq, scales, rows, cols, early, s);
+  return launch(NormRow<bf16>{(bf16*)x, (const bf16*)delta, w, ldx, ldd, w_dtype, eps, w_offset}, vec, q, ldq, scales, rows, cols, early, s);
 }
 
 // The rows of oi_silu_mul's output, not rounded: act(gate) * up of gate_up [rows, 2 inter] (row stride ldx elements), which lies
 // in blocks of `block` gate values followed by their up values.
 OI_API int oi_silu_mul_int8(void* q, long long ldq, float* scales, const void* gate_up, int dtype, long long ldx, int rows, int inter,
-                            int block, int act, void* stream) {
+                            int block, int act, int early, void* stream) {
   if (int rc = check_rows("silu_mul_int8", q, ldq, scales, rows, inter)) return rc;
   OI_REQUIRE(dtype == OI_F32 || dtype == OI_BF16, "silu_mul_int8: unknown dtype code %d", dtype);
-  OI_REQUIRE(inter <= (1 << 30) && block >= 1 && inter % block == 0, "silu_mul_int8: %d values in blocks of %d", inter, block);
+  OI_REQUIRE(block >= 1 && inter % block == 0, "silu_mul_int8: %d values in blocks of %d", inter, block);
   OI_REQUIRE(act == OI_ACT_SILU || act == OI_ACT_GELU_TANH, "silu_mul_int8: unknown activation code %d", act);
   if (rows == 0) return OI_OK;
   cudaStream_t s = (cudaStream_t)stream;
@@ -432,14 +437,14 @@ OI_API int oi_silu_mul_int8(void* q, long long ldq, float* scales, const void* g
   if (shift == -2 && (block & (block - 1)) == 0)
     for (shift = 0; 1 << shift < block; ++shift) {}
   const bool vec = block % 8 == 0 && on_borders(gate_up, ldx, dtype == OI_F32 ? 4 : 2);
-  if (dtype == OI_F32) return launch(GateRow<float>{(const float*)gate_up, ldx, block, act, shift}, vec, q, ldq, scales, rows, inter, s);
-  return launch(GateRow<bf16>{(const bf16*)gate_up, ldx, block, act, shift}, vec, q, ldq, scales, rows, inter, s);
+  if (dtype == OI_F32) return launch(GateRow<float>{(const float*)gate_up, ldx, block, act, shift}, vec, q, ldq, scales, rows, inter, early, s);
+  return launch(GateRow<bf16>{(const bf16*)gate_up, ldx, block, act, shift}, vec, q, ldq, scales, rows, inter, early, s);
 }
 
 // out[r, :] = round(q[r, :] * scales[r]) (row stride ldo elements)
 OI_API int oi_dequantize_int8(void* out, int dtype, long long ldo, const void* q, long long ldq, const float* scales, int rows, int cols,
                               void* stream) {
-  OI_REQUIRE(rows >= 0 && cols >= 1, "dequantize_int8: bad sizes rows=%d cols=%d", rows, cols);
+  OI_REQUIRE(rows >= 0 && cols >= 1 && cols <= (1 << 30), "dequantize_int8: bad sizes rows=%d cols=%d", rows, cols);
   OI_REQUIRE(dtype == OI_F32 || dtype == OI_BF16, "dequantize_int8: unknown dtype code %d", dtype);
   OI_REQUIRE(rows <= 1 || ldo >= cols, "dequantize_int8: rows of %d that start %lld apart", cols, ldo);
   if (rows == 0) return OI_OK;

@@ -23,6 +23,7 @@ from . import lib as _lib
 from .lib import KernelError
 from .ops import act_code
 
+MOST = 1 << 30             # rows, and numbers of a row
 ALIGN = 16                 # bytes that the rows of 8-bit operands start on
 MAX_WIDTH = 131071         # the longest sum of products of two 8-bit integers that a 32-bit integer holds: 128 * 128 * 131071 < 2^31
 
@@ -35,28 +36,29 @@ class Int8Rows(NamedTuple):
     scales: torch.Tensor
 
 
-# The checks below ask a tensor for each thing once and hand on what they found: at a few rows a call's time is the host's.
+# At a few rows a call's time is the host's. So a tensor is asked for each thing once, one test covers all that may be wrong, and what
+# exactly it was is found out behind it.
 
 def _float_rows(t: torch.Tensor, what: str) -> Tuple[int, int, int, int]:
     """(dtype code, rows, width, row stride) of a matrix of floating rows (any row stride, neighbours next to each other)."""
-    code = _DT.get(t.dtype)
+    code, shape, strides = _DT.get(t.dtype), t.shape, t.stride()
+    if code is not None and len(shape) == 2:
+        rows, width = shape
+        if (strides[1] == 1 and 0 < width <= MOST or width == 1) and rows <= MOST:
+            return code, rows, width, strides[0]
     if code is None:
         raise KernelError(f"{what}: dtype {t.dtype} is not supported (float32 or bfloat16)")
-    shape, strides = t.shape, t.stride()
-    if len(shape) != 2 or shape[1] < 1 or (strides[1] != 1 and shape[1] > 1):
-        raise KernelError(f"{what}: expected rows of at least one number, neighbours next to each other: shape {tuple(shape)}, strides {strides}")
-    return code, shape[0], shape[1], strides[0]
+    raise KernelError(f"{what}: expected rows of at least one number, neighbours next to each other (at most {MOST} of either): shape {tuple(shape)}, strides {strides}")
 
 
-def _int8_rows(held: Int8Rows, what: str) -> Tuple[int, int, int, int, int, int]:
+def _int8_rows(values: torch.Tensor, scales: torch.Tensor, what: str) -> Tuple[int, int, int, int, int, int]:
     """(address, row stride, rows, width, address of the scales, device index) of 8-bit rows. The stride of one row is its width
     rounded up to what rows start on (it means nothing then)."""
-    values, scales = held
     if values.dtype != torch.int8 or scales.dtype != torch.float32:
         raise KernelError(f"{what}: 8-bit rows are int8 with float32 scales: {values.dtype}, {scales.dtype}")
     shape, strides = values.shape, values.stride()
-    if len(shape) != 2 or shape[1] < 1 or (strides[1] != 1 and shape[1] > 1):
-        raise KernelError(f"{what}: expected rows of at least one integer, neighbours next to each other: shape {tuple(shape)}, strides {strides}")
+    if len(shape) != 2 or not 0 < shape[1] <= MOST or (strides[1] != 1 and shape[1] > 1) or shape[0] > MOST:
+        raise KernelError(f"{what}: expected rows of at least one integer, neighbours next to each other (at most {MOST} of either): shape {tuple(shape)}, strides {strides}")
     rows, width = shape
     address, stride = values.data_ptr(), strides[0] if rows > 1 else -(-width // ALIGN) * ALIGN
     if address % ALIGN or stride % ALIGN or stride < width:
@@ -76,19 +78,21 @@ def _cuda(device: int, what: str) -> None:
 
 def empty_rows(rows: int, width: int, device) -> Int8Rows:
     """Room for rows of 8-bit integers."""
-    room = -(-width // ALIGN) * ALIGN
-    return Int8Rows(torch.empty_strided((rows, width), (room, 1), dtype=torch.int8, device=device),
-                    torch.empty(rows, dtype=torch.float32, device=device))
+    values = (torch.empty_strided((rows, width), (-(-width // ALIGN) * ALIGN, 1), dtype=torch.int8, device=device) if width % ALIGN
+              else torch.empty(rows, width, dtype=torch.int8, device=device))
+    return Int8Rows(values, torch.empty(rows, dtype=torch.float32, device=device))
 
 
 def _room(out: Optional[Int8Rows], x: torch.Tensor, rows: int, width: int, device: int, what: str):
     """(8-bit rows, their address, row stride, address of the scales)"""
+    if device < 0:
+        _cuda(device, what)
     if out is None:
-        out = empty_rows(rows, width, x.device)
-        return out, out.values.data_ptr(), -(-width // ALIGN) * ALIGN, out.scales.data_ptr()
-    address, stride, has_rows, has_width, scales, on = _int8_rows(out, what)
+        out = values, scales = empty_rows(rows, width, x.device)
+        return out, values.data_ptr(), -(-width // ALIGN) * ALIGN, scales.data_ptr()
+    address, stride, has_rows, has_width, scales, on = _int8_rows(*out, what)
     if (has_rows, has_width, on) != (rows, width, device):
-        raise KernelError(f"{what}: room for {(has_rows, has_width)} on {out.values.device}, needed {(rows, width)} on {x.device}")
+        raise KernelError(f"{what}: room for {(has_rows, has_width)} on {out[0].device}, needed {(rows, width)} on {x.device}")
     return out, address, stride, scales
 
 
@@ -103,22 +107,16 @@ def _launch(device: int, what: str, entry, *args) -> None:
         _lib.check(code, what)
 
 
-def _done(L, given: Optional[Int8Rows]) -> None:
-    """Rows written into given memory may be those of a weight, which products fetch ahead: the next launch starts behind this one."""
-    if given is not None:
-        L.oi_launch_fence()
-
-
 def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
     """The rows of ``x`` [rows, width] (float32 or bfloat16, row stride free) as 8-bit integers."""
     code, rows, width, stride = _float_rows(x, "quantize_int8")
     device = x.get_device()
-    _cuda(device, "quantize_int8")
     held, q, ldq, scales = _room(out, x, rows, width, device, "quantize_int8")
     if rows:
         L = _lib.load()
-        _launch(device, "quantize_int8", L.oi_quantize_int8, q, ldq, scales, x.data_ptr(), code, stride, rows, width)
-        _done(L, out)
+        _launch(device, "quantize_int8", L.oi_quantize_int8, q, ldq, scales, x.data_ptr(), code, stride, rows, width, out is None)
+        if out is not None:
+            L.oi_launch_fence()      # it may be a weight's memory, which products fetch ahead: the next launch starts behind this one
     return held
 
 
@@ -128,29 +126,27 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, delta: Op
 
     ``delta``: x <- x + delta first (rounded, stored in x), the norm is of the sum as it is stored."""
     code, rows, width, stride = _float_rows(x, "rmsnorm_int8")
-    device, address = x.get_device(), x.data_ptr()
-    w_code = _DT.get(weight.dtype)
+    device, address, w_code = x.get_device(), x.data_ptr(), _DT.get(weight.dtype)
     if w_code is None or weight.shape != (width,) or not weight.is_contiguous() or weight.get_device() != device:
         raise KernelError(f"rmsnorm_int8: expected a float32 or bfloat16 weight of {width} numbers on {x.device}: {weight.dtype} {tuple(weight.shape)} on {weight.device}")
     d_address = d_stride = 0
     if delta is not None:
-        d_code, d_rows, d_width, d_stride = _float_rows(delta, "rmsnorm_int8 delta")
-        if (d_code, d_rows, d_width, delta.get_device()) != (code, rows, width, device):
+        if delta.dtype != x.dtype or delta.shape != x.shape or delta.get_device() != device:
             raise KernelError(f"rmsnorm_int8: x and delta must share a dtype, a shape and a device: {x.dtype} {tuple(x.shape)} on {x.device}, {delta.dtype} {tuple(delta.shape)} on {delta.device}")
+        d_stride, d_address = _float_rows(delta, "rmsnorm_int8 delta")[3], delta.data_ptr()
         if rows > 1 and stride < width:
             raise KernelError(f"rmsnorm_int8: rows that overlap (row stride {stride}, width {width}) cannot take a sum")
-        d_address = delta.data_ptr()
         size = 2 if code else 4
         if (d_address < address + ((rows - 1) * stride + width) * size and address < d_address + ((rows - 1) * d_stride + width) * size
                 and rows and (d_address, d_stride) != (address, stride)):
             raise KernelError("rmsnorm_int8: x and delta must be the same rows or not overlap")
-    _cuda(device, "rmsnorm_int8")
     held, q, ldq, scales = _room(out, x, rows, width, device, "rmsnorm_int8")
     if rows:
         L = _lib.load()
         _launch(device, "rmsnorm_int8", L.oi_rmsnorm_int8, q, ldq, scales, address, stride, d_address, d_stride, code, weight.data_ptr(),
-                w_code, rows, width, eps, weight_offset)
-        _done(L, out)
+                w_code, rows, width, eps, weight_offset, out is None)
+        if out is not None:
+            L.oi_launch_fence()      # as in quantize_int8
     return held
 
 
@@ -164,12 +160,12 @@ def silu_mul_int8(gate_up: torch.Tensor, block: Optional[int] = None, act: str =
         raise KernelError(f"silu_mul_int8: gate_up of {both} numbers in blocks of {block} gates and {block} ups")
     act_c = act_code(act)
     device = gate_up.get_device()
-    _cuda(device, "silu_mul_int8")
     held, q, ldq, scales = _room(out, gate_up, rows, inter, device, "silu_mul_int8")
     if rows:
         L = _lib.load()
-        _launch(device, "silu_mul_int8", L.oi_silu_mul_int8, q, ldq, scales, gate_up.data_ptr(), code, stride, rows, inter, block, act_c)
-        _done(L, out)
+        _launch(device, "silu_mul_int8", L.oi_silu_mul_int8, q, ldq, scales, gate_up.data_ptr(), code, stride, rows, inter, block, act_c, out is None)
+        if out is not None:
+            L.oi_launch_fence()      # as in quantize_int8
     return held
 
 
@@ -192,7 +188,7 @@ def _results(out: Optional[torch.Tensor], dtype: torch.dtype, rows: int, width: 
 
 def dequantize_int8(rows: Int8Rows, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The numbers that 8-bit rows stand for, rounded once to ``dtype`` (float32 or bfloat16) or to that of ``out`` (row stride free)."""
-    q, ldq, count, width, scales, device = _int8_rows(rows, "dequantize_int8")
+    q, ldq, count, width, scales, device = _int8_rows(*rows, "dequantize_int8")
     out, code, stride = _results(out, dtype, count, width, rows[0], device, "dequantize_int8")
     if count:
         _launch(device, "dequantize_int8", _lib.load().oi_dequantize_int8, out.data_ptr(), code, stride, q, ldq, scales, count, width)
@@ -206,7 +202,7 @@ class Int8Weight:
     fetches its weight while the kernel ahead of it on the stream still runs, but for the first one on each stream. Later
     changes of the weight's tensors (by torch, or through ``out`` of the functions above) are ordered by the stream as ever."""
 
-    __slots__ = ("values", "scales", "channels", "width", "device", "operands", "stream")
+    __slots__ = ("values", "scales", "channels", "width", "device", "stream", "_seen", "_operands")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor) -> None:
         if values.dim() != 2 or values.dtype != torch.int8 or scales.shape != values.shape[:1]:
@@ -221,9 +217,18 @@ class Int8Weight:
             values = held
         self.values, self.scales, self.device = values, scales.contiguous(), values.device
         self.channels, self.width = rows, width
-        q, ldq, _, _, scale, device = _int8_rows(Int8Rows(self.values, self.scales), "Int8Weight")
-        self.operands = (q, ldq, scale, device)
         self.stream = None          # of the last product: what wrote the weight is known to be done there
+        self._seen = None
+        self.operands()
+
+    def operands(self):
+        """What ``_int8_rows`` says of the weight; asked again when its tensors have been given other memory."""
+        values, scales = self.values, self.scales
+        seen = (values.data_ptr(), scales.data_ptr(), values.shape, values.stride(), scales.shape)
+        if seen != self._seen:
+            self._operands = _int8_rows(values, scales, "Int8Weight")
+            self._seen, self.stream = seen, None
+        return self._operands
 
     @classmethod
     def quantize(cls, w: torch.Tensor) -> "Int8Weight":
@@ -236,11 +241,10 @@ def linear_int8(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = 
     """x [rows, width] times the weight [channels, width], transposed: sums of 8-bit products exact in 32-bit integers, then
     float32(sum) * x's scale * the channel's scale (+ the channel's ``bias``, float32) and one rounding to ``out_dtype``
     (float32 or bfloat16, or that of ``out`` [rows, channels], whose row stride is free)."""
-    q, ldq, rows, width, scales, device = _int8_rows(x, "linear_int8")
-    w, ldw, w_scales, w_device = weight.operands
-    channels = weight.channels
-    if width != weight.width or device != w_device:
-        raise KernelError(f"linear_int8: rows of {width} on {x[0].device} and a weight of {channels} x {weight.width} on {weight.device}")
+    q, ldq, rows, width, scales, device = _int8_rows(*x, "linear_int8")
+    w, ldw, channels, w_width, w_scales, w_device = weight.operands()
+    if width != w_width or device != w_device:
+        raise KernelError(f"linear_int8: rows of {width} on {x[0].device} and a weight of {channels} x {w_width} on {weight.device}")
     b = 0
     if bias is not None:
         if bias.dtype != torch.float32 or bias.shape != (channels,) or not bias.is_contiguous() or bias.get_device() != device:

@@ -95,9 +95,9 @@ _SIGNATURES = {
     "oi_add2_cast": [P, P, P, P, I, L, P],
     "oi_token_gate": [P, L, I, P, P, I, L, I, I, I, I, P],
     "oi_gemm_stream_glu": [P, I, L, P, L, P, L, I, I, I, I, I, F, P],
-    "oi_quantize_int8": [P, L, P, P, I, L, I, I, P],
-    "oi_rmsnorm_int8": [P, L, P, P, L, P, L, I, P, I, I, I, F, F, P],
-    "oi_silu_mul_int8": [P, L, P, P, I, L, I, I, I, I, P],
+    "oi_quantize_int8": [P, L, P, P, I, L, I, I, I, P],
+    "oi_rmsnorm_int8": [P, L, P, P, L, P, L, I, P, I, I, I, F, F, I, P],
+    "oi_silu_mul_int8": [P, L, P, P, I, L, I, I, I, I, I, P],
     "oi_dequantize_int8": [P, I, L, P, L, P, I, I, P],
     "oi_linear_int8": [P, I, L, P, L, P, P, L, P, P, I, I, I, P],
     "oi_linear_int8_status": [ctypes.POINTER(c_int)],

@@ -49,6 +49,12 @@ def test_floating_rows():
         refused("not on a CUDA device", call, X)
 
 
+def test_more_rows_than_an_entry_point_counts():
+    many = torch.zeros(1, 1).expand(2 ** 31 + 5, 1)
+    refused("at most 1073741824", int8.quantize_int8, many)
+    refused("at most 1073741824", int8.dequantize_int8, int8.Int8Rows(torch.zeros(1, 1, dtype=torch.int8).expand(2 ** 31 + 5, 1), torch.ones(3)))
+
+
 def test_norm():
     def norm(x=X, w=torch.ones(32), **kw):
         int8.rmsnorm_int8(x, w, 1e-6, **kw)
@@ -93,15 +99,18 @@ def test_weight_and_product():
 
 
 @pytest.mark.parametrize("name,args", [
-    ("oi_quantize_int8", (1, 32, 1, 1, 7, 32, 1, 32)),                     # an unknown dtype
-    ("oi_quantize_int8", (1, 32, 1, 1, 0, 32, -1, 32)),
-    ("oi_quantize_int8", (1, 32, 1, 1, 0, 32, 1, 0)),
-    ("oi_quantize_int8", (0, 32, 1, 1, 0, 32, 1, 32)),
-    ("oi_quantize_int8", (1, 16, 1, 1, 0, 32, 2, 32)),                     # rows that overlap
-    ("oi_rmsnorm_int8", (1, 32, 1, 1, 16, 1, 32, 0, 1, 0, 2, 32, 1e-6, 0.0)),
-    ("oi_rmsnorm_int8", (1, 32, 1, 1, 32, 0, 0, 0, 1, 5, 2, 32, 1e-6, 0.0)),
-    ("oi_silu_mul_int8", (1, 32, 1, 1, 0, 64, 1, 32, 5, 1)),
-    ("oi_silu_mul_int8", (1, 32, 1, 1, 0, 64, 1, 32, 32, 9)),
+    ("oi_quantize_int8", (1, 32, 1, 1, 7, 32, 1, 32, 1)),                     # an unknown dtype
+    ("oi_quantize_int8", (1, 32, 1, 1, 0, 32, -1, 32, 1)),
+    ("oi_quantize_int8", (1, 32, 1, 1, 0, 32, 1, 0, 1)),
+    ("oi_quantize_int8", (0, 32, 1, 1, 0, 32, 1, 32, 1)),
+    ("oi_quantize_int8", (1, 16, 1, 1, 0, 32, 2, 32, 1)),                     # rows that overlap
+    ("oi_quantize_int8", (1, 1 << 31, 1, 1, 0, 32, 1, (1 << 30) + 1, 1)),
+    ("oi_dequantize_int8", (1, 0, 1 << 31, 1, 1 << 31, 1, 1, (1 << 30) + 1)),
+    ("oi_linear_int8", (16, 1, 8, 16, 32, 16, 16, 32, 16, 0, (1 << 30) + 1, 8, 32)),
+    ("oi_rmsnorm_int8", (1, 32, 1, 1, 16, 1, 32, 0, 1, 0, 2, 32, 1e-6, 0.0, 1)),
+    ("oi_rmsnorm_int8", (1, 32, 1, 1, 32, 0, 0, 0, 1, 5, 2, 32, 1e-6, 0.0, 1)),
+    ("oi_silu_mul_int8", (1, 32, 1, 1, 0, 64, 1, 32, 5, 1, 1)),
+    ("oi_silu_mul_int8", (1, 32, 1, 1, 0, 64, 1, 32, 32, 9, 1)),
     ("oi_dequantize_int8", (1, 5, 32, 1, 32, 1, 1, 32)),
     ("oi_dequantize_int8", (1, 0, 16, 1, 32, 1, 2, 32)),
     ("oi_linear_int8", (16, 1, 8, 16, 32, 16, 16, 32, 16, 0, 4, 8, 131072)),   # a sum that 32 bits may not hold
