@@ -49,11 +49,11 @@ struct Scales {
 //              ahead (programmatic dependent launch), which may still be writing x
 //   warp 1     allocates tensor memory (behind that wait: a kernel ahead that needs all of it may not have taken its own
 //              yet), one thread issues four products (K = 32) a stage
-//   the others (four, or eight) read the accumulator (one row of w a thread) and deposit, or with c = 1 scale and store; then
+//   the others (four to sixteen) read the accumulator (one row of w a thread) and deposit, or with c = 1 scale and store; then
 //              all warps add up, scale and store.
 // What the results cost shows in the instructions per column: with a column at a time, a branch and a cluster address each, and
 // six warps, 128 columns took 8,000 cycles to deposit and 8,700 to store (N 1024, K 1024, c 1).
-constexpr int kFewColumns = 32;             // up to so many rows of x a tile four warps read results, else eight
+constexpr int kFewColumns = 32, kMoreColumns = 64;      // up to so many rows of x a tile four warps read results, or eight, else sixteen
 
 struct Shape {
   int M, N, num_kb, kb_per_rank, bn, stages, tmem_cols;
@@ -135,7 +135,8 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     for (int c = threadIdx.x - 64; c < g.bn; c += 32 * kReaders) sx_s[c] = c < cols ? scales.sx[m0 + c] : 0.f;
     asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kReaders) : "memory");      // the warps that read results
   }
-  const float b = scales.bias && n < g.N ? scales.bias[n] : 0.f;
+  const bool biased = scales.bias != nullptr;
+  const float b = biased && n < g.N ? scales.bias[n] : 0.f;
 
   bool ok = true;
   if (warp == 0) {
@@ -207,12 +208,19 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         for (int e = 0; e < 16; e += 4)
           if (c0 + e < cols) asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};\n"
                        ::"r"(dst + (unsigned)(c0 + e) * 4), "r"(v[e]), "r"(v[e + 1]), "r"(v[e + 2]), "r"(v[e + 3]) : "memory");
-      } else if (n < g.N) {
-        TOut* at = out + (size_t)(m0 + c0) * ldo + n;
+      } else {
+        float y[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e, at += ldo) {
-          const float y = finish((int)v[e], sx_s[c0 + e], sw, b, scales.bias != nullptr);
-          if (c0 + e < cols) *at = from_f32<TOut>(y);
+        for (int e = 0; e < 16; e += 4) {
+          const float4 sx = *reinterpret_cast<const float4*>(sx_s + c0 + e);
+          y[e] = finish((int)v[e], sx.x, sw, b, biased), y[e + 1] = finish((int)v[e + 1], sx.y, sw, b, biased);
+          y[e + 2] = finish((int)v[e + 2], sx.z, sw, b, biased), y[e + 3] = finish((int)v[e + 3], sx.w, sw, b, biased);
+        }
+        TOut* at = out + (size_t)(m0 + c0) * ldo + n;
+        if (n < g.N) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e, at += ldo)
+            if (c0 + e < cols) *at = from_f32<TOut>(y[e]);
         }
       }
     }
@@ -235,7 +243,6 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         }
         const float4 sx = *reinterpret_cast<const float4*>(sx_s + c);
         TOut* at = out + (size_t)(m0 + c) * ldo + n;
-        const bool biased = scales.bias != nullptr;
         *at = from_f32<TOut>(finish(sum.x, sx.x, sw, b, biased));
         if (c + 1 < cols) at[ldo] = from_f32<TOut>(finish(sum.y, sx.y, sw, b, biased));
         if (c + 2 < cols) at[2 * ldo] = from_f32<TOut>(finish(sum.z, sx.z, sw, b, biased));
@@ -549,8 +556,9 @@ int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const vo
     oi_launch_cluster(kernel, dim3(c, z, ceil_div(N, BM)), threads, smem, s, c, mw, mx, out, ldo, scales, g);
     return (int)OI_OK;
   };
-  static bool few[64], more[64];
-  rc = g.bn <= kFewColumns ? go(linear_int8_rows_kernel<TOut, 4>, 192, few) : go(linear_int8_rows_kernel<TOut, 8>, 320, more);
+  static bool few[64], more[64], most[64];
+  rc = g.bn <= kFewColumns ? go(linear_int8_rows_kernel<TOut, 4>, 192, few)
+       : g.bn <= kMoreColumns ? go(linear_int8_rows_kernel<TOut, 8>, 320, more) : go(linear_int8_rows_kernel<TOut, 16>, 576, most);
   if (rc) return rc;
   OI_CHECK_LAUNCH();
   return OI_OK;
@@ -581,9 +589,9 @@ int launch_pair(TOut* out, long long ldo, const void* x, long long ldx, const vo
 // What a product takes in us, from what was measured (B200; N 128 to 32,000, K 128 to 16,000, 1 to 4,096 rows), to choose a kernel, the
 // tiles of x and the slices of K.
 // Few rows: a stage of 128 bytes of K is 16 KB of w and `cols` rows of x at what one SM takes in, for as many CTAs as an SM has to
-// run; the weight's bytes come from memory; every round of CTAs costs 2.3 around its first copy and its results, 0.012 a column of
-// the accumulator, or added up over a cluster 0.7 and 0.028 a column. Clusters of four and eight do not fill the SMs (35 of four: two
-// rounds). Many rows: 4.5, and for each round of tiles 0.33 a stage, or what a tile's results take: 3.2, and 5.5 where result rows do
+// run; the weight's bytes come from memory; every round of CTAs costs 2.3 around its first copy and its results, 0.006 to 0.008 a column
+// of the accumulator, or added up over a cluster 0.7 and 0.028 a column. Clusters of four and eight do not fill the SMs (35 of four: two
+// rounds). Many rows: 4.5, and for each round of tiles 0.33 a stage, or what a tile's results take: 3.2, and 6.5 where result rows do
 // not start on 16-byte borders.
 float few_rows_us(int M, int N, int num_kb, int c, int z, int sms) {
   const int cols = ceil_div(M, z), bn = ceil_div(cols, 16) * 16, kb = ceil_div(num_kb, c), at_once = c == 8 ? sms * 2 / 3 : c == 4 ? sms - 20 : sms;
@@ -591,12 +599,12 @@ float few_rows_us(int M, int N, int num_kb, int c, int z, int sms) {
   const int on_an_sm = ctas <= at_once || bn > 128 ? 1 : 2;
   const float rounds = (float)((ctas + at_once * on_an_sm - 1) / (at_once * on_an_sm));
   const float stream = (float)((ctas + at_once - 1) / at_once) * kb * (0.185f + 0.0005f * cols), memory = (float)N * num_kb * BK / 6.4e6f;
-  const float results = c > 1 ? 0.7f + 0.028f * (cols < bn - 12 ? cols : bn) : (bn > 128 ? 0.02f : 0.012f) * bn;
+  const float results = c > 1 ? 0.7f + 0.028f * (cols < bn - 12 ? cols : bn) : (bn > 128 ? 0.008f : 0.006f) * bn;
   return rounds * (2.3f + results * on_an_sm) + (stream > memory ? stream : memory);
 }
 float many_rows_us(int M, int N, int num_kb, bool on_borders, int sms) {
   const long long tiles = (long long)ceil_div(M, 256) * ceil_div(N, 256);
-  const float products = 0.33f * num_kb, results = on_borders ? 3.2f : 5.5f, a_round = products > results ? products : results;
+  const float products = 0.33f * num_kb, results = on_borders ? 3.2f : 6.5f, a_round = products > results ? products : results;
   return 4.5f + (float)((tiles + sms / 2 - 1) / (sms / 2)) * a_round;
 }
 
