@@ -223,7 +223,14 @@ def on_device(int8, x, sx):
 # rows on both sides of every size at which another tile is taken; sums that fill a stage, miss it by one, and leave slices empty
 SHAPES = [(1, 1, 1), (1, 128, 128), (1, 5, 16), (2, 33, 31), (3, 130, 129), (8, 256, 127), (15, 1000, 64), (16, 128, 4096), (17, 256, 500), (31, 300, 1024), (32, 1536, 4096),
           (33, 257, 2048), (48, 640, 1000), (64, 1024, 4096), (65, 384, 96), (100, 4096, 777), (127, 129, 8192), (128, 1024, 1024), (129, 999, 2048), (200, 128, 300),
-          (256, 512, 512), (257, 2049, 333), (300, 6144, 256), (512, 513, 1025), (777, 1000, 2001), (1024, 2048, 640), (2050, 300, 4100), (5000, 130, 72), (1, 9000, 14000), (4, 64, 60000)]
+          (256, 512, 512), (257, 2049, 333), (300, 6144, 256), (512, 513, 1025), (777, 1000, 2001), (1024, 2048, 640), (2050, 300, 4100), (5000, 130, 72), (1, 9000, 14000), (4, 64, 60000),
+          # every kernel, number of slices, of warps that read results, and place of the partial sums: few rows by one, two, four and eight CTAs ...
+          (194, 9522, 546), (276, 9555, 408), (137, 13516, 33), (83, 9769, 33), (262, 8322, 134), (427, 6948, 519), (197, 5048, 33), (34, 10895, 37),
+          (99, 5008, 5688), (66, 4827, 4703), (263, 3153, 7355), (3905, 130, 5552), (390, 550, 1747), (20, 3580, 1500),
+          (109, 2548, 5457), (141, 3266, 5385), (33, 2547, 1578), (3097, 47, 3526), (17, 34, 1267), (389, 36, 1449),
+          (99, 815, 13890), (131, 1311, 10041), (1610, 72, 16138), (34, 880, 3675), (394, 42, 899), (1, 33, 917),
+          # ... and many rows, with result rows on 16-byte borders, on four-byte borders, and on none; more tiles than pairs of CTAs
+          (1845, 6736, 139), (444, 15348, 1940), (327, 14293, 2407)]
 
 
 @pytest.mark.parametrize("rows,channels,width", SHAPES)
