@@ -262,50 +262,54 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 }
 
 // ------------------------------------------------------------------------------------------------
-// Many rows. Pairs of CTAs (a cluster of two, cta_group::2) compute 256 x 256 tiles, persistent: pair p works on tiles p, p +
-// pairs, ... (row tiles fastest, so that pairs that run at the same time share tiles of w through L2). The CTA of rank r holds
-// rows [128 r, +128) of the tile's rows of x and of w in its shared memory, and the accumulator of its 128 rows x 256 columns
-// in its tensor memory, double buffered (512 columns): while the epilogue warps drain one tile the next is formed.
-//   warp 0     of both CTAs loads its own halves, counted on the even CTA's "full" barrier
-//   warp 1     of the even CTA issues the products (M = 256, N = 256, K = 32) for both
-//   warps 2-17 of both CTAs drain their own tensor memory and arrive on the even CTA's "drained" barrier
+// Many rows, transposed as above. Pairs of CTAs (a cluster of two, cta_group::2) compute tiles of 256 channels x `bn` rows of x (a
+// multiple of 32 up to 256: rows are shared out evenly over the tiles, so 777 of them need not be 1,024), persistent: pair p
+// works on tiles p, p + pairs, ... (tiles of x fastest, so that pairs that run at the same time share tiles of w through L2).
+// The CTA of rank r holds 128 of the tile's rows of w and half of its rows of x in its shared memory, so a byte of x is fetched
+// once for 256 channels, and the accumulator of its 128 channels x bn columns in its tensor memory, double buffered: while the
+// other warps drain one tile the next is formed.
+//   warp 0      of both CTAs loads its own halves, counted on the even CTA's "full" barrier
+//   warp 1      of the even CTA issues the products (M = 256, N = bn, K = 32) for both
+//   warps 2-17  of both CTAs drain their own tensor memory (32 channels a warp, every fourth group of rows) and arrive on the even
+//               CTA's "drained" barrier. A warp scales 32 channels of a few rows, turns them in shared memory, and a TMA store carries
+//               them out: 4096 x 4096 x 512 takes 16.5 us so (float32 20.8), 19.7 (28.8) with 16-byte stores by the warps.
 constexpr int kEpilogueWarps = 16;
-constexpr int kParts = kEpilogueWarps / 4;                          // the warps of a quarter of the lanes share its columns
-constexpr int kPartCols = 256 / kParts;
+constexpr int kParts = kEpilogueWarps / 4;                          // the warps of a quarter of the lanes share the rows of x
 constexpr int kPairThreads = 64 + 32 * kEpilogueWarps;
-constexpr int kPairStages = 5;
-constexpr int kPairStageBytes = 2 * kBoxBytes;
-constexpr int kBufferBytes = 32 * 64;                               // a warp's results on their way out: 32 rows of 64 bytes
-constexpr int kPairBufferOffset = kPairStages * kPairStageBytes;
-constexpr int kPairScaleOffset = kPairBufferOffset + kEpilogueWarps * kBufferBytes;      // per warp its channels' scales, then biases
-constexpr int kPairBarOffset = kPairScaleOffset + kEpilogueWarps * 2 * kPartCols * 4;  // full, empty, acc_full[2], acc_empty[2], tmem slot, abort
-constexpr int kPairSmem = kPairBarOffset + (2 * kPairStages + 4) * 8 + 16 + 1024;
+constexpr int kBufferBytes = 2048;                                  // a warp's results on their way out: 32 channels of 32 or (float32) 16 rows
+constexpr int kPairMostStages = 8;
+constexpr int kPairRingBytes = 180 * 1024;
+constexpr int kPairBufferOffset = kPairRingBytes;
+constexpr int kPairScaleOffset = kPairBufferOffset + kEpilogueWarps * kBufferBytes;      // per warp the scales of its rows of x
+constexpr int kPairBarOffset = kPairScaleOffset + kEpilogueWarps * (256 / kParts) * 4;   // full, empty, acc_full[2], acc_empty[2], tmem slot, abort
+constexpr int kPairSmem = kPairBarOffset + (2 * kPairMostStages + 4) * 8 + 16 + 1024;
 static_assert(kPairSmem <= 227 * 1024, "more shared memory than a CTA may have");
 
 template <typename TOut>
 __global__ void __launch_bounds__(kPairThreads)
-linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                         const __grid_constant__ CUtensorMap map_out, TOut* out, long long ldo, const Scales scales, int M, int N, int num_kb,
-                        int tma_out) {
+                        int bn, int stages, int tma_out) {
   pdl_start();
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const unsigned smem_base = tc::smem_u32(smem);
   const unsigned bar_base = smem_base + kPairBarOffset;
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
-  auto empty_bar = [&](int s) { return bar_base + 8u * (kPairStages + s); };
-  auto acc_full_bar = [&](int a) { return bar_base + 8u * (2 * kPairStages + a); };
-  auto acc_empty_bar = [&](int a) { return bar_base + 8u * (2 * kPairStages + 2 + a); };
-  unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + kPairBarOffset + (2 * kPairStages + 4) * 8);
+  auto empty_bar = [&](int s) { return bar_base + 8u * (kPairMostStages + s); };
+  auto acc_full_bar = [&](int a) { return bar_base + 8u * (2 * kPairMostStages + a); };
+  auto acc_empty_bar = [&](int a) { return bar_base + 8u * (2 * kPairMostStages + 2 + a); };
+  unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + kPairBarOffset + (2 * kPairMostStages + 4) * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned rank = tc::cluster_ctarank();
   const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
-  const int m_tiles = (M + 255) / 256, num_tiles = m_tiles * ((N + 255) / 256);
+  const int m_tiles = (M + bn - 1) / bn, num_tiles = m_tiles * ((N + 255) / 256);
+  const unsigned stage_bytes = kBoxBytes + (bn / 2) * BK;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kPairStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       tc::mbar_init(full_bar(s), 1);
       tc::mbar_init(empty_bar(s), 1);
     }
@@ -329,20 +333,20 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
   if (warp == 0) {
     const bool leader = tc::elect_one();
     Ring at;
-    int ahead = kPairStages;                         // stages that have not been used yet
+    int ahead = stages;                              // stages that have not been used yet
     bool ok = true;
     for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
-      const int m0 = (tile % m_tiles) * 256 + (int)rank * 128, n0 = (tile / m_tiles) * 256 + (int)rank * 128;
-      for (int kb = 0; kb < num_kb; ++kb, at.next(kPairStages)) {
+      const int m0 = (tile % m_tiles) * bn + (int)rank * (bn / 2), n0 = (tile / m_tiles) * 256 + (int)rank * 128;
+      for (int kb = 0; kb < num_kb; ++kb, at.next(stages)) {
         const int s = at.stage;
         if (ahead > 0) --ahead;
         else if (!wait_on(empty_bar(s), at.parity ^ 1, abort_flag, 11)) { ok = false; break; }
         if (leader) {
-          if (rank == 0) tc::mbar_expect_tx(full_bar(s), 2 * kPairStageBytes);
+          if (rank == 0) tc::mbar_expect_tx(full_bar(s), 2 * stage_bytes);
           const unsigned counted_on = tc::map_to_rank(full_bar(s), 0);
-          const unsigned dst = smem_base + s * kPairStageBytes;
-          tc::tma_load_2d_pair(dst, &map_x, kb * BK, m0, counted_on);
-          tc::tma_load_2d_pair(dst + kBoxBytes, &map_w, kb * BK, n0, counted_on);
+          const unsigned dst = smem_base + s * stage_bytes;
+          tc::tma_load_2d_pair(dst, &map_w, kb * BK, n0, counted_on);
+          tc::tma_load_2d_pair(dst + kBoxBytes, &map_x, kb * BK, m0, counted_on);
         }
         __syncwarp();
       }
@@ -350,7 +354,7 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
   } else if (warp == 1) {
     if (rank == 0) {
       const bool leader = tc::elect_one();
-      constexpr unsigned idesc = tc::idesc_i8_s32(256, 256);
+      const unsigned idesc = tc::idesc_i8_s32(256, bn);
       Ring at;
       int local = 0;
       bool ok = true;
@@ -362,12 +366,12 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
           tc::fence_after();
         }
         const unsigned tmem_acc = tmem_base + (unsigned)(a * 256);
-        for (int kb = 0; kb < num_kb; ++kb, at.next(kPairStages)) {
+        for (int kb = 0; kb < num_kb; ++kb, at.next(stages)) {
           const int s = at.stage;
           ok = wait_on(full_bar(s), at.parity, abort_flag, 12);
           if (!ok) break;
           tc::fence_after();
-          const unsigned a_addr = smem_base + s * kPairStageBytes;
+          const unsigned a_addr = smem_base + s * stage_bytes;
           const unsigned long long da = tc::desc_k_major_sw128(a_addr), db = tc::desc_k_major_sw128(a_addr + kBoxBytes);
           if (leader) {
 #pragma unroll
@@ -382,111 +386,100 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
       }
     }
   } else {
-    const int quarter = warp & 3;            // a warp may only touch lanes [32 * (warp % 4), +32)
+    const int quarter = warp & 3;                    // a warp may only touch lanes [32 * (warp % 4), +32)
     const int part = (warp - 2) >> 2;
-    constexpr int kCols = 64 / (int)sizeof(TOut);             // columns of a row of the buffer
+    constexpr int kTake = kBufferBytes / 32 / (int)sizeof(TOut);      // rows of x at a time
+    constexpr int kTurns = 256 / kTake / kParts;                      // of this warp in a tile
     unsigned char* buffer = smem + kPairBufferOffset + (warp - 2) * kBufferBytes;
-    float* sw_s = reinterpret_cast<float*>(smem + kPairScaleOffset) + (warp - 2) * 2 * kPartCols;
-    float* b_s = sw_s + kPartCols;
+    float* sx_s = reinterpret_cast<float*>(smem + kPairScaleOffset) + (warp - 2) * (256 / kParts);
     const bool biased = scales.bias != nullptr;
     int local = 0;
     // the next tile's scales are asked for a tile ahead: where sums are short the results, not the products, take the time
-    float next_sx, next_sw[kPartCols / 32], next_b[kPartCols / 32];
+    float next_sw, next_b, next_sx[2];
     auto ask = [&](int tile) {
-      const int m = (tile % m_tiles) * 256 + (int)rank * 128 + quarter * 32 + lane, n0 = (tile / m_tiles) * 256 + part * kPartCols + lane;
-      next_sx = tile < num_tiles && m < M ? scales.sx[m] : 0.f;
+      const bool there = tile < num_tiles;
+      const int n = (tile / m_tiles) * 256 + (int)rank * 128 + quarter * 32 + lane;
+      next_sw = there && n < N ? scales.sw[n] : 0.f;
+      next_b = there && biased && n < N ? scales.bias[n] : 0.f;
 #pragma unroll
-      for (int i = 0; i < kPartCols / 32; ++i) {
-        const bool there = tile < num_tiles && n0 + 32 * i < N;
-        next_sw[i] = there ? scales.sw[n0 + 32 * i] : 0.f;
-        next_b[i] = there && biased ? scales.bias[n0 + 32 * i] : 0.f;
+      for (int i = 0; i < 2; ++i) {
+        const int at = 32 * i + lane, row = (at / kTake * kParts + part) * kTake + at % kTake, m = (tile % m_tiles) * bn + row;
+        next_sx[i] = there && row < bn && m < M ? scales.sx[m] : 0.f;
       }
     };
     ask(pair);
     for (int tile = pair; tile < num_tiles; tile += num_pairs, ++local) {
       const int a = local & 1;
-      const int m0 = (tile % m_tiles) * 256 + (int)rank * 128 + quarter * 32, n0 = (tile / m_tiles) * 256 + part * kPartCols;
-      const float sx = next_sx;
-#pragma unroll
-      for (int i = 0; i < kPartCols / 32; ++i) {
-        sw_s[32 * i + lane] = next_sw[i];
-        b_s[32 * i + lane] = next_b[i];
-      }
+      const int m0 = (tile % m_tiles) * bn, n0 = (tile / m_tiles) * 256 + (int)rank * 128 + quarter * 32;
+      const float sw = next_sw, b = next_b;
+      sx_s[lane] = next_sx[0];
+      sx_s[32 + lane] = next_sx[1];
       __syncwarp();
       ask(tile + num_pairs);
       if (!wait_on(acc_full_bar(a), (unsigned)(local >> 1) & 1, abort_flag, 13)) break;
       tc::fence_after();
-      const unsigned tmem_acc = tmem_base + (unsigned)(a * 256 + part * kPartCols) + ((unsigned)(quarter * 32) << 16);
+      const unsigned tmem_acc = tmem_base + (unsigned)(a * 256) + ((unsigned)(quarter * 32) << 16);
+      const int turns = ((min(bn, M - m0) + kTake - 1) / kTake - part + kParts - 1) / kParts;      // groups of rows that are this warp's
 #pragma unroll 1
-      for (int c = 0; c < kPartCols; c += kCols) {
-        unsigned v[kCols];
-        if constexpr (kCols == 32) tc::tmem_ld32(tmem_acc + (unsigned)c, v);
-        else tc::tmem_ld16(tmem_acc + (unsigned)c, v);
-        tc::tmem_ld_wait();
-        if (c + kCols == kPartCols) {                // all of this warp's part is read: the products may fill it again
+      for (int i = 0; i < kTurns; ++i) {
+        unsigned v[kTake];
+        const int row0 = (i * kParts + part) * kTake;
+        if (i < turns) {
+          if constexpr (kTake == 32) tc::tmem_ld32(tmem_acc + (unsigned)row0, v);
+          else tc::tmem_ld16(tmem_acc + (unsigned)row0, v);
+          tc::tmem_ld_wait();
+        }
+        if (i >= turns - 1) {                        // all of this warp's part is read: the products may fill it again
           tc::fence_before();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive_cluster(tc::map_to_rank(acc_empty_bar(a), 0));
         }
-        if (n0 + c >= N || m0 >= M) continue;        // the same for the whole warp
-        float y[kCols];
+        if (i < turns && n0 < N) {
+          TOut y[kTake];
 #pragma unroll
-        for (int e = 0; e < kCols; e += 4) {
-          const float4 sw = *reinterpret_cast<const float4*>(sw_s + c + e);
-          y[e] = __fmul_rn(__fmul_rn((float)(int)v[e], sx), sw.x), y[e + 1] = __fmul_rn(__fmul_rn((float)(int)v[e + 1], sx), sw.y);
-          y[e + 2] = __fmul_rn(__fmul_rn((float)(int)v[e + 2], sx), sw.z), y[e + 3] = __fmul_rn(__fmul_rn((float)(int)v[e + 3], sx), sw.w);
-        }
-        if (biased) {
-#pragma unroll
-          for (int e = 0; e < kCols; e += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(b_s + c + e);
-            y[e] = __fadd_rn(y[e], b.x), y[e + 1] = __fadd_rn(y[e + 1], b.y), y[e + 2] = __fadd_rn(y[e + 2], b.z), y[e + 3] = __fadd_rn(y[e + 3], b.w);
+          for (int e = 0; e < kTake; e += 4) {
+            const float4 sx = *reinterpret_cast<const float4*>(sx_s + i * kTake + e);
+            y[e] = from_f32<TOut>(finish((int)v[e], sx.x, sw, b, biased)), y[e + 1] = from_f32<TOut>(finish((int)v[e + 1], sx.y, sw, b, biased));
+            y[e + 2] = from_f32<TOut>(finish((int)v[e + 2], sx.z, sw, b, biased)), y[e + 3] = from_f32<TOut>(finish((int)v[e + 3], sx.w, sw, b, biased));
           }
-        }
-        if (lane == 0) tc::bulk_wait<0>();           // the buffer's last contents are on their way
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {                // 16 bytes at a time, their place turned by the row (the copy's swizzle)
-          uint4 o;
-          if constexpr (sizeof(TOut) == 2) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) reinterpret_cast<__nv_bfloat162*>(&o)[e] = __floats2bfloat162_rn(y[8 * j + 2 * e], y[8 * j + 2 * e + 1]);
-          } else {
-            o = make_uint4(__float_as_uint(y[4 * j]), __float_as_uint(y[4 * j + 1]), __float_as_uint(y[4 * j + 2]), __float_as_uint(y[4 * j + 3]));
-          }
-          *reinterpret_cast<uint4*>(buffer + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = o;
-        }
-        if (tma_out) {
-          tc::fence_async_smem();
+          if (lane == 0) tc::bulk_wait<0>();         // the buffer's last contents are on their way
           __syncwarp();
-          if (lane == 0) {
-            tc::tma_store_2d(&map_out, tc::smem_u32(buffer), n0 + c, m0);
-            tc::bulk_commit();
-          }
-        } else {
-          // Rows that do not start on 16-byte borders: two rows at a time, four bytes a lane. A row of bfloat16 may start between two
-          // four-byte borders: its pairs are then put together from neighbours' words, its first and last number stored alone.
-          __syncwarp();
-          const int half = lane >> 4, word = lane & 15, left = min(kCols, N - (n0 + c));
-          const unsigned char* from = buffer + half * 64 + (word & 3) * 4;
-          TOut* dst = out + (size_t)(m0 + half) * ldo + n0 + c;
-#pragma unroll 4
-          for (int i = 0; i < 16; ++i, dst += 2 * ldo) {
-            const unsigned own = *reinterpret_cast<const unsigned*>(from + i * 128 + (((word >> 2) ^ (i & 3)) << 4));
-            const bool live = m0 + 2 * i + half < M;
-            if constexpr (sizeof(TOut) == 4) {
-              if (live && word < left) dst[word] = __uint_as_float(own);
-            } else {
-              const unsigned next = __shfl_down_sync(0xffffffffu, own, 1);
-              const int odd = (int)((uintptr_t)dst >> 1) & 1, at = 2 * word + odd;
-              const unsigned two = odd ? __byte_perm(own, next, 0x5432) : own;
-              if (live && at + 1 < left) *reinterpret_cast<unsigned*>(dst + at) = two;
-              else if (live && at < left) dst[at] = __ushort_as_bfloat16((unsigned short)two);
-              if (live && odd && word == 0) dst[0] = __ushort_as_bfloat16((unsigned short)own);
+          TOut* held = reinterpret_cast<TOut*>(buffer) + lane;      // a row of x: 32 channels next to each other
+#pragma unroll
+          for (int e = 0; e < kTake; ++e) held[e * 32] = y[e];
+          if (tma_out) {
+            tc::fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tc::tma_store_2d(&map_out, tc::smem_u32(buffer), n0, m0 + row0);
+              tc::bulk_commit();
             }
+          } else {
+            // Result rows that do not start on 16-byte borders: four bytes a lane. A row of bfloat16 may start between two four-byte
+            // borders: its pairs are then put together from neighbours' words, its first and last number stored alone.
+            __syncwarp();
+            constexpr int kWords = 32 * (int)sizeof(TOut) / 4, kRowsAtOnce = 32 / kWords;
+            const int own_row = lane / kWords, word = lane % kWords, left = min(32, N - n0), live_rows = min(kTake, M - m0 - row0);
+            TOut* dst = out + (size_t)(m0 + row0 + own_row) * ldo + n0;
+#pragma unroll 4
+            for (int r = own_row; r < kTake; r += kRowsAtOnce, dst += kRowsAtOnce * ldo) {
+              const unsigned own = reinterpret_cast<const unsigned*>(buffer)[r * kWords + word];
+              const bool live = r < live_rows;
+              if constexpr (sizeof(TOut) == 4) {
+                if (live && word < left) dst[word] = __uint_as_float(own);
+              } else {
+                const unsigned next = __shfl_down_sync(0xffffffffu, own, 1);
+                const int odd = (int)((uintptr_t)dst >> 1) & 1, at = 2 * word + odd;
+                const unsigned two = odd ? __byte_perm(own, next, 0x5432) : own;
+                if (live && at + 1 < left) *reinterpret_cast<unsigned*>(dst + at) = two;
+                else if (live && at < left) dst[at] = __ushort_as_bfloat16((unsigned short)two);
+                if (live && odd && word == 0) dst[0] = __ushort_as_bfloat16((unsigned short)own);
+              }
+            }
+            __syncwarp();
           }
-          __syncwarp();
         }
+        if (i >= turns - 1) break;
       }
     }
     if (lane == 0) tc::bulk_wait<0, true>();
@@ -520,9 +513,12 @@ int allow_smem(Kernel kernel, int bytes, bool (&done)[64]) {
 
 constexpr int kMostStages = 12, kSmemOfTwo = 110 * 1024, kSmemOfOne = 208 * 1024;
 
-// result rows that start on 16-byte borders can be copied out by TMA
+// Result rows that start and end on 16-byte borders can be copied out by TMA. (Of a row that ends inside 16 bytes the copy writes
+// what is behind the end, too.)
 template <typename TOut>
-bool rows_on_borders(const TOut* out, long long ldo) { return (uintptr_t)out % 16 == 0 && ldo * sizeof(TOut) % 16 == 0; }
+bool rows_on_borders(const TOut* out, long long ldo, int N) {
+  return (uintptr_t)out % 16 == 0 && ldo * sizeof(TOut) % 16 == 0 && N * sizeof(TOut) % 16 == 0;
+}
 
 template <typename TOut>
 int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
@@ -566,22 +562,24 @@ int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const vo
 
 template <typename TOut>
 int launch_pair(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
-                cudaStream_t s) {
-  CUtensorMap mx, mw;
-  int rc = tc::make_map_2d_i8(&mx, x, M, K, ldx, BM);
-  OI_REQUIRE(rc == 0, "linear_int8: tensor map for x failed (%d; -1: cuTensorMapEncodeTiled is not available)", rc);
-  rc = tc::make_map_2d_i8(&mw, w, N, K, ldw, BM);
-  OI_REQUIRE(rc == 0, "linear_int8: tensor map for the weight failed (%d)", rc);
-  const bool tma_out = rows_on_borders(out, ldo);
+                int bn, cudaStream_t s) {
+  CUtensorMap mw, mx;
+  int rc = tc::make_map_2d_i8(&mw, w, N, K, ldw, BM);
+  OI_REQUIRE(rc == 0, "linear_int8: tensor map for the weight failed (%d; -1: cuTensorMapEncodeTiled is not available)", rc);
+  rc = tc::make_map_2d_i8(&mx, x, M, K, ldx, bn / 2);
+  OI_REQUIRE(rc == 0, "linear_int8: tensor map for x failed (%d)", rc);
+  const bool tma_out = rows_on_borders(out, ldo, N);
   CUtensorMap mo = mx;
-  if (tma_out && (rc = tc::make_map_2d_out(&mo, out, sizeof(TOut) == 4, M, N, ldo, 32))) OI_REQUIRE(false, "linear_int8: tensor map for the result failed (%d)", rc);
+  if (tma_out && (rc = tc::make_map_2d_out(&mo, out, sizeof(TOut) == 4, M, N, ldo, 32, kBufferBytes / 32 / (int)sizeof(TOut))))
+    OI_REQUIRE(false, "linear_int8: tensor map for the result failed (%d)", rc);
   auto kernel = linear_int8_pair_kernel<TOut>;
   static bool allowed[64];
   if ((rc = allow_smem(kernel, kPairSmem, allowed))) return rc;
-  const long long tiles = (long long)ceil_div(M, 256) * ceil_div(N, 256);
+  const long long tiles = (long long)ceil_div(M, bn) * ceil_div(N, 256);
   OI_REQUIRE(tiles < (1LL << 30), "linear_int8: %d rows of %d results are too many", M, N);
   const int most = oi_sm_count() / 2, pairs = tiles < most ? (int)tiles : most;
-  oi_launch_cluster(kernel, 2 * pairs, kPairThreads, kPairSmem, s, 2, mx, mw, mo, out, ldo, scales, M, N, ceil_div(K, BK), (int)tma_out);
+  const int fit = kPairRingBytes / (kBoxBytes + bn / 2 * BK), stages = fit < kPairMostStages ? fit : kPairMostStages;
+  oi_launch_cluster(kernel, 2 * pairs, kPairThreads, kPairSmem, s, 2, mw, mx, mo, out, ldo, scales, M, N, ceil_div(K, BK), bn, stages, (int)tma_out);
   OI_CHECK_LAUNCH();
   return OI_OK;
 }
@@ -589,23 +587,30 @@ int launch_pair(TOut* out, long long ldo, const void* x, long long ldx, const vo
 // What a product takes in us, from what was measured (B200; N 128 to 32,000, K 128 to 16,000, 1 to 4,096 rows), to choose a kernel, the
 // tiles of x and the slices of K.
 // Few rows: a stage of 128 bytes of K is 16 KB of w and `cols` rows of x at what one SM takes in, for as many CTAs as an SM has to
-// run; the weight's bytes come from memory; every round of CTAs costs 2.3 around its first copy and its results, 0.006 to 0.008 a column
-// of the accumulator, or added up over a cluster 0.7 and 0.028 a column. Clusters of four and eight do not fill the SMs (35 of four: two
-// rounds). Many rows: 4.5, and for each round of tiles 0.33 a stage, or what a tile's results take: 3.2, and 6.5 where result rows do
-// not start on 16-byte borders.
+// run; the weight's bytes come from memory, all copies through L2 (16 TB/s); every round of CTAs costs 2.3 around its first copy and its results, 0.006 to 0.008 a column
+// of the accumulator, or added up over a cluster 0.5 and 0.038 a row of x. Clusters of four and eight do not fill the SMs (35 of four: two
+// rounds).
+// Many rows: 4.5, and for each round of tiles its stages (16 KB of w and half the tile's rows of x for each CTA) or, where sums are
+// short, its results, which take longer where result rows do not start on 16-byte borders.
 float few_rows_us(int M, int N, int num_kb, int c, int z, int sms) {
   const int cols = ceil_div(M, z), bn = ceil_div(cols, 16) * 16, kb = ceil_div(num_kb, c), at_once = c == 8 ? sms * 2 / 3 : c == 4 ? sms - 20 : sms;
   const long long ctas = (long long)ceil_div(N, BM) * z * c;
   const int on_an_sm = ctas <= at_once || bn > 128 ? 1 : 2;
   const float rounds = (float)((ctas + at_once * on_an_sm - 1) / (at_once * on_an_sm));
-  const float stream = (float)((ctas + at_once - 1) / at_once) * kb * (0.185f + 0.0005f * cols), memory = (float)N * num_kb * BK / 6.4e6f;
-  const float results = c > 1 ? 0.7f + 0.028f * (cols < bn - 12 ? cols : bn) : (bn > 128 ? 0.008f : 0.006f) * bn;
-  return rounds * (2.3f + results * on_an_sm) + (stream > memory ? stream : memory);
+  float stream = (float)((ctas + at_once - 1) / at_once) * kb * (0.185f + 0.0005f * cols);
+  const float memory = (float)N * num_kb * BK / 6.4e6f, l2 = (float)ctas * kb * BK * (BM + cols) / 16e6f;
+  if (stream < memory) stream = memory;
+  if (stream < l2) stream = l2;
+  const float results = c > 1 ? 0.5f + 0.038f * cols : (bn > 128 ? 0.008f : 0.006f) * bn;
+  return rounds * (2.3f + results * on_an_sm) + stream;
 }
-float many_rows_us(int M, int N, int num_kb, bool on_borders, int sms) {
-  const long long tiles = (long long)ceil_div(M, 256) * ceil_div(N, 256);
-  const float products = 0.33f * num_kb, results = on_borders ? 3.2f : 6.5f, a_round = products > results ? products : results;
-  return 4.5f + (float)((tiles + sms / 2 - 1) / (sms / 2)) * a_round;
+float many_rows_us(int M, int N, int num_kb, int bn, bool f32, bool on_borders, int sms) {
+  const long long tiles = (long long)ceil_div(M, bn) * ceil_div(N, 256);
+  const float products = (0.14f + 0.00074f * bn) * num_kb;
+  const float results = (on_borders ? (f32 ? 1.0f + 0.0105f * bn : 1.4f + 0.0066f * bn) : (f32 ? 1.5f + 0.0165f * bn : 2.5f + 0.019f * bn)) + 0.4f * products;
+  const float rounds = (float)((tiles + sms / 2 - 1) / (sms / 2)), work = rounds * (products > results ? products : results);
+  const float memory = (float)N * num_kb * BK / 6.4e6f;
+  return 4.5f + (work > memory ? work : memory);
 }
 
 template <typename TOut>
@@ -613,7 +618,12 @@ int launch(TOut* out, long long ldo, const void* x, long long ldx, const void* w
            cudaStream_t s) {
   const int num_kb = ceil_div(K, BK), sms = oi_sm_count(), least = ceil_div(M, 256);
   int best_c = 0, best_z = 0;
-  float best = many_rows_us(M, N, num_kb, rows_on_borders(out, ldo), sms);
+  int best_bn = 256;
+  float best = 3.4e38f;
+  for (int bn = 32; bn <= 256; bn += 32) {
+    const float us = many_rows_us(M, N, num_kb, bn, sizeof(TOut) == 4, rows_on_borders(out, ldo, N), sms);
+    if (us <= best) best = us, best_bn = bn;
+  }
   if (least <= 16 && ceil_div(N, BM) <= 65535) {
     for (int z = least; z <= 4 * least + 4 && z <= ceil_div(M, 16); ++z)
       for (int c = 1; c <= 8 && (c == 1 || (c - 1) * ceil_div(num_kb, c) < num_kb); c *= 2) {     // no slice without a stage
@@ -621,7 +631,7 @@ int launch(TOut* out, long long ldo, const void* x, long long ldx, const void* w
         if (us < best) best = us, best_c = c, best_z = z;
       }
   }
-  return best_c ? launch_rows(out, ldo, x, ldx, w, ldw, scales, M, N, K, best_c, best_z, s) : launch_pair(out, ldo, x, ldx, w, ldw, scales, M, N, K, s);
+  return best_c ? launch_rows(out, ldo, x, ldx, w, ldw, scales, M, N, K, best_c, best_z, s) : launch_pair(out, ldo, x, ldx, w, ldw, scales, M, N, K, best_bn, s);
 }
 
 }  // namespace

@@ -313,16 +313,17 @@ inline int make_map_2d_bf16(CUtensorMap* map, const void* base, long long rows, 
                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
-// rows x cols result matrix (float32 or bfloat16, row stride ld in elements) for stores of box_rows rows of 64 bytes, 64-byte swizzle.
-inline int make_map_2d_out(CUtensorMap* map, void* base, bool f32, long long rows, long long cols, long long ld, int box_rows) {
+// rows x cols result matrix (float32 or bfloat16, row stride ld in elements, rows on 16-byte borders) for stores of box_rows rows of box_cols
+// numbers that lie one behind the other in shared memory.
+inline int make_map_2d_out(CUtensorMap* map, void* base, bool f32, long long rows, long long cols, long long ld, int box_cols, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return -1;
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)ld * (f32 ? 4 : 2)};
-  cuuint32_t box[2] = {f32 ? 16u : 32u, (cuuint32_t)box_rows};
+  cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   return (int)fn(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr,
-                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 // rows x K 8-bit matrix with row stride ld (bytes, a multiple of 16); boxes of box_rows x 128 bytes, 128-byte swizzle, zeros
 // outside the matrix (K need not be a multiple of anything).

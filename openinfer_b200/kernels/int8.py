@@ -25,6 +25,9 @@ from .ops import act_code
 
 MOST = 1 << 30             # rows, and numbers of a row
 ALIGN = 16                 # bytes that the rows of 8-bit operands start on
+# Rows that are allocated here are a multiple of so many bytes apart: 128 bytes of a row then lie in as few lines of the caches as they
+# can (rows 16 bytes off: 2538 x 7746 x 11239 186 us, 149 so; 264 x 4096 x 12200 27.9 and 19.7; 1 x 6144 x 4100 7.6 and 7.3).
+APART = 64
 MAX_WIDTH = 131071         # the longest sum of products of two 8-bit integers that a 32-bit integer holds: 128 * 128 * 131071 < 2^31
 
 _DT = {torch.float32: 0, torch.bfloat16: 1}
@@ -78,7 +81,7 @@ def _cuda(device: int, what: str) -> None:
 
 def empty_rows(rows: int, width: int, device) -> Int8Rows:
     """Room for rows of 8-bit integers."""
-    values = (torch.empty_strided((rows, width), (-(-width // ALIGN) * ALIGN, 1), dtype=torch.int8, device=device) if width % ALIGN
+    values = (torch.empty_strided((rows, width), (-(-width // APART) * APART, 1), dtype=torch.int8, device=device) if width % APART
               else torch.empty(rows, width, dtype=torch.int8, device=device))
     return Int8Rows(values, torch.empty(rows, dtype=torch.float32, device=device))
 
@@ -89,7 +92,7 @@ def _room(out: Optional[Int8Rows], x: torch.Tensor, rows: int, width: int, devic
         _cuda(device, what)
     if out is None:
         out = values, scales = empty_rows(rows, width, x.device)
-        return out, values.data_ptr(), -(-width // ALIGN) * ALIGN, scales.data_ptr()
+        return out, values.data_ptr(), -(-width // APART) * APART, scales.data_ptr()
     address, stride, has_rows, has_width, scales, on = _int8_rows(*out, what)
     if (has_rows, has_width, on) != (rows, width, device):
         raise KernelError(f"{what}: room for {(has_rows, has_width)} on {out[0].device}, needed {(rows, width)} on {x.device}")
@@ -198,7 +201,8 @@ def dequantize_int8(rows: Int8Rows, dtype: torch.dtype = torch.bfloat16, out: Op
 class Int8Weight:
     """A weight [channels, width] for ``linear_int8``: int8 values with a float32 scale for each output channel, laid out once.
 
-    Values whose rows do not start on 16-byte borders are copied into rows that do; others are kept as they are. A product
+    Values whose rows do not start on 16-byte borders, or are wider than 64 and not a multiple of 64 bytes apart, are copied into rows
+    that are; others are kept as they are. A product
     fetches its weight while the kernel ahead of it on the stream still runs, but for the first one on each stream. Later
     changes of the weight's tensors (by torch, or through ``out`` of the functions above) are ordered by the stream as ever."""
 
@@ -211,7 +215,8 @@ class Int8Weight:
         if not 1 <= width <= MAX_WIDTH:
             raise KernelError(f"Int8Weight: sums of {width} products (1 to {MAX_WIDTH} are exact in 32 bits)")
         strides = values.stride()
-        if (width > 1 and strides[1] != 1) or values.data_ptr() % ALIGN or (rows > 1 and (strides[0] % ALIGN or strides[0] < width)):
+        if (width > 1 and strides[1] != 1) or values.data_ptr() % ALIGN or (rows > 1 and (
+                strides[0] % (APART if width > APART else ALIGN) or strides[0] < width)):
             held = empty_rows(rows, width, values.device).values
             held.copy_(values)
             values = held

@@ -83,8 +83,10 @@ def test_weight_and_product():
     refused("exact in 32 bits", int8.Int8Weight, torch.zeros(1, int8.MAX_WIDTH + 1, dtype=torch.int8), torch.ones(1))
     refused("exact in 32 bits", int8.Int8Weight, ROWS[:, :0], SCALES)
     refused("float32 scales", int8.Int8Weight, ROWS, SCALES.bfloat16())
-    w = int8.Int8Weight(torch.ones(5, 33, dtype=torch.int8), torch.ones(10)[::2])     # laid out in rows of 48
-    assert w.values.stride() == (48, 1) and bool((w.values == 1).all()) and w.scales.is_contiguous()
+    w = int8.Int8Weight(torch.ones(5, 33, dtype=torch.int8), torch.ones(10)[::2])     # laid out in rows of 64
+    assert w.values.stride() == (64, 1) and bool((w.values == 1).all()) and w.scales.is_contiguous()
+    wide = int8.Int8Weight(torch.arange(4 * 80).view(4, 80).to(torch.int8), torch.ones(4))
+    assert wide.values.stride() == (128, 1) and torch.equal(wide.values, torch.arange(4 * 80).view(4, 80).to(torch.int8))
     kept = int8.Int8Weight(ROWS, SCALES)
     assert kept.values.data_ptr() == ROWS.data_ptr()
     rows = int8.Int8Rows(ROWS, SCALES)

@@ -223,14 +223,17 @@ def on_device(int8, x, sx):
 # rows on both sides of every size at which another tile is taken; sums that fill a stage, miss it by one, and leave slices empty
 SHAPES = [(1, 1, 1), (1, 128, 128), (1, 5, 16), (2, 33, 31), (3, 130, 129), (8, 256, 127), (15, 1000, 64), (16, 128, 4096), (17, 256, 500), (31, 300, 1024), (32, 1536, 4096),
           (33, 257, 2048), (48, 640, 1000), (64, 1024, 4096), (65, 384, 96), (100, 4096, 777), (127, 129, 8192), (128, 1024, 1024), (129, 999, 2048), (200, 128, 300),
-          (256, 512, 512), (257, 2049, 333), (300, 6144, 256), (512, 513, 1025), (777, 1000, 2001), (1024, 2048, 640), (2050, 300, 4100), (5000, 130, 72), (1, 9000, 14000), (4, 64, 60000),
-          # every kernel, number of slices, of warps that read results, and place of the partial sums: few rows by one, two, four and eight CTAs ...
-          (194, 9522, 546), (276, 9555, 408), (137, 13516, 33), (83, 9769, 33), (262, 8322, 134), (427, 6948, 519), (197, 5048, 33), (34, 10895, 37),
-          (99, 5008, 5688), (66, 4827, 4703), (263, 3153, 7355), (3905, 130, 5552), (390, 550, 1747), (20, 3580, 1500),
-          (109, 2548, 5457), (141, 3266, 5385), (33, 2547, 1578), (3097, 47, 3526), (17, 34, 1267), (389, 36, 1449),
-          (99, 815, 13890), (131, 1311, 10041), (1610, 72, 16138), (34, 880, 3675), (394, 42, 899), (1, 33, 917),
-          # ... and many rows, with result rows on 16-byte borders, on four-byte borders, and on none; more tiles than pairs of CTAs
-          (1845, 6736, 139), (444, 15348, 1940), (327, 14293, 2407)]
+          (256, 512, 512), (257, 2049, 333), (300, 6144, 256), (512, 513, 1025), (777, 1000, 2001), (1024, 2048, 640), (2050, 300, 4100), (5000, 130, 72), (1, 9000, 14000), (4, 64, 60000)]
+# Every kernel, width of its tiles, number of slices, of warps that read results, and place of the partial sums; result rows on 16-byte
+# borders, on four-byte borders, and on none; more tiles than pairs of CTAs.
+TILES = [(370, 2972, 7657), (574, 7354, 3863), (309, 8746, 3887), (629, 8798, 2673), (1532, 671, 7446), (1367, 3287, 3872), (442, 5427, 4611),
+          (1789, 2761, 2951), (464, 4400, 7640), (1599, 1672, 2630), (1784, 3048, 757), (763, 4112, 1824), (2003, 5096, 186), (624, 5560, 2014),
+          (1570, 9128, 55), (2496, 1736, 1546), (1845, 6736, 139), (616, 2552, 8097), (67, 10187, 33), (194, 9522, 546), (140, 15241, 130),
+          (1, 32, 33), (34, 10895, 37), (276, 9555, 408), (137, 13516, 33), (197, 5048, 33), (427, 6948, 519), (262, 8322, 134), (83, 9769, 33),
+          (18, 32, 33), (127, 9708, 32), (389, 33, 32), (108, 5112, 7677), (66, 4827, 4703), (1, 32, 692), (36, 4895, 2498), (3232, 178, 7209),
+          (2455, 147, 3658), (1765, 513, 9245), (17, 34, 1061), (3053, 32, 3017), (105, 3407, 6918), (71, 2413, 5902), (129, 2256, 14702),
+          (1, 32, 401), (33, 2092, 2422), (3112, 32, 5562), (2099, 32, 2845), (269, 1898, 7347), (21, 32, 786), (389, 36, 1449), (105, 1506, 10930),
+          (65, 1113, 9920), (130, 1413, 14655), (1, 33, 917), (33, 830, 4806), (1164, 34, 14005), (812, 33, 5825), (22, 32, 977), (409, 36, 2770)]
 
 
 @pytest.mark.parametrize("rows,channels,width", SHAPES)
@@ -247,6 +250,19 @@ def test_product(int8, rows, channels, width):
             out = torch.full((rows, channels + pad), -7.0, dtype=dtype, device=DEV)
             int8.linear_int8(held, weight, bias=bias.to(DEV), out=out[:, :channels])
             assert torch.equal(out[:, :channels].cpu(), product_exactly(x, sx, w, sw, bias, dtype)) and bool((out[:, channels:] == -7.0).all())
+
+
+@pytest.mark.parametrize("rows,channels,width", TILES)
+def test_product_by_every_kind_of_tile(int8, rows, channels, width):
+    (x, sx), (w, sw) = integers(rows, width, 1), integers(channels, width, 2)
+    bias = randn(channels, seed=3)
+    held, weight = on_device(int8, x, sx), int8.Int8Weight(w.to(DEV), sw.to(DEV))
+    assert torch.equal(int8.linear_int8(held, weight).cpu(), product_exactly(x, sx, w, sw, None, torch.bfloat16))
+    out = torch.full((rows, channels + 1), -7.0, device=DEV)
+    for dtype, room in ((torch.float32, out[:, :channels]), (torch.float32, None)):
+        got = int8.linear_int8(held, weight, bias=bias.to(DEV), out_dtype=dtype, out=room)
+        assert torch.equal(got.cpu(), product_exactly(x, sx, w, sw, bias, dtype))
+    assert bool((out[:, channels:] == -7.0).all())
 
 
 def test_the_longest_and_largest_sums(int8):
