@@ -584,25 +584,25 @@ int launch_pair(TOut* out, long long ldo, const void* x, long long ldx, const vo
   return OI_OK;
 }
 
-// What a product takes in us, from what was measured (B200; N 128 to 32,000, K 128 to 16,000, 1 to 4,096 rows), to choose a kernel, the
-// tiles of x and the slices of K.
+// What a product takes in us, from what was measured (B200; N 32 to 152,000, K 128 to 16,000, 1 to 8,192 rows), to choose a kernel, its
+// tiles of x and the slices of K. Over 150 sizes, most of them drawn, the choice took at most 1.24 times the fastest choice's time, in the
+// median 1.00.
 // Few rows: a stage of 128 bytes of K is 16 KB of w and `cols` rows of x at what one SM takes in, for as many CTAs as an SM has to
-// run; the weight's bytes come from memory, all copies through L2 (16 TB/s); every round of CTAs costs 2.3 around its first copy and its results, 0.006 to 0.008 a column
-// of the accumulator, or added up over a cluster 0.5 and 0.038 a row of x. Clusters of four and eight do not fill the SMs (35 of four: two
-// rounds).
+// run; the weight's bytes come from memory and all copies through L2 (16 TB/s). Every round of CTAs costs 2.3 around its first copy
+// and its results, 0.006 to 0.008 a column of the accumulator, or added up over a cluster 0.5 and 0.038 a row of x. Clusters of four
+// and eight do not fill the SMs (35 of four: two rounds).
 // Many rows: 4.5, and for each round of tiles its stages (16 KB of w and half the tile's rows of x for each CTA) or, where sums are
-// short, its results, which take longer where result rows do not start on 16-byte borders.
+// short, its results, which take longer where result rows do not start and end on 16-byte borders.
 float few_rows_us(int M, int N, int num_kb, int c, int z, int sms) {
   const int cols = ceil_div(M, z), bn = ceil_div(cols, 16) * 16, kb = ceil_div(num_kb, c), at_once = c == 8 ? sms * 2 / 3 : c == 4 ? sms - 20 : sms;
   const long long ctas = (long long)ceil_div(N, BM) * z * c;
   const int on_an_sm = ctas <= at_once || bn > 128 ? 1 : 2;
   const float rounds = (float)((ctas + at_once * on_an_sm - 1) / (at_once * on_an_sm));
-  float stream = (float)((ctas + at_once - 1) / at_once) * kb * (0.185f + 0.0005f * cols);
+  const float products = (float)((ctas + at_once - 1) / at_once) * kb * (0.185f + 0.0005f * cols);
   const float memory = (float)N * num_kb * BK / 6.4e6f, l2 = (float)ctas * kb * BK * (BM + cols) / 16e6f;
-  if (stream < memory) stream = memory;
-  if (stream < l2) stream = l2;
   const float results = c > 1 ? 0.5f + 0.038f * cols : (bn > 128 ? 0.008f : 0.006f) * bn;
-  return rounds * (2.3f + results * on_an_sm) + stream;
+  const float around = 2.3f + results * on_an_sm, copies = memory > l2 ? memory : l2, work = products + (rounds - 1.f) * around;
+  return around + (work > copies ? work : copies);
 }
 float many_rows_us(int M, int N, int num_kb, int bn, bool f32, bool on_borders, int sms) {
   const long long tiles = (long long)ceil_div(M, bn) * ceil_div(N, 256);
@@ -610,7 +610,7 @@ float many_rows_us(int M, int N, int num_kb, int bn, bool f32, bool on_borders, 
   const float results = (on_borders ? (f32 ? 1.0f + 0.0105f * bn : 1.4f + 0.0066f * bn) : (f32 ? 1.5f + 0.0165f * bn : 2.5f + 0.019f * bn)) + 0.4f * products;
   const float rounds = (float)((tiles + sms / 2 - 1) / (sms / 2)), work = rounds * (products > results ? products : results);
   const float memory = (float)N * num_kb * BK / 6.4e6f;
-  return 4.5f + (work > memory ? work : memory);
+  return 4.5f + (work > memory ? work : memory + 0.05f * work);      // (of equal ones that with the least to do)
 }
 
 template <typename TOut>
