@@ -3,9 +3,10 @@
 // addition, tile or slice of K matters to a result; then float(sum) * sx * sw + bias in float32, in that order, and one
 // rounding to the output's type.
 //
-// Two kernels. Operands are staged by TMA as rows of 128 bytes (128-byte swizzle); bytes beyond K or beyond the last row are
-// zeros of the copy. Every wait on an mbarrier is bounded: one that runs out sets an error word and a flag that ends all roles
-// of the CTA, which still joins its cluster's barriers, frees its tensor memory and returns. No load uses cluster multicast.
+// Three kernels: for up to 16 rows on mma.sync, for few and for many rows on tcgen05. The operands of the latter two are staged by TMA as
+// rows of 128 bytes (128-byte swizzle); bytes beyond K or beyond the last row are zeros of the copy. Every wait on an mbarrier is
+// bounded: one that runs out sets an error word and a flag that ends all roles of the CTA, which still joins its cluster's barriers,
+// frees its tensor memory and returns. No load uses cluster multicast.
 #include "oi_api.h"
 #include "tcgen05.cuh"
 
@@ -498,6 +499,214 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
   }
 }
 
+// ------------------------------------------------------------------------------------------------
+// Up to 16 rows, on mma.sync: what counts is the chain behind the wait for x, and the kernel above has a TMA copy of x, a
+// tensor-memory round trip, deposits and a cluster barrier there. One CTA per SM owns whole rows of w, 16 at a time, so no sums cross
+// CTAs:
+//   warp 8     copies rows into shared memory (cp.async.bulk, one copy per row of a stage, counted on an mbarrier), as many as the
+//              ring holds before the kernel ahead on the stream has finished
+//   warps 0-7  share out K (blocks of 128 bytes in turn). After the wait a warp reads its part of x straight into the registers that
+//              mma.sync takes as operand B (rows of x on the 8-column side); 16 rows of w are operand A. The k index inside a block is
+//              permuted alike for both, so 32 contiguous bytes of a row are a lane's fragments of four products. The eight warps'
+//              sums meet in shared memory.
+// Rows of a stage are 2,048 + 16 bytes apart, so that the eight lanes that a 16-byte shared load serves at once hit different banks.
+// Bytes of x behind K are made zeros; whatever lies there in w then does not count. Sixteen lanes that each ask for a row fill the ring
+// sooner, one elected lane that asks for all keeps up a longer stream (with a norm ahead, us: N 9216 K 2048 5.1 and 5.6, N 24576 K 4096
+// 18.7 and 17.7), so the one is taken where the ring holds all of a CTA's rows, the other where it does not.
+//
+// Measured (us, one row, a norm and the product in turn inside a graph; the kernel above at its best -> this one; the norm alone 1.7
+// to 1.9): N 4096 K 4096 6.9 -> 5.6, N 6144 K 4096 8.9 -> 6.8, N 9216 K 2048 7.3 -> 5.1, N 24576 K 4096 20.5 -> 17.7 (its bytes: 15.4). With
+// eight rows 7.5 -> 5.9, 9.2 -> 7.3, 7.4 -> 5.5, 21.0 -> 18.2. What bounds it: the stream where the ring is shorter than a CTA's rows, else
+// the chain behind the wait; many short rows are a barrier for each 32 of them (N 16384 K 1024 7.7 above, 8.1 here).
+constexpr int kFewWarps = 8, kFewThreads = (kFewWarps + 1) * 32;
+constexpr int kChunkBlocks = 2, kChunk = kChunkBlocks * kFewWarps * 128;     // bytes of a row in a stage
+constexpr int kFewRowBytes = kChunk + 16, kFewStage = 16 * kFewRowBytes, kFewMostStages = 6;
+constexpr int kFewPart = 8192;                 // the warps' sums: 8 x 16 x 16, or twice 8 x 16 x 8
+
+struct FewArgs {
+  const signed char *x, *w;
+  void* out;
+  long long ldx, ldw, ldo;
+  Scales scales;
+  int M, N, K, groups, stages;
+  int at_once;              // the ring holds all of a CTA's rows
+};
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 lds128(unsigned addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+// 16 bytes of a row of x from byte k on, past L1 (other SMs have just written them); what lies at K and behind is zero. The 16 bytes that
+// hold byte K - 1 belong to the row: rows start on 16-byte borders.
+__device__ __forceinline__ uint4 load_x16(const signed char* row, int k, int K) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (k < K) {
+    v = __ldcg(reinterpret_cast<const uint4*>(row + k));
+    if (K - k < 16) {
+      unsigned* words = reinterpret_cast<unsigned*>(&v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int left = K - k - 4 * i;
+        words[i] &= left >= 4 ? 0xffffffffu : left > 0 ? (1u << 8 * left) - 1u : 0u;
+      }
+    }
+  }
+  return v;
+}
+__device__ __forceinline__ void few_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(kFewWarps * 32) : "memory"); }
+
+// NT: groups of eight rows of x; B: blocks of a warp over the whole row
+template <int NT, int B, typename TOut>
+__global__ void __launch_bounds__(kFewThreads)
+linear_int8_few_kernel(const __grid_constant__ FewArgs a) {
+  pdl_trigger();
+  constexpr int kHeld = 2 / NT, kTokens = 8 * NT, kEach = 16 * kTokens;          // groups whose sums wait for one barrier: 256 sums
+  static_assert(kHeld * kFewWarps * kEach * 4 == kFewPart && kHeld * kEach == kFewWarps * 32, "one sum a thread");
+  extern __shared__ __align__(1024) unsigned char smem[];
+  int* part = reinterpret_cast<int*>(smem);                  // [held][warp][rows of w][rows of x]
+  const unsigned ring = tc::smem_u32(smem) + kFewPart, bars = ring + a.stages * kFewStage;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kFewPart + a.stages * (kFewStage + 16));
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (a.stages + s); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int chunks = (a.K + kChunk - 1) / kChunk, blocks = (a.K + 127) / 128;
+  const int turn = blockIdx.x % chunks;                      // the chunk of a row that this CTA begins with: not all read the same of x at once
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      tc::mbar_init(full_bar(s), 1);
+      tc::mbar_init(empty_bar(s), kFewWarps);
+    }
+    *abort_flag = 0;
+    tc::mbar_fence_init();
+  }
+  __syncthreads();
+
+  if (warp == kFewWarps) {
+    const bool leader = tc::elect_one();
+    const unsigned long long once = tc::policy_evict_first();
+    Ring at;
+    int ahead = a.stages;
+    bool ok = true;
+    for (int grp = blockIdx.x; grp < a.groups && ok; grp += gridDim.x) {
+      const int rows = min(16, a.N - grp * 16);
+      const signed char* from = a.w + (size_t)grp * 16 * a.ldw;
+      for (int c = 0; c < chunks; ++c, at.next(a.stages)) {
+        if (ahead > 0) --ahead;
+        else if (!wait_on(empty_bar(at.stage), at.parity ^ 1, abort_flag, 21)) { ok = false; break; }
+        const int k0 = (c + turn < chunks ? c + turn : c + turn - chunks) * kChunk;
+        const unsigned len = (unsigned)min((a.K - k0 + 15) & ~15, kChunk), dst = ring + at.stage * kFewStage;
+        if (leader) tc::mbar_expect_tx(full_bar(at.stage), rows * len);
+        __syncwarp();
+        if (a.at_once) {
+          if (lane < rows) tc::bulk_load_hint(dst + lane * kFewRowBytes, from + k0 + lane * a.ldw, len, full_bar(at.stage), once);
+        } else if (leader) {
+          const signed char* src = from + k0;
+#pragma unroll 4
+          for (int r = 0; r < rows; ++r, src += a.ldw) tc::bulk_load_hint(dst + r * kFewRowBytes, src, len, full_bar(at.stage), once);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    const int g = lane >> 2, c4 = lane & 3;
+    auto block_of = [&](int i) {                             // the i-th block of this warp
+      const int c = i / kChunkBlocks + turn;
+      return ((c < chunks ? c : c - chunks) * kChunkBlocks + (i & 1)) * kFewWarps + warp;
+    };
+    const unsigned my_w = ring + g * kFewRowBytes + warp * 128 + c4 * 32;
+    // this thread's sum of every batch of groups: row m of x, channel `col` of group `f`
+    const int f = threadIdx.x / kEach, m = threadIdx.x / 16 % kTokens, col = threadIdx.x % 16;
+    const bool biased = a.scales.bias != nullptr;
+    auto channel = [&](int first) { return ((long long)first + f * (int)gridDim.x) * 16 + col; };
+    auto asked = [&](const float* of, int first) { return channel(first) < a.N ? of[channel(first)] : 0.f; };
+    float next_sw = asked(a.scales.sw, blockIdx.x);          // a batch ahead
+    bool ok = wait_on(full_bar(0), 0, abort_flag, 22);       // weights: not waited for behind x
+    pdl_wait();
+    uint4 xr[B][NT][2];
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int k = i / kChunkBlocks < chunks ? block_of(i) * 128 + c4 * 32 : a.K, m = g + 8 * t;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) xr[i][t][h] = m < a.M ? load_x16(a.x + (size_t)m * a.ldx, k + 16 * h, a.K) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+    const float sx = m < a.M ? a.scales.sx[m] : 0.f;
+    float next_b = biased ? asked(a.scales.bias, blockIdx.x) : 0.f, sw = 0.f, b = 0.f;
+
+    Ring at;
+    int held = 0, first = blockIdx.x;
+    for (int grp = blockIdx.x; grp < a.groups; grp += gridDim.x) {
+      if (held == 0) {
+        sw = next_sw, b = next_b;
+        next_sw = asked(a.scales.sw, first + kHeld * gridDim.x);
+        if (biased) next_b = asked(a.scales.bias, first + kHeld * gridDim.x);
+      }
+      int acc[NT][2][4] = {};
+#pragma unroll
+      for (int c = 0; c < B / kChunkBlocks; ++c) {
+        if (c < chunks) {
+          if (ok) ok = wait_on(full_bar(at.stage), at.parity, abort_flag, 22);
+          const unsigned src = my_w + at.stage * kFewStage;
+#pragma unroll
+          for (int j = 0; j < kChunkBlocks; ++j) {
+            const int i = c * kChunkBlocks + j;
+            if (block_of(i) < blocks) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const unsigned at16 = src + j * kFewWarps * 128 + h * 16;
+                const uint4 lo = lds128(at16), hi = lds128(at16 + 8 * kFewRowBytes);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                  mma_s8(acc[t][0], lo.x, hi.x, lo.y, hi.y, xr[i][t][h].x, xr[i][t][h].y);
+                  mma_s8(acc[t][1], lo.z, hi.z, lo.w, hi.w, xr[i][t][h].z, xr[i][t][h].w);
+                }
+              }
+            }
+          }
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(empty_bar(at.stage));
+          at.next(a.stages);
+        }
+      }
+      int* dst = part + (held * kFewWarps + warp) * kEach;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          *reinterpret_cast<int2*>(dst + (q * 8 + g) * kTokens + t * 8 + c4 * 2) =
+              make_int2(acc[t][0][2 * q] + acc[t][1][2 * q], acc[t][0][2 * q + 1] + acc[t][1][2 * q + 1]);
+      }
+      const bool last = grp + (int)gridDim.x >= a.groups;
+      if (++held == kHeld || last) {
+        few_sync();
+        const long long n = channel(first);
+        if (f < held && m < a.M && n < a.N) {
+          const int* src = part + f * kFewWarps * kEach + col * kTokens + m;
+          int sum = 0;
+#pragma unroll
+          for (int q = 0; q < kFewWarps; ++q) sum += src[q * kEach];
+          reinterpret_cast<TOut*>(a.out)[(size_t)m * a.ldo + n] = from_f32<TOut>(finish(sum, sx, sw, b, biased));
+        }
+        held = 0;
+        first = grp + gridDim.x;
+        if (!last) few_sync();
+      }
+    }
+  }
+  __syncthreads();
+  if (*abort_flag && threadIdx.x == 0)
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);        // copies still landing in this CTA's shared memory
+  __syncthreads();
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 // The shared memory that a kernel may ask for, allowed once for each device that it runs on.
 template <typename Kernel>
@@ -584,6 +793,36 @@ int launch_pair(TOut* out, long long ldo, const void* x, long long ldx, const vo
   return OI_OK;
 }
 
+// The longest row of w beside M rows of x, which lie in registers; 0: too many rows
+int few_longest(int M) { return M <= 8 ? 12288 : M <= 16 ? 8192 : 0; }
+
+template <typename TOut>
+int launch_few(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
+               cudaStream_t s) {
+  FewArgs f = {(const signed char*)x, (const signed char*)w, out, ldx, ldw, ldo, scales, M, N, K, ceil_div(N, 16), 0, 0};
+  const int chunks = ceil_div(K, kChunk), grid = f.groups < oi_sm_count() ? f.groups : oi_sm_count();
+  const long long wanted = (long long)ceil_div(f.groups, grid) * chunks;
+  f.stages = wanted < kFewMostStages ? (int)wanted : kFewMostStages;
+  f.at_once = wanted <= kFewMostStages;
+  const int smem = kFewPart + f.stages * (kFewStage + 16) + 16;
+  auto go = [&](auto kernel, bool (&allowed)[64]) {
+    if (int bad = allow_smem(kernel, kFewPart + kFewMostStages * (kFewStage + 16) + 16, allowed)) return bad;
+    oi_launch(kernel, grid, kFewThreads, smem, s, f);
+    return (int)OI_OK;
+  };
+  static bool allowed[8][64];
+  int rc;
+  if (M <= 8)
+    rc = chunks <= 1 ? go(linear_int8_few_kernel<1, 2, TOut>, allowed[0]) : chunks <= 2 ? go(linear_int8_few_kernel<1, 4, TOut>, allowed[1])
+         : chunks <= 4 ? go(linear_int8_few_kernel<1, 8, TOut>, allowed[2]) : go(linear_int8_few_kernel<1, 12, TOut>, allowed[3]);
+  else
+    rc = chunks <= 1 ? go(linear_int8_few_kernel<2, 2, TOut>, allowed[4]) : chunks <= 2 ? go(linear_int8_few_kernel<2, 4, TOut>, allowed[5])
+         : go(linear_int8_few_kernel<2, 8, TOut>, allowed[6]);
+  if (rc) return rc;
+  OI_CHECK_LAUNCH();
+  return OI_OK;
+}
+
 // What a product takes in us, from what was measured (B200; N 32 to 152,000, K 128 to 16,000, 1 to 8,192 rows), to choose a kernel, its
 // tiles of x and the slices of K. Over 150 sizes, most of them drawn, the choice took at most 1.24 times the fastest choice's time, in the
 // median 1.00.
@@ -603,6 +842,14 @@ float few_rows_us(int M, int N, int num_kb, int c, int z, int sms) {
   const float results = c > 1 ? 0.5f + 0.038f * cols : (bn > 128 ? 0.008f : 0.006f) * bn;
   const float around = 2.3f + results * on_an_sm, copies = memory > l2 ? memory : l2, work = products + (rounds - 1.f) * around;
   return around + (work > copies ? work : copies);
+}
+// Up to 16 rows on mma.sync: 16 rows of w after another, a stage of 2,048 bytes of each at the copy rate or the barrier behind them; x
+// into registers.
+float few_us(int M, int N, int K, int sms) {
+  const int groups = ceil_div(ceil_div(N, 16), sms), chunks = ceil_div(K, kChunk);
+  const float bytes = (float)K / (chunks * kChunk);
+  const float stage = M <= 8 ? (0.72f * bytes > 0.58f / chunks ? 0.72f * bytes : 0.58f / chunks) : (0.9f * bytes > 0.7f / chunks ? 0.9f * bytes : 0.7f / chunks);
+  return (M <= 8 ? 1.4f : 1.6f + 0.0002f * K) + groups * chunks * stage;
 }
 float many_rows_us(int M, int N, int num_kb, int bn, bool f32, bool on_borders, int sms) {
   const long long tiles = (long long)ceil_div(M, bn) * ceil_div(N, 256);
@@ -631,6 +878,7 @@ int launch(TOut* out, long long ldo, const void* x, long long ldx, const void* w
         if (us < best) best = us, best_c = c, best_z = z;
       }
   }
+  if (M <= 16 && K <= few_longest(M) && few_us(M, N, K, sms) < best) return launch_few(out, ldo, x, ldx, w, ldw, scales, M, N, K, s);
   return best_c ? launch_rows(out, ldo, x, ldx, w, ldw, scales, M, N, K, best_c, best_z, s) : launch_pair(out, ldo, x, ldx, w, ldw, scales, M, N, K, best_bn, s);
 }
 

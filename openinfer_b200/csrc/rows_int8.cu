@@ -164,11 +164,11 @@ struct GateRow {
   __device__ __forceinline__ float again(int d) const { return glu_act<true>(to_f32(at(d)[0]), to_f32(at(d)[block]), act, 0.f); }
 };
 
-// A row in registers, UNITS times eight numbers a thread, read once: by LANES of a warp (rows of up to 1,024 numbers, several rows a
-// block) or, LANES 0, by a block. early: the next kernel may be scheduled while this one runs (not where the rows may be those of a
+// A row in registers, UNITS times eight numbers a thread, read once: by LANES of a warp (short rows, several a block) or, LANES 0, by a block. early: the next kernel may be scheduled while this one runs (not where the rows may be those of a
 // weight: a product fetches its weight before it waits). kVec: 16 bytes a load, eight neighbours a thread; else neighbours lie in neighbouring threads and the bytes
 // are put together in shared memory. One exchange between the warps: the largest magnitude and a norm's sum of squares at
-// once. How a row is shared out goes by its length alone, so that a row's result does not depend on how many there are.
+// once. How a norm's row is shared out goes by its length alone, so that its
+// result does not depend on how many there are.
 template <typename Row, bool kVec, int UNITS, int LANES>
 __global__ void __launch_bounds__(LANES || UNITS == 1 ? 256 : UNITS == 2 ? 768 : 512)
 rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows, int cols, int early) {
@@ -303,13 +303,20 @@ __global__ void __launch_bounds__(1024) long_rows_int8_kernel(Row row, signed ch
 template <typename Row, bool kVec>
 void launch_rows(const Row& row, signed char* q, long long ldq, float* scales, int rows, int cols, int early, cudaStream_t s) {
   const int units = ceil_div(cols, 8);
-  if (units <= 128) {
-    auto go = [&](auto kernel, int lanes) { oi_launch(kernel, ceil_div(rows, 256 / lanes), 256, kVec ? 0 : 8 * 1024, s, row, q, ldq, scales, rows, cols, early); };
+  if (units <= 64) {
+    auto go = [&](auto kernel, int lanes) { oi_launch(kernel, ceil_div(rows, 256 / lanes), 256, kVec ? 0 : 8 * 512, s, row, q, ldq, scales, rows, cols, early); };
     if (units <= 16) go(rows_int8_kernel<Row, kVec, 1, 16>, 16);
     else if (units <= 32) go(rows_int8_kernel<Row, kVec, 1, 32>, 32);
-    else if (units <= 64) go(rows_int8_kernel<Row, kVec, 2, 32>, 32);
-    else go(rows_int8_kernel<Row, kVec, 4, 32>, 32);
+    else go(rows_int8_kernel<Row, kVec, 2, 32>, 32);
     return;
+  }
+  // Rows of up to 1,024 in a block are back sooner (one row, us: norm 3.7 in a warp, 1.8 so), in a warp there are more of them on the way
+  // (8,192 rows: 5.1, and 6.2 in blocks). A norm's sum has one order whatever the number of rows; without one, either will do.
+  if constexpr (!Row::kNorm) {
+    if (units > 96 && units <= 128 && rows >= 2048) {
+      oi_launch(rows_int8_kernel<Row, kVec, 4, 32>, ceil_div(rows, 8), 256, kVec ? 0 : 8 * 1024, s, row, q, ldq, scales, rows, cols, early);
+      return;
+    }
   }
   auto go = [&](auto kernel, int each) {
     oi_launch(kernel, rows, ceil_div(ceil_div(units, each), 32) * 32, kVec ? 0 : ceil_div(cols, 16) * 16, s, row, q, ldq, scales, rows, cols, early);

@@ -98,6 +98,11 @@ __device__ __forceinline__ void bulk_wait() {
 }
 // what this thread wrote to shared memory by plain stores is there for copies issued later
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+// `bytes` (a multiple of 16) from 16-byte aligned global to 16-byte aligned shared memory, with an L2 cache policy
+__device__ __forceinline__ void bulk_load_hint(unsigned dst, const void* src, unsigned bytes, unsigned bar, unsigned long long policy) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;\n"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy) : "memory");
+}
 __device__ __forceinline__ unsigned long long policy_evict_first() {
   unsigned long long p;
   asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(p));

@@ -234,6 +234,10 @@ TILES = [(370, 2972, 7657), (574, 7354, 3863), (309, 8746, 3887), (629, 8798, 26
           (2455, 147, 3658), (1765, 513, 9245), (17, 34, 1061), (3053, 32, 3017), (105, 3407, 6918), (71, 2413, 5902), (129, 2256, 14702),
           (1, 32, 401), (33, 2092, 2422), (3112, 32, 5562), (2099, 32, 2845), (269, 1898, 7347), (21, 32, 786), (389, 36, 1449), (105, 1506, 10930),
           (65, 1113, 9920), (130, 1413, 14655), (1, 33, 917), (33, 830, 4806), (1164, 34, 14005), (812, 33, 5825), (22, 32, 977), (409, 36, 2770)]
+# Up to 16 rows: every length of the registers that hold x, one and two groups of eight rows, rows of w that the ring holds and that it does not
+FEW = [(8, 32, 8836), (7, 126, 9360), (1, 32, 33), (5, 46, 32), (8, 34, 2234), (3, 39, 2064), (2, 33, 4292), (8, 47, 5408), (10, 42, 34), (13, 34, 32),
+       (16, 37, 2310), (14, 32, 2736), (9, 38, 4452), (16, 32, 5328), (8, 3650, 9116), (2, 4034, 8944), (1, 14218, 1377), (5, 14860, 1312),
+       (8, 7377, 2220), (1, 13154, 2544), (4, 3073, 6529), (8, 4796, 4720), (16, 8629, 2049), (12, 2369, 8192), (16, 2368, 4096), (6, 150, 12288)]
 
 
 @pytest.mark.parametrize("rows,channels,width", SHAPES)
@@ -252,7 +256,7 @@ def test_product(int8, rows, channels, width):
             assert torch.equal(out[:, :channels].cpu(), product_exactly(x, sx, w, sw, bias, dtype)) and bool((out[:, channels:] == -7.0).all())
 
 
-@pytest.mark.parametrize("rows,channels,width", TILES)
+@pytest.mark.parametrize("rows,channels,width", TILES + FEW)
 def test_product_by_every_kind_of_tile(int8, rows, channels, width):
     (x, sx), (w, sw) = integers(rows, width, 1), integers(channels, width, 2)
     bias = randn(channels, seed=3)
