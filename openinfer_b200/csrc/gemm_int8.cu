@@ -53,7 +53,11 @@ struct Scales {
 //   the others (four to sixteen) read the accumulator (one row of w a thread) and deposit, or with c = 1 scale and store; then
 //              all warps add up, scale and store.
 // What the results cost shows in the instructions per column: with a column at a time, a branch and a cluster address each, and
-// six warps, 128 columns took 8,000 cycles to deposit and 8,700 to store (N 1024, K 1024, c 1).
+// six warps, 128 columns took 8,000 cycles to deposit and 8,700 to store (N 1024, K 1024, c 1); stored two channels a lane, by lanes that
+// trade halves, 4.6 us instead of 4.3 (500 x 4095 x 512).
+// Measured (us; what its bytes at the copy rate and its operations at twice the bfloat16 rate take): 32 x 24576 x 4096 19.6 (15.6),
+// 64 x 6144 x 4096 9.8 (4.0), 512 x 4096 x 4096 11.2 (5.2), 264 x 4096 x 12288 18.8 (8.5), a head of 151936 x 4096 with 64 rows 102 (98).
+// Bound by what one SM takes in (some 110 GB/s, 32 KB a stage of 128 rows) and, short sums, by launch, x, results.
 constexpr int kFewColumns = 32, kMoreColumns = 64;      // up to so many rows of x a tile four warps read results, or eight, else sixteen
 
 struct Shape {
@@ -109,12 +113,6 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
       tc::tma_load_2d(smem_base + s * stage_bytes, &map_w, (kb0 + s) * BK, n0, full_bar(s));
     }
   }
-  // what the sums are multiplied by is fetched under the copies: a channel's scale in its thread, later every row's in shared memory
-  const int cols = min(g.bn, g.M - m0);  // rows of x in this tile
-  const int quarter = warp & 3;          // a warp may only touch lanes [32 * (warp % 4), +32) of tensor memory
-  const int rows_mine = BM / csize;      // channels that this CTA adds up
-  const int n = n0 + (csize > 1 ? rank * rows_mine + (int)threadIdx.x % rows_mine : quarter * 32 + lane);
-  const float sw = n < g.N ? scales.sw[n] : 0.f;
   pdl_wait();
   if (warp == 1) {
     tc::tmem_alloc(tc::smem_u32(tmem_slot), g.tmem_cols);
@@ -125,6 +123,12 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     for (int s = 0; s < pre; ++s)
       tc::tma_load_2d(smem_base + s * stage_bytes + kBoxBytes, &map_x, (kb0 + s) * BK, m0, full_bar(s));
   }
+  // what the sums are multiplied by is fetched under the copies: a channel's scale in its thread, later every row's in shared memory
+  const int cols = min(g.bn, g.M - m0);  // rows of x in this tile
+  const int quarter = warp & 3;          // a warp may only touch lanes [32 * (warp % 4), +32) of tensor memory
+  const int rows_mine = BM / csize;      // channels that this CTA adds up
+  const int n = n0 + (csize > 1 ? rank * rows_mine + (int)threadIdx.x % rows_mine : quarter * 32 + lane);
+  const float sw = n < g.N ? scales.sw[n] : 0.f;
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -273,7 +277,11 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 //   warp 1      of the even CTA issues the products (M = 256, N = bn, K = 32) for both
 //   warps 2-17  of both CTAs drain their own tensor memory (32 channels a warp, every fourth group of rows) and arrive on the even
 //               CTA's "drained" barrier. A warp scales 32 channels of a few rows, turns them in shared memory, and a TMA store carries
-//               them out: 4096 x 4096 x 512 takes 16.5 us so (float32 20.8), 19.7 (28.8) with 16-byte stores by the warps.
+//               them out: 4096 x 4096 x 512 takes 18.5 us so (float32 21; 16.5 with channels across the tile, whose rows need
+//               no turning, but then tiles are 256 rows high), with 16-byte stores by the warps 3 and 8 more.
+// Measured (us; at twice the bfloat16 rate): 8192 x 24576 x 4096 496 (502; 3.33 POP/s, the library's bfloat16 product 1017), 2048 x 4096 x 4096
+// 26 (21), 777 x 24576 x 4096 63 (48; tiles of 256 rows 71), 264 x 24576 x 4096 31 (17.5; 36). Bound by the tensor cores and their power
+// where tiles fill the pairs evenly, else by the last round of them; with K of 512 by the results.
 constexpr int kEpilogueWarps = 16;
 constexpr int kParts = kEpilogueWarps / 4;                          // the warps of a quarter of the lanes share the rows of x
 constexpr int kPairThreads = 64 + 32 * kEpilogueWarps;
@@ -625,7 +633,6 @@ linear_int8_few_kernel(const __grid_constant__ FewArgs a) {
     const bool biased = a.scales.bias != nullptr;
     auto channel = [&](int first) { return ((long long)first + f * (int)gridDim.x) * 16 + col; };
     auto asked = [&](const float* of, int first) { return channel(first) < a.N ? of[channel(first)] : 0.f; };
-    float next_sw = asked(a.scales.sw, blockIdx.x);          // a batch ahead
     bool ok = wait_on(full_bar(0), 0, abort_flag, 22);       // weights: not waited for behind x
     pdl_wait();
     uint4 xr[B][NT][2];
@@ -639,6 +646,7 @@ linear_int8_few_kernel(const __grid_constant__ FewArgs a) {
       }
     }
     const float sx = m < a.M ? a.scales.sx[m] : 0.f;
+    float next_sw = asked(a.scales.sw, blockIdx.x);          // a batch ahead
     float next_b = biased ? asked(a.scales.bias, blockIdx.x) : 0.f, sw = 0.f, b = 0.f;
 
     Ring at;

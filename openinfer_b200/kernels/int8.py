@@ -39,6 +39,9 @@ class Int8Rows(NamedTuple):
     scales: torch.Tensor
 
 
+_new_rows = tuple.__new__
+
+
 # At a few rows a call's time is the host's. So a tensor is asked for each thing once, one test covers all that may be wrong, and what
 # exactly it was is found out behind it.
 
@@ -79,11 +82,16 @@ def _cuda(device: int, what: str) -> None:
         raise KernelError(f"{what}: the tensor is not on a CUDA device; this package has no CPU path")
 
 
+def _elsewhere(device: int) -> bool:
+    """Whether tensors are on another CUDA device than the calling thread's current one: the call is then made again on theirs."""
+    return device >= 0 and device != _lib.current_device()
+
+
 def empty_rows(rows: int, width: int, device) -> Int8Rows:
     """Room for rows of 8-bit integers."""
     values = (torch.empty_strided((rows, width), (-(-width // APART) * APART, 1), dtype=torch.int8, device=device) if width % APART
               else torch.empty(rows, width, dtype=torch.int8, device=device))
-    return Int8Rows(values, torch.empty(rows, dtype=torch.float32, device=device))
+    return _new_rows(Int8Rows, (values, torch.empty(rows, dtype=torch.float32, device=device)))
 
 
 def _room(out: Optional[Int8Rows], x: torch.Tensor, rows: int, width: int, device: int, what: str):
@@ -99,25 +107,19 @@ def _room(out: Optional[Int8Rows], x: torch.Tensor, rows: int, width: int, devic
     return out, address, stride, scales
 
 
-def _launch(device: int, what: str, entry, *args) -> None:
-    """Calls an entry point with the current stream of the tensors' own device, whatever the calling thread's current one is."""
-    if device == _lib.current_device():
-        code = entry(*args, _lib.current_stream())
-    else:
-        with torch.cuda.device(device):
-            code = entry(*args, _lib.current_stream())
-    if code:
-        _lib.check(code, what)
-
-
 def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
     """The rows of ``x`` [rows, width] (float32 or bfloat16, row stride free) as 8-bit integers."""
     code, rows, width, stride = _float_rows(x, "quantize_int8")
     device = x.get_device()
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return quantize_int8(x, out)
     held, q, ldq, scales = _room(out, x, rows, width, device, "quantize_int8")
     if rows:
         L = _lib.load()
-        _launch(device, "quantize_int8", L.oi_quantize_int8, q, ldq, scales, x.data_ptr(), code, stride, rows, width, out is None)
+        failed = L.oi_quantize_int8(q, ldq, scales, x.data_ptr(), code, stride, rows, width, out is None, _lib.current_stream())
+        if failed:
+            _lib.check(failed, "quantize_int8")
         if out is not None:
             L.oi_launch_fence()      # it may be a weight's memory, which products fetch ahead: the next launch starts behind this one
     return held
@@ -143,11 +145,16 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, delta: Op
         if (d_address < address + ((rows - 1) * stride + width) * size and address < d_address + ((rows - 1) * d_stride + width) * size
                 and rows and (d_address, d_stride) != (address, stride)):
             raise KernelError("rmsnorm_int8: x and delta must be the same rows or not overlap")
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return rmsnorm_int8(x, weight, eps, delta=delta, weight_offset=weight_offset, out=out)
     held, q, ldq, scales = _room(out, x, rows, width, device, "rmsnorm_int8")
     if rows:
         L = _lib.load()
-        _launch(device, "rmsnorm_int8", L.oi_rmsnorm_int8, q, ldq, scales, address, stride, d_address, d_stride, code, weight.data_ptr(),
-                w_code, rows, width, eps, weight_offset, out is None)
+        failed = L.oi_rmsnorm_int8(q, ldq, scales, address, stride, d_address, d_stride, code, weight.data_ptr(), w_code, rows, width, eps,
+                                   weight_offset, out is None, _lib.current_stream())
+        if failed:
+            _lib.check(failed, "rmsnorm_int8")
         if out is not None:
             L.oi_launch_fence()      # as in quantize_int8
     return held
@@ -163,10 +170,15 @@ def silu_mul_int8(gate_up: torch.Tensor, block: Optional[int] = None, act: str =
         raise KernelError(f"silu_mul_int8: gate_up of {both} numbers in blocks of {block} gates and {block} ups")
     act_c = act_code(act)
     device = gate_up.get_device()
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return silu_mul_int8(gate_up, block, act, out)
     held, q, ldq, scales = _room(out, gate_up, rows, inter, device, "silu_mul_int8")
     if rows:
         L = _lib.load()
-        _launch(device, "silu_mul_int8", L.oi_silu_mul_int8, q, ldq, scales, gate_up.data_ptr(), code, stride, rows, inter, block, act_c, out is None)
+        failed = L.oi_silu_mul_int8(q, ldq, scales, gate_up.data_ptr(), code, stride, rows, inter, block, act_c, out is None, _lib.current_stream())
+        if failed:
+            _lib.check(failed, "silu_mul_int8")
         if out is not None:
             L.oi_launch_fence()      # as in quantize_int8
     return held
@@ -192,9 +204,14 @@ def _results(out: Optional[torch.Tensor], dtype: torch.dtype, rows: int, width: 
 def dequantize_int8(rows: Int8Rows, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The numbers that 8-bit rows stand for, rounded once to ``dtype`` (float32 or bfloat16) or to that of ``out`` (row stride free)."""
     q, ldq, count, width, scales, device = _int8_rows(*rows, "dequantize_int8")
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return dequantize_int8(rows, dtype, out)
     out, code, stride = _results(out, dtype, count, width, rows[0], device, "dequantize_int8")
     if count:
-        _launch(device, "dequantize_int8", _lib.load().oi_dequantize_int8, out.data_ptr(), code, stride, q, ldq, scales, count, width)
+        failed = _lib.load().oi_dequantize_int8(out.data_ptr(), code, stride, q, ldq, scales, count, width, _lib.current_stream())
+        if failed:
+            _lib.check(failed, "dequantize_int8")
     return out
 
 
@@ -202,11 +219,12 @@ class Int8Weight:
     """A weight [channels, width] for ``linear_int8``: int8 values with a float32 scale for each output channel, laid out once.
 
     Values whose rows do not start on 16-byte borders, or are wider than 64 and not a multiple of 64 bytes apart, are copied into rows
-    that are; others are kept as they are. A product
-    fetches its weight while the kernel ahead of it on the stream still runs, but for the first one on each stream. Later
-    changes of the weight's tensors (by torch, or through ``out`` of the functions above) are ordered by the stream as ever."""
+    that are; others are kept as they are. A product fetches its weight's values while the kernel ahead of it on the stream still
+    runs, but for the first one on each stream and the first one after a change of the weight's tensors, by torch or through ``out``
+    of the functions above. Of a change that torch does not count (through ``.data``, or of tensors made in inference mode) tell
+    with ``changed()``."""
 
-    __slots__ = ("values", "scales", "channels", "width", "device", "stream", "_seen", "_operands")
+    __slots__ = ("values", "scales", "channels", "width", "device", "stream", "_seen", "_operands", "_counted")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor) -> None:
         if values.dim() != 2 or values.dtype != torch.int8 or scales.shape != values.shape[:1]:
@@ -223,13 +241,17 @@ class Int8Weight:
         self.values, self.scales, self.device = values, scales.contiguous(), values.device
         self.channels, self.width = rows, width
         self.stream = None          # of the last product: what wrote the weight is known to be done there
-        self._seen = None
+        self._seen, self._counted = None, not self.values.is_inference()
         self.operands()
 
+    def changed(self) -> None:
+        """The weight's tensors hold new values: the next product waits for what is ahead of it."""
+        self.stream = None
+
     def operands(self):
-        """What ``_int8_rows`` says of the weight; asked again when its tensors have been given other memory."""
+        """What ``_int8_rows`` says of the weight; asked again when its tensors have been given other memory or values."""
         values, scales = self.values, self.scales
-        seen = (values.data_ptr(), scales.data_ptr(), values.shape, values.stride(), scales.shape)
+        seen = (values.data_ptr(), scales.data_ptr(), values.shape, values.stride(), scales.shape, values._version if self._counted else 0)
         if seen != self._seen:
             self._operands = _int8_rows(values, scales, "Int8Weight")
             self._seen, self.stream = seen, None
@@ -250,29 +272,24 @@ def linear_int8(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = 
     w, ldw, channels, w_width, w_scales, w_device = weight.operands()
     if width != w_width or device != w_device:
         raise KernelError(f"linear_int8: rows of {width} on {x[0].device} and a weight of {channels} x {w_width} on {weight.device}")
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return linear_int8(x, weight, bias, out_dtype, out)
     b = 0
     if bias is not None:
         if bias.dtype != torch.float32 or bias.shape != (channels,) or not bias.is_contiguous() or bias.get_device() != device:
             raise KernelError(f"linear_int8: expected {channels} float32 numbers of bias on {x[0].device}: {bias.dtype} {tuple(bias.shape)} on {bias.device}")
         b = bias.data_ptr()
-    out, code, stride = _results(out, out_dtype, rows, channels, x[0], device, "linear_int8")
+    out, code, out_stride = _results(out, out_dtype, rows, channels, x[0], device, "linear_int8")
     if rows and channels:
-        if device == _lib.current_device():
-            _product(weight, out.data_ptr(), code, stride, q, ldq, scales, w, ldw, w_scales, b, rows, channels, width)
-        else:
-            with torch.cuda.device(device):
-                _product(weight, out.data_ptr(), code, stride, q, ldq, scales, w, ldw, w_scales, b, rows, channels, width)
+        L, stream = _lib.load(), _lib.current_stream()
+        if weight.stream != stream:
+            L.oi_launch_fence()          # the first product on a stream starts when all that is ahead of it has finished
+            weight.stream = stream
+        failed = L.oi_linear_int8(out.data_ptr(), code, out_stride, q, ldq, scales, w, ldw, w_scales, b, rows, channels, width, stream)
+        if failed:
+            _lib.check(failed, "linear_int8")
     return out
-
-
-def _product(weight: Int8Weight, *args) -> None:
-    L, stream = _lib.load(), _lib.current_stream()
-    if weight.stream != stream:
-        L.oi_launch_fence()          # the first product on a stream starts when all that is ahead of it has finished
-        weight.stream = stream
-    code = L.oi_linear_int8(*args, stream)
-    if code:
-        _lib.check(code, "linear_int8")
 
 
 def status() -> int:

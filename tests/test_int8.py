@@ -55,6 +55,25 @@ def test_more_rows_than_an_entry_point_counts():
     refused("at most 1073741824", int8.dequantize_int8, int8.Int8Rows(torch.zeros(1, 1, dtype=torch.int8).expand(2 ** 31 + 5, 1), torch.ones(3)))
 
 
+def test_a_weight_that_torch_changes_is_waited_for_again():
+    w = int8.Int8Weight(ROWS.clone(), SCALES.clone())
+    w.operands()
+    w.stream = 7
+    w.operands()
+    assert w.stream == 7
+    w.values.fill_(3)
+    w.operands()
+    assert w.stream is None
+    w.stream = 7
+    w.changed()
+    assert w.stream is None
+    with torch.inference_mode():
+        w = int8.Int8Weight(ROWS.clone(), SCALES.clone())
+    w.stream = 7
+    w.operands()
+    assert w.stream == 7
+
+
 def test_norm():
     def norm(x=X, w=torch.ones(32), **kw):
         int8.rmsnorm_int8(x, w, 1e-6, **kw)

@@ -431,6 +431,35 @@ def test_two_streams_at_once(int8):
         assert all(torch.equal(w, g) for g in several)
 
 
+def test_tensors_on_another_device_than_the_current_one(int8, monkeypatch):
+    """Each call is made under the tensors' own device, and only there."""
+    current, entered = [5], []
+
+    class Device:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            entered.append(self.device)
+            self.was, current[0] = current[0], self.device
+
+        def __exit__(self, *exc):
+            current[0] = self.was
+
+    x, w = randn(6, 512).to(DEV), randn(40, 512, seed=1).to(DEV)
+    weight = int8.Int8Weight.quantize(w)
+    norm_w = torch.ones(512, device=DEV)
+    calls = (lambda: int8.quantize_int8(x).values, lambda: int8.rmsnorm_int8(x, norm_w, 1e-6).values, lambda: int8.silu_mul_int8(x, block=8).values,
+             lambda: int8.dequantize_int8(int8.Int8Rows(weight.values, weight.scales)), lambda: int8.linear_int8(held, weight))
+    held = int8.quantize_int8(x)
+    want = [c() for c in calls]
+    monkeypatch.setattr(int8._lib, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    got = [c() for c in calls]
+    assert entered == [0] * len(calls) and current == [5]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_results_that_lie_beyond_2_to_the_31(int8):
     """70,000 rows of 32,768 results: the last ones begin 2.3e9 numbers behind the first."""
     rows, channels = 70000, 32768
