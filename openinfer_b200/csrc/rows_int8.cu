@@ -12,6 +12,17 @@ namespace {
 // |y| as bits: ordered like the numbers, infinities above all finite ones and NaNs above those
 __device__ __forceinline__ unsigned magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
 
+// act(gate) * up by the special-function unit's exponential and reciprocal (2 ulp each): what follows is a rounding to 8 bits. A gate far
+// below zero is an infinite exponential and a zero.
+template <int ACT>
+__device__ __forceinline__ float gated(float g, float u) {
+  const float t = ACT == OI_ACT_GELU_TANH ? 1.5957691216057308f * (g + 0.044715f * g * g * g) : g;
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(e) : "f"(-1.4426950408889634f * t));
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(1.f + e));
+  return g * r * u;
+}
+
 // What a row is multiplied by, from the largest magnitude of its numbers. A norm's rows come without the reciprocal root mean
 // square `common`, which all of a row shares: q does not depend on it, the scale takes it up.
 struct RowScale {
@@ -27,11 +38,9 @@ struct RowScale {
     scale = keep ? (most * common) / 127.f : __uint_as_float(0x7fffffffu);
     if (tiny) scale *= 0x1p-80f;
   }
-  // round(y * inv) in the low byte: added to 1.5 * 2^23, the sum's last bit stands for one (ties to even, as the sum is rounded)
-  __device__ __forceinline__ unsigned byte(float y) const {
-    if (tiny) y *= 0x1p80f;
-    return __float_as_uint(__fadd_rn(__fmul_rn(y, inv), 12582912.f));
-  }
+  // round(y * inv) in the low byte: added to 1.5 * 2^23, the sum's last bit stands for one (ties to even, as the sum is rounded).
+  // Of a tiny row: y times 2^80.
+  __device__ __forceinline__ unsigned byte(float y) const { return __float_as_uint(__fadd_rn(__fmul_rn(y, inv), 12582912.f)); }
   __device__ __forceinline__ unsigned four(float a, float b, float c, float d) const {
     return __byte_perm(__byte_perm(byte(a), byte(b), 0x0040), __byte_perm(byte(c), byte(d), 0x0040), 0x5410) & keep;
   }
@@ -55,6 +64,17 @@ struct Eight {
     } else {
       const unsigned w = reinterpret_cast<const unsigned*>(v)[e >> 1];
       return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+    }
+  }
+  // each number plus the other's, rounded once
+  __device__ __forceinline__ void add(const Eight& other) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) set(e, get(e) + other.get(e));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        reinterpret_cast<__nv_bfloat162*>(v)[i] = __hadd2(reinterpret_cast<const __nv_bfloat162*>(v)[i], reinterpret_cast<const __nv_bfloat162*>(other.v)[i]);
     }
   }
   __device__ __forceinline__ void set(int e, T x) {
@@ -111,8 +131,7 @@ struct NormRow {
   }
   __device__ __forceinline__ void make(int d, Raw& raw, float (&y)[8], float& squares) const {
     if (delta) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) raw.x.set(e, from_f32<T>(raw.x.get(e) + raw.delta.get(e)));
+      raw.x.add(raw.delta);
       raw.x.store(x + d);
     }
     float wv[8];
@@ -151,12 +170,11 @@ struct NormRow {
   __device__ __forceinline__ float again(int d) const { return to_f32(x[d]) * (w_offset + load_as_f32(w, w_dtype, d)); }
 };
 
-// The activation by the special-function unit's exponential and reciprocal (2 ulp each): what follows is a rounding to 8 bits
-template <typename T>
+template <typename T, int ACT>
 struct GateRow {
   const T* x;
   long long ldx;
-  int block, act, shift;     // shift: of a block that is a power of two; -1: all gates, then all ups; -2: any other
+  int block, shift;     // shift: of a block that is a power of two; -1: all gates, then all ups; -2: any other
   static constexpr bool kNorm = false;
   struct Raw { Eight<T> gate, up; };
   __device__ __forceinline__ void begin(long long r) { x += r * ldx; }
@@ -167,12 +185,12 @@ struct GateRow {
   }
   __device__ __forceinline__ void make(int d, Raw& raw, float (&y)[8], float& squares) const {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = glu_act<true>(raw.gate.get(e), raw.up.get(e), act, 0.f);
+    for (int e = 0; e < 8; ++e) y[e] = gated<ACT>(raw.gate.get(e), raw.up.get(e));
   }
   struct RawOne { T gate, up; };
   __device__ __forceinline__ void fetch_one(int d, RawOne& raw) const { raw.gate = at(d)[0], raw.up = at(d)[block]; }
-  __device__ __forceinline__ float make_one(int d, const RawOne& raw, float& squares) const { return glu_act<true>(to_f32(raw.gate), to_f32(raw.up), act, 0.f); }
-  __device__ __forceinline__ float again(int d) const { return glu_act<true>(to_f32(at(d)[0]), to_f32(at(d)[block]), act, 0.f); }
+  __device__ __forceinline__ float make_one(int d, const RawOne& raw, float& squares) const { return gated<ACT>(to_f32(raw.gate), to_f32(raw.up)); }
+  __device__ __forceinline__ float again(int d) const { return gated<ACT>(to_f32(at(d)[0]), to_f32(at(d)[block])); }
 };
 
 // A row in registers, UNITS times eight numbers a thread, read once: by LANES of a warp (short rows, several a block) or, LANES 0, by
@@ -251,7 +269,7 @@ rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows
     }
   }
 #pragma unroll
-  for (int i = 0; i < UNITS * 8; ++i) most = max(most, magnitude(y[i / 8][i % 8]));
+  for (int i = 0; i < UNITS * 8; i += 2) most = __vimax3_u32(most, magnitude(y[i / 8][i % 8]), magnitude(y[i / 8][i % 8 + 1]));
   if constexpr (LANES > 0 && LANES < 32) {
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) {
@@ -276,6 +294,10 @@ rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows
   if constexpr (Row::kNorm) common = rsqrtf(squares / (float)row_cols + row.eps);
   const RowScale s(most, common);
   if (me == 0 && (!LANES || live)) scales[r] = s.scale;
+  if (s.tiny) {
+#pragma unroll
+    for (int i = 0; i < UNITS * 8; ++i) y[i / 8][i % 8] *= 0x1p80f;
+  }
   if constexpr (kVec) {
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
@@ -333,7 +355,7 @@ __global__ void __launch_bounds__(1024) long_rows_int8_kernel(Row row, signed ch
   float common = 1.f;
   if constexpr (Row::kNorm) common = rsqrtf(warp_sum(part_squares[threadIdx.x & 31]) / (float)cols + row.eps);
   const RowScale s(most, common);
-  for (int d = threadIdx.x; d < cols; d += 1024) q[d] = (signed char)(s.byte(row.again(d)) & s.keep);
+  for (int d = threadIdx.x; d < cols; d += 1024) q[d] = (signed char)(s.byte(s.tiny ? row.again(d) * 0x1p80f : row.again(d)) & s.keep);
   if (threadIdx.x == 0) scales[r] = s.scale;
 }
 
@@ -481,8 +503,12 @@ OI_API int oi_silu_mul_int8(void* q, long long ldq, float* scales, const void* g
   if (shift == -2 && (block & (block - 1)) == 0)
     for (shift = 0; 1 << shift < block; ++shift) {}
   const bool vec = block % 8 == 0 && on_borders(gate_up, ldx, dtype == OI_F32 ? 4 : 2);
-  if (dtype == OI_F32) return launch(GateRow<float>{(const float*)gate_up, ldx, block, act, shift}, vec, q, ldq, scales, rows, inter, early, s);
-  return launch(GateRow<bf16>{(const bf16*)gate_up, ldx, block, act, shift}, vec, q, ldq, scales, rows, inter, early, s);
+  auto go = [&](auto row) { return launch(row, vec, q, ldq, scales, rows, inter, early, s); };
+  if (dtype == OI_F32)
+    return act == OI_ACT_SILU ? go(GateRow<float, OI_ACT_SILU>{(const float*)gate_up, ldx, block, shift})
+                              : go(GateRow<float, OI_ACT_GELU_TANH>{(const float*)gate_up, ldx, block, shift});
+  return act == OI_ACT_SILU ? go(GateRow<bf16, OI_ACT_SILU>{(const bf16*)gate_up, ldx, block, shift})
+                            : go(GateRow<bf16, OI_ACT_GELU_TANH>{(const bf16*)gate_up, ldx, block, shift});
 }
 
 // out[r, :] = round(q[r, :] * scales[r]) (row stride ldo elements)
