@@ -77,6 +77,10 @@ struct Eight {
         reinterpret_cast<__nv_bfloat162*>(v)[i] = __hadd2(reinterpret_cast<const __nv_bfloat162*>(v)[i], reinterpret_cast<const __nv_bfloat162*>(other.v)[i]);
     }
   }
+  __device__ __forceinline__ void set_pair(int e, float a, float b) {      // e even
+    if constexpr (sizeof(T) == 4) set(e, a), set(e + 1, b);
+    else reinterpret_cast<__nv_bfloat162*>(v)[e >> 1] = __floats2bfloat162_rn(a, b);
+  }
   __device__ __forceinline__ void set(int e, T x) {
     if constexpr (sizeof(T) == 4) reinterpret_cast<unsigned*>(v)[e] = __float_as_uint(x);
     else {
@@ -400,53 +404,69 @@ int launch(const Row& row, bool vec, void* q, long long ldq, float* scales, int 
 bool on_borders(const void* p, long long ld, int esize) { return (uintptr_t)p % 16 == 0 && ld * esize % 16 == 0; }
 
 // Sixteen numbers a thread: neighbours where rows start on 16-byte borders, else one of each 1 << lanes_log; 256 >> lanes_log rows a
-// block (65536 x 128 with a block a row 69 us, 5.9 so; 8192 x 4096 19 us, 5.3 TB/s). A byte becomes a number without a conversion: with its sign turned it is the last byte of 2^23 + 128 + q.
-template <typename T, bool kVec, bool kWide>
+// block (65536 x 128 with a block a row 69 us, 5.9 so). Bound by memory: many long rows give a thread both its loads (kTimes 2) before
+// it stores (8192 x 4096 16.2 us, 6.2 TB/s, for 18.9 with one; 8 x 4096 1.5 for 1.3 and 8192 x 640 4.8 for 3.8, so one there).
+// A byte becomes a number without a conversion: with its sign turned it is the last byte of 2^23 + 128 + q.
+template <typename T, bool kVec, bool kWide, int kTimes>
 __global__ void __launch_bounds__(256) dequantize_kernel(T* out, long long ldo, const signed char* q, long long ldq, const float* scales, int rows,
                                                          int cols, int lanes_log) {
   pdl_start();
   if constexpr (kWide) lanes_log = 8;
   const int lanes = 1 << lanes_log, lane = threadIdx.x & (lanes - 1), step = kVec ? 1 : lanes;
   const long long r = ((long long)blockIdx.x << (8 - lanes_log)) + (threadIdx.x >> lanes_log);
-  const int d = blockIdx.y * (lanes * 16) + (kVec ? lane * 16 : lane);
-  if (r >= rows || d >= cols) return;
+  const int first = blockIdx.y * (lanes * 16 * kTimes) + (kVec ? lane * 16 : lane);
+  if (r >= rows || first >= cols) return;
   const float scale = scales[r];
   out += r * ldo;
   q += r * ldq;
-  if (kVec && d + 16 <= cols) {
-    const uint4 v = *reinterpret_cast<const uint4*>(q + d);
-    const unsigned words[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
+  uint4 v[kTimes];
+  if constexpr (kVec) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      Eight<T> o;
+    for (int i = 0; i < kTimes; ++i)
+      if (first + i * lanes * 16 + 16 <= cols) v[i] = *reinterpret_cast<const uint4*>(q + first + i * lanes * 16);
+  }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float f = __uint_as_float(__byte_perm(words[2 * h + e / 4], 0x4b000000u, 0x7650 + e % 4)) - 8388736.f;
-        o.set(e, from_f32<T>(f * scale));
+  for (int i = 0; i < kTimes; ++i) {
+    const int d = first + i * lanes * 16;
+    if (kVec && d + 16 <= cols) {
+      const unsigned words[4] = {v[i].x ^ 0x80808080u, v[i].y ^ 0x80808080u, v[i].z ^ 0x80808080u, v[i].w ^ 0x80808080u};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        Eight<T> o;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const unsigned word = words[2 * h + e / 4];
+          const float f0 = (__uint_as_float(__byte_perm(word, 0x4b000000u, 0x7650 + e % 4)) - 8388736.f) * scale;
+          const float f1 = (__uint_as_float(__byte_perm(word, 0x4b000000u, 0x7651 + e % 4)) - 8388736.f) * scale;
+          o.set_pair(e, f0, f1);
+        }
+        o.store(out + d + 8 * h);
       }
-      o.store(out + d + 8 * h);
+    } else {
+      signed char one[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) one[e] = d + e * step < cols ? q[d + e * step] : 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (d + e * step < cols) out[d + e * step] = from_f32<T>((float)one[e] * scale);
     }
-  } else {
-    signed char v[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = d + e * step < cols ? q[d + e * step] : 0;
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (d + e * step < cols) out[d + e * step] = from_f32<T>((float)v[e] * scale);
   }
 }
 
 template <typename T>
 int launch_dequantize(T* out, long long ldo, const signed char* q, long long ldq, const float* scales, int rows, int cols, cudaStream_t s) {
+  const bool vec = on_borders(out, rows > 1 ? ldo : 0, sizeof(T));
+  const bool two = vec && cols > 2048 && (long long)rows * cols >= 1 << 22;
+  const int each = two ? 32 : 16;
   int lanes_log = 0;
-  while (lanes_log < 8 && 16 << lanes_log < cols) ++lanes_log;
-  const dim3 grid(ceil_div(rows, 256 >> lanes_log), ceil_div(cols, 16 << lanes_log));
+  while (lanes_log < 8 && each << lanes_log < cols) ++lanes_log;
+  const dim3 grid(ceil_div(rows, 256 >> lanes_log), ceil_div(cols, each << lanes_log));
   OI_REQUIRE(grid.y <= 65535, "dequantize_int8: bad sizes rows=%d cols=%d", rows, cols);
-  const bool vec = on_borders(out, rows > 1 ? ldo : 0, sizeof(T)), wide = lanes_log == 8;
+  const bool wide = lanes_log == 8;
   auto go = [&](auto kernel) { oi_launch(kernel, grid, 256, 0, s, out, ldo, q, ldq, scales, rows, cols, lanes_log); };
-  if (vec) wide ? go(dequantize_kernel<T, true, true>) : go(dequantize_kernel<T, true, false>);
-  else wide ? go(dequantize_kernel<T, false, true>) : go(dequantize_kernel<T, false, false>);
-  OI_CHECK_LAUNCH();
+  if (two) wide ? go(dequantize_kernel<T, true, true, 2>) : go(dequantize_kernel<T, true, false, 2>);
+  else if (vec) wide ? go(dequantize_kernel<T, true, true, 1>) : go(dequantize_kernel<T, true, false, 1>);
+  else wide ? go(dequantize_kernel<T, false, true, 1>) : go(dequantize_kernel<T, false, false, 1>);
   return OI_OK;
 }
 
