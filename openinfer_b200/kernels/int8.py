@@ -18,6 +18,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import lib as _lib
 from .lib import KernelError
@@ -107,6 +108,14 @@ def _room(out: Optional[Int8Rows], x: torch.Tensor, rows: int, width: int, devic
     return out, address, stride, scales
 
 
+def _written(L, held: Int8Rows) -> None:
+    """Given rows have been written. They may be those of a weight, which products fetch ahead: a product by it sees the change, on
+    whatever stream it is, and this thread's next launch starts behind this one."""
+    L.oi_launch_fence()
+    if not held[0].is_inference():
+        increment_version(held[0])
+
+
 def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
     """The rows of ``x`` [rows, width] (float32 or bfloat16, row stride free) as 8-bit integers."""
     code, rows, width, stride = _float_rows(x, "quantize_int8")
@@ -121,7 +130,7 @@ def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
         if failed:
             _lib.check(failed, "quantize_int8")
         if out is not None:
-            L.oi_launch_fence()      # it may be a weight's memory, which products fetch ahead: the next launch starts behind this one
+            _written(L, held)
     return held
 
 
@@ -156,7 +165,7 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, delta: Op
         if failed:
             _lib.check(failed, "rmsnorm_int8")
         if out is not None:
-            L.oi_launch_fence()      # as in quantize_int8
+            _written(L, held)
     return held
 
 
@@ -180,7 +189,7 @@ def silu_mul_int8(gate_up: torch.Tensor, block: Optional[int] = None, act: str =
         if failed:
             _lib.check(failed, "silu_mul_int8")
         if out is not None:
-            L.oi_launch_fence()      # as in quantize_int8
+            _written(L, held)
     return held
 
 
@@ -244,6 +253,11 @@ class Int8Weight:
         self._seen, self._counted = None, not self.values.is_inference()
         self.operands()
 
+    def __setattr__(self, name: str, value) -> None:
+        object.__setattr__(self, name, value)
+        if name in ("values", "scales"):
+            object.__setattr__(self, "stream", None)      # other tensors: as after a change
+
     def changed(self) -> None:
         """The weight's tensors hold new values: the next product waits for what is ahead of it."""
         self.stream = None
@@ -285,10 +299,12 @@ def linear_int8(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = 
         L, stream = _lib.load(), _lib.current_stream()
         if weight.stream != stream:
             L.oi_launch_fence()          # the first product on a stream starts when all that is ahead of it has finished
-            weight.stream = stream
         failed = L.oi_linear_int8(out.data_ptr(), code, out_stride, q, ldq, scales, w, ldw, w_scales, b, rows, channels, width, stream)
         if failed:
+            weight.stream = None
             _lib.check(failed, "linear_int8")
+        if weight.stream != stream:
+            weight.stream = stream
     return out
 
 

@@ -145,3 +145,17 @@ def test_the_library_refuses_before_it_launches(name, args):
     L = klib.load(verbose=False)
     assert getattr(L, name)(*args, None) == 1
     assert name[3:].encode() in L.oi_last_error()
+
+
+def test_a_weight_given_other_tensors_is_waited_for_again():
+    w = int8.Int8Weight(ROWS.clone(), SCALES.clone())
+    for name in ("values", "scales"):
+        w.stream = 7
+        setattr(w, name, getattr(w, name).clone())
+        assert w.stream is None
+    w.stream = 7
+    w.operands()
+    assert w.stream is None                          # the new values' place is seen
+    w.stream = 7
+    w.operands()
+    assert w.stream == 7

@@ -337,6 +337,51 @@ def test_a_weight_that_is_written_again(int8, rows):
         assert torch.equal(g, want[i % 3])
 
 
+@pytest.mark.parametrize("write", ["quantize", "norm", "gate"])
+def test_a_weight_written_through_out_is_not_fetched_ahead_on_its_stream(int8, write):
+    """Another stream's launch comes between the write and the weight's next product on the writing stream."""
+    ws = [randn(64, 256, seed=s).to(DEV) for s in range(2)]
+    norm_w = torch.ones(128, device=DEV)
+    make = {"quantize": lambda x, **kw: int8.quantize_int8(x, **kw), "gate": lambda x, **kw: int8.silu_mul_int8(x, **kw),
+            "norm": lambda x, **kw: int8.rmsnorm_int8(x[:, :128], norm_w, 1e-6, **kw)}[write]
+    width = 256 if write == "quantize" else 128
+    x = int8.quantize_int8(randn(3, width).to(DEV))
+    weight = int8.Int8Weight(*make(ws[0]))
+    want = int8.linear_int8(x, int8.Int8Weight(*make(ws[1])))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        int8.linear_int8(x, weight)
+        weight.operands()
+        assert weight.stream is not None
+        make(ws[1], out=int8.Int8Rows(weight.values, weight.scales))
+        with torch.cuda.stream(torch.cuda.Stream()):
+            int8.quantize_int8(x.values.float())
+        weight.operands()
+        assert weight.stream is None                 # the next product starts behind what is ahead of it
+        got = int8.linear_int8(x, weight)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_a_product_that_is_refused_leaves_the_weight_to_be_waited_for(int8, monkeypatch):
+    x = int8.quantize_int8(randn(3, 64).to(DEV))
+    weight = int8.Int8Weight.quantize(randn(8, 64).to(DEV))
+    library = int8._lib.load()
+
+    class Refusing:
+        oi_launch_fence = staticmethod(library.oi_launch_fence)
+        oi_linear_int8 = staticmethod(lambda *args: 1)
+
+    with monkeypatch.context() as m:
+        m.setattr(int8._lib, "load", lambda: Refusing)
+        m.setattr(int8._lib, "check", lambda rc, what: (_ for _ in ()).throw(RuntimeError(what)))
+        with pytest.raises(RuntimeError, match="linear_int8"):
+            int8.linear_int8(x, weight)
+    assert weight.stream is None
+    int8.linear_int8(x, weight)
+    assert weight.stream is not None
+
+
 # ------------------------------------------------------------------------------------------------------------ together
 def layer(int8, h, branch, norm_w, gate_up, down, block):
     """A feed-forward layer as a model runs it: norm of the sum, gate and up, activation, down."""
