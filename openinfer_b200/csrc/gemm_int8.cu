@@ -10,6 +10,8 @@
 #include "oi_api.h"
 #include "tcgen05.cuh"
 
+int oi_take_rows_int8_error(int* error);    // rows_int8.cu
+
 namespace {
 
 constexpr int BM = 128;                     // rows of an operand's box
@@ -716,18 +718,6 @@ linear_int8_few_kernel(const __grid_constant__ FewArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-// The shared memory that a kernel may ask for, allowed once for each device that it runs on.
-template <typename Kernel>
-int allow_smem(Kernel kernel, int bytes, bool (&done)[64]) {
-  int dev = 0;
-  OI_CHECK_CUDA(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64 || !done[dev]) {
-    OI_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    if (dev >= 0 && dev < 64) done[dev] = true;
-  }
-  return OI_OK;
-}
-
 constexpr int kMostStages = 12, kSmemOfTwo = 110 * 1024, kSmemOfOne = 208 * 1024;
 
 // Result rows that start and end on 16-byte borders can be copied out by TMA. (Of a row that ends inside 16 bytes the copy writes
@@ -765,7 +755,7 @@ int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const vo
   rc = tc::make_map_2d_i8(&mx, x, M, K, ldx, g.bn);
   OI_REQUIRE(rc == 0, "linear_int8: tensor map for x failed (%d)", rc);
   auto go = [&](auto kernel, int threads, bool (&allowed)[64]) {
-    if (int bad = allow_smem(kernel, 227 * 1024, allowed)) return bad;
+    if (int bad = tc::allow_smem(kernel, 227 * 1024, allowed)) return bad;
     oi_launch_cluster(kernel, dim3(c, z, ceil_div(N, BM)), threads, smem, s, c, mw, mx, out, ldo, scales, g);
     return (int)OI_OK;
   };
@@ -791,7 +781,7 @@ int launch_pair(TOut* out, long long ldo, const void* x, long long ldx, const vo
     OI_REQUIRE(false, "linear_int8: tensor map for the result failed (%d)", rc);
   auto kernel = linear_int8_pair_kernel<TOut>;
   static bool allowed[64];
-  if ((rc = allow_smem(kernel, kPairSmem, allowed))) return rc;
+  if ((rc = tc::allow_smem(kernel, kPairSmem, allowed))) return rc;
   const long long tiles = (long long)ceil_div(M, bn) * ceil_div(N, 256);
   OI_REQUIRE(tiles < (1LL << 30), "linear_int8: %d rows of %d results are too many", M, N);
   const int most = oi_sm_count() / 2, pairs = tiles < most ? (int)tiles : most;
@@ -814,7 +804,7 @@ int launch_few(TOut* out, long long ldo, const void* x, long long ldx, const voi
   f.at_once = wanted <= kFewMostStages;
   const int smem = kFewPart + f.stages * (kFewStage + 16) + 16;
   auto go = [&](auto kernel, bool (&allowed)[64]) {
-    if (int bad = allow_smem(kernel, kFewPart + kFewMostStages * (kFewStage + 16) + 16, allowed)) return bad;
+    if (int bad = tc::allow_smem(kernel, kFewPart + kFewMostStages * (kFewStage + 16) + 16, allowed)) return bad;
     oi_launch(kernel, grid, kFewThreads, smem, s, f);
     return (int)OI_OK;
   };
@@ -912,7 +902,8 @@ OI_API int oi_linear_int8(void* out, int out_dtype, long long ldo, const void* x
 }
 
 // 0 when no bounded wait has run out since the last call; otherwise which role gave up (few rows: 1 copies, 2 products, 3
-// results; many rows: 11 to 13 the same, 14 products waiting for drained results). Synchronises the device; clears the word.
+// results; many rows: 11 to 13 the same, 14 products waiting for drained results; up to 16 rows: 21, 22) or that a row kernel's copies did
+// not come (31). Synchronises the device; clears the words.
 OI_API int oi_linear_int8_status(int* status) {
   int v = 0;
   OI_CHECK_CUDA(cudaMemcpyFromSymbol(&v, g_int8_error, sizeof(int)));
@@ -920,6 +911,7 @@ OI_API int oi_linear_int8_status(int* status) {
     int zero = 0;
     OI_CHECK_CUDA(cudaMemcpyToSymbol(g_int8_error, &zero, sizeof(int)));
   }
-  *status = v;
+  if (int rc = oi_take_rows_int8_error(status)) return rc;
+  if (v != 0) *status = v;
   return OI_OK;
 }

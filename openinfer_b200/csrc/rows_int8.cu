@@ -6,8 +6,11 @@
 //   an infinity or a NaN:   q = 0, scale NaN, so that what is made of the row is NaN and other rows are not touched
 // All arithmetic in float32; y is not rounded to the stored type of its input before it becomes an integer.
 #include "oi_api.h"
+#include "tcgen05.cuh"
 
 namespace {
+
+__device__ int g_rows_int8_error = 0;       // set to a non-zero code when a bounded wait ran out
 
 // |y| as bits: ordered like the numbers, infinities above all finite ones and NaNs above those
 __device__ __forceinline__ unsigned magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
@@ -98,11 +101,16 @@ template <typename T>
 struct PlainRow {
   const T* x;
   long long ldx;
-  static constexpr bool kNorm = false;
+  static constexpr bool kNorm = false, kRing = sizeof(T) == 2;
   struct Raw { Eight<T> x; };
+  struct Kept {};
+  __host__ __device__ __forceinline__ int bytes(int cols) const { return cols * (int)sizeof(T); }
+  __device__ __forceinline__ void copy(unsigned dst, long long r, int cols, unsigned bar) const { tc::bulk_load(dst, x + r * ldx, bytes(cols), bar); }
+  __device__ __forceinline__ void lies_at(const unsigned char* held, int cols) { x = reinterpret_cast<const T*>(held); }
   __device__ __forceinline__ void begin(long long r) { x += r * ldx; }
+  __device__ __forceinline__ void keep(int d, Kept& kept) const {}
   __device__ __forceinline__ void fetch(int d, Raw& raw) const { raw.x.load(x + d); }
-  __device__ __forceinline__ void make(int d, Raw& raw, float (&y)[8], float& squares) const {
+  __device__ __forceinline__ void make(int d, Raw& raw, const Kept& kept, float (&y)[8], float& squares) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = raw.x.get(e);
   }
@@ -121,19 +129,32 @@ struct NormRow {
   long long ldx, ldd;
   int w_dtype;
   float eps, w_offset;
-  static constexpr bool kNorm = true;
-  struct Raw { Eight<T> x, delta; Eight<float> w; };
+  static constexpr bool kNorm = true, kRing = true;
+  struct Raw { Eight<T> x, delta; };
+  struct Kept { Eight<float> w; };
+  __host__ __device__ __forceinline__ int bytes(int cols) const { return cols * (int)sizeof(T) * (delta ? 2 : 1); }
+  __device__ __forceinline__ void copy(unsigned dst, long long r, int cols, unsigned bar) const {
+    const unsigned each = cols * (unsigned)sizeof(T);
+    tc::bulk_load(dst, x + r * ldx, each, bar);
+    if (delta) tc::bulk_load(dst + each, delta + r * ldd, each, bar);
+  }
+  __device__ __forceinline__ void lies_at(unsigned char* held, int cols) {
+    x = reinterpret_cast<T*>(held);
+    if (delta) delta = x + cols;
+  }
   __device__ __forceinline__ void begin(long long r) {
     x += r * ldx;
     if (delta) delta += r * ldd;
   }
+  __device__ __forceinline__ void keep(int d, Kept& kept) const {
+    if (w_dtype == OI_F32) kept.w.load(reinterpret_cast<const float*>(w) + d);
+    else kept.w.v[0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(w) + d);
+  }
   __device__ __forceinline__ void fetch(int d, Raw& raw) const {
     raw.x.load(x + d);
     if (delta) raw.delta.load(delta + d);
-    if (w_dtype == OI_F32) raw.w.load(reinterpret_cast<const float*>(w) + d);
-    else raw.w.v[0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(w) + d);
   }
-  __device__ __forceinline__ void make(int d, Raw& raw, float (&y)[8], float& squares) const {
+  __device__ __forceinline__ void make(int d, Raw& raw, const Kept& kept, float (&y)[8], float& squares) const {
     if (delta) {
       raw.x.add(raw.delta);
       raw.x.store(x + d);
@@ -141,10 +162,10 @@ struct NormRow {
     float wv[8];
     if (w_dtype == OI_F32) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) wv[e] = raw.w.get(e);
+      for (int e = 0; e < 8; ++e) wv[e] = kept.w.get(e);
     } else {
       Eight<bf16> wb;
-      wb.v[0] = raw.w.v[0];
+      wb.v[0] = kept.w.v[0];
 #pragma unroll
       for (int e = 0; e < 8; ++e) wv[e] = wb.get(e);
     }
@@ -179,15 +200,17 @@ struct GateRow {
   const T* x;
   long long ldx;
   int block, shift;     // shift: of a block that is a power of two; -1: all gates, then all ups; -2: any other
-  static constexpr bool kNorm = false;
+  static constexpr bool kNorm = false, kRing = false;
   struct Raw { Eight<T> gate, up; };
+  struct Kept {};
+  __device__ __forceinline__ void keep(int d, Kept& kept) const {}
   __device__ __forceinline__ void begin(long long r) { x += r * ldx; }
   __device__ __forceinline__ const T* at(int d) const { return x + d + (shift >= 0 ? d >> shift << shift : shift == -1 ? 0 : d / block * block); }
   __device__ __forceinline__ void fetch(int d, Raw& raw) const {
     raw.gate.load(at(d));
     raw.up.load(at(d) + block);
   }
-  __device__ __forceinline__ void make(int d, Raw& raw, float (&y)[8], float& squares) const {
+  __device__ __forceinline__ void make(int d, Raw& raw, const Kept& kept, float (&y)[8], float& squares) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = gated<ACT>(raw.gate.get(e), raw.up.get(e));
   }
@@ -204,11 +227,10 @@ struct GateRow {
 // its length alone, so that its result does not depend on how many there are. early: the next kernel may be scheduled while this one
 // runs (not where the rows may be those of a weight: a product fetches its weight before it waits).
 //
-// Bound by memory, or at few rows by the chain load, exchange, store. Measured (bytes read and written, each once): norm with residual of
-// 8192 x 4096 42 us (5.6 TB/s; read once for each thing asked of the row 150), 4096 x 8192 44 (5.3), 65536 x 128 10.8, one row of 4,096 2.2;
-// 2736 x 12288 71 (3.3: with two residual rows and the weight in registers too few rows are on an SM at a time; rows kept in bfloat16
-// and multiplied twice: 68); gate of 4096 x 12288 50 (5.0; two units a thread in 768 threads, four in 384 60), plain rows of
-// 8192 x 4096 20 (5.0), 6144 x 4097 in float32 off every border 33 (3.8).
+// Bound by memory, or at few rows by the chain load, exchange, store; beside memory by instructions (issue slots 64 to 69 % busy at
+// 16384 x 4096). Measured (bytes read and written, each once): norm with residual of 8192 x 4096 39.6 us (5.9 TB/s; read once for each thing
+// asked of the row 150), 4096 x 8192 42 (5.6), 65536 x 128 9.9, one row of 4,096 2.1; gate of 4096 x 12288 47 (5.3; four units a thread in 384
+// threads 60, two in 768 so), plain rows of 8192 x 4096 19.4 (5.2), 6144 x 4097 in float32 off every border 33 (3.8).
 template <typename Row, bool kVec, int UNITS, int LANES>
 __global__ void __launch_bounds__(LANES || UNITS == 1 ? 256 : UNITS == 2 ? 768 : 512)
 rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows, int cols, int early) {
@@ -236,19 +258,20 @@ rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows
     return row.make_one(d, raw, squares);
   };
   if constexpr (kVec) {
-    constexpr int kAhead = UNITS < 2 ? UNITS : 2;      // units asked for before the first is used
+    constexpr int kAhead = UNITS < 4 ? UNITS : 2;      // units asked for before the first is used
 #pragma unroll
     for (int u0 = 0; u0 < UNITS; u0 += kAhead) {
       typename Row::Raw raw[kAhead];
+      typename Row::Kept kept[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const int d = (me + (u0 + u) * step) * 8;
-        if (d + 8 <= cols) row.fetch(d, raw[u]);
+        if (d + 8 <= cols) row.fetch(d, raw[u]), row.keep(d, kept[u]);
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const int d = (me + (u0 + u) * step) * 8;
-        if (d + 8 <= cols) row.make(d, raw[u], y[u0 + u], squares);
+        if (d + 8 <= cols) row.make(d, raw[u], kept[u], y[u0 + u], squares);
         else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[u0 + u][e] = d + e < cols ? one(d + e) : 0.f;
@@ -331,6 +354,104 @@ rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows
   }
 }
 
+// Many wide rows. What bounds the kernel above there is that registers hold what is on the way as well as what is at hand: of a norm's row of
+// 12,288 with its residual one block fits an SM, and nothing is on the way while it exchanges and stores. Here rows come into shared memory by
+// bulk copies, two or more ahead, one or two blocks an SM take them in turn, and a norm's weights stay in registers. A row is shared
+// out as above, so its bits are the same. Measured (us, above -> this; bfloat16 norm with residual, without, plain rows): 4096 x 8704 58.0 -> 49.3,
+// 47.3 -> 44.1, 28.4 -> 23.3; 4096 x 12288 97.2 -> 57.0 (6.2 TB/s), 83.6 -> 46.1, 34.7 -> 28.7; 1200 x 12288, from L2, 21.9 -> 18.1, 19.3 -> 16.3,
+// 9.0 -> 9.4; 4096 x 16384 110 -> 87, 93 -> 54, 46.6 -> 35.6; 300 x 12288 7.5 -> 8.1; gates and rows of up to 8,192 are faster above, and so are
+// float32's plain rows (4096 x 12288 38 -> 43). Bound by memory; with a ring of two rows (16384 with residual) by the wait for the next.
+constexpr int kRingMost = 8, kRingUnits = 4, kRingBytes = 208 * 1024;
+
+template <typename Row>
+__global__ void __launch_bounds__(512)
+ring_rows_int8_kernel(const Row row, signed char* q, long long ldq, float* scales, int rows, int cols, int stages, int early) {
+  if (early) pdl_trigger();
+  extern __shared__ __align__(128) unsigned char ring[];
+  __shared__ __align__(8) unsigned long long bars[kRingMost];
+  __shared__ float part_squares[2][32];
+  __shared__ unsigned part_most[2][32];
+  __shared__ int aborted;
+  volatile int* abort_flag = &aborted;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, me = threadIdx.x, step = blockDim.x;
+  const unsigned ring_base = tc::smem_u32(ring), bar_base = tc::smem_u32(bars), stage_bytes = row.bytes(cols);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) tc::mbar_init(bar_base + 8u * s, 1);
+    aborted = 0;
+    tc::mbar_fence_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  const int count = (rows - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  auto ask = [&](int i, int s) {                     // thread 0
+    tc::mbar_expect_tx(bar_base + 8u * s, stage_bytes);
+    row.copy(ring_base + s * stage_bytes, blockIdx.x + (long long)i * gridDim.x, cols, bar_base + 8u * s);
+  };
+  if (threadIdx.x == 0)
+    for (int i = 0; i < stages && i < count; ++i) ask(i, i);
+  typename Row::Kept kept[kRingUnits];
+#pragma unroll
+  for (int u = 0; u < kRingUnits; ++u)
+    if ((me + u * step) * 8 < cols) row.keep((me + u * step) * 8, kept[u]);
+  int s = 0;
+  unsigned parity = 0;
+  bool ok = true;
+  for (int i = 0; i < count; ++i) {
+    const long long r = blockIdx.x + (long long)i * gridDim.x;
+    Row mine = row, held = row;
+    mine.begin(r);
+    held.lies_at(ring + s * stage_bytes, cols);
+    if (ok) ok = tc::mbar_wait(bar_base + 8u * s, parity, abort_flag, &g_rows_int8_error, 31);
+    float y[kRingUnits][8], squares = 0.f;
+    unsigned most = 0u;
+#pragma unroll
+    for (int u = 0; u < kRingUnits; ++u) {
+      const int d = (me + u * step) * 8;
+      typename Row::Raw raw;
+      if (ok && d < cols) {
+        held.fetch(d, raw);
+        mine.make(d, raw, kept[u], y[u], squares);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[u][e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kRingUnits * 8; k += 2) most = __vimax3_u32(most, magnitude(y[k / 8][k % 8]), magnitude(y[k / 8][k % 8 + 1]));
+    if (!ok) most = 0x7fffffffu;                     // what did not come is no number
+    most = __reduce_max_sync(0xffffffffu, most);
+    if constexpr (Row::kNorm) squares = warp_sum(squares);
+    if (lane == 0) {
+      part_most[i & 1][warp] = most;
+      part_squares[i & 1][warp] = squares;
+    }
+    __syncthreads();                                 // the stage is read; the other part may be written again
+    if (threadIdx.x == 0 && i + stages < count && ok) ask(i + stages, s);
+    most = __reduce_max_sync(0xffffffffu, lane < warps ? part_most[i & 1][lane] : 0u);
+    if constexpr (Row::kNorm) squares = warp_sum(lane < warps ? part_squares[i & 1][lane] : 0.f);
+    float common = 1.f;
+    if constexpr (Row::kNorm) common = rsqrtf(squares / (float)cols + row.eps);
+    const RowScale sc(most, common);
+    if (me == 0) scales[r] = sc.scale;
+    if (sc.tiny) {
+#pragma unroll
+      for (int k = 0; k < kRingUnits * 8; ++k) y[k / 8][k % 8] *= 0x1p80f;
+    }
+    signed char* to = q + r * ldq;
+#pragma unroll
+    for (int u = 0; u < kRingUnits; ++u) {
+      const int d = (me + u * step) * 8;
+      const uint2 o = {sc.four(y[u][0], y[u][1], y[u][2], y[u][3]), sc.four(y[u][4], y[u][5], y[u][6], y[u][7])};
+      if (d < cols) *reinterpret_cast<uint2*>(to + d) = o;
+    }
+    if (++s == stages) s = 0, parity ^= 1;
+  }
+  __syncthreads();
+  if (*abort_flag && threadIdx.x == 0)
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);      // copies still landing in this block's shared memory
+  __syncthreads();
+}
+
 // Rows longer than 512 threads hold in registers: one block a row, read once for each thing that is asked of all of it.
 template <typename Row>
 __global__ void __launch_bounds__(1024) long_rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int cols, int early) {
@@ -374,10 +495,19 @@ void launch_rows(const Row& row, signed char* q, long long ldq, float* scales, i
     return;
   }
   // Rows of up to 1,024 in a block are back sooner (one row, us: norm 3.7 in a warp, 1.8 so), in a warp there are more of them on the way
-  // (8,192 rows: 5.1, and 6.2 in blocks). A norm's sum has one order whatever the number of rows; without one, either will do.
+  // (8,192 rows: 5.1, and 6.2 in blocks; 8192 x 640 5.7 -> 4.2, its gates 8.1 -> 7.3, float32 gates 7.7 -> 8.2 and so left in blocks, 2048 x 640
+  // 3.1 -> 3.5). A norm's sum has one order whatever the number of rows; without one, either will do.
   if constexpr (!Row::kNorm) {
-    if (units > 96 && units <= 128 && rows >= 2048) {
-      oi_launch(rows_int8_kernel<Row, kVec, 4, 32>, ceil_div(rows, 8), 256, kVec ? 0 : 8 * 1024, s, row, q, ldq, scales, rows, cols, early);
+    constexpr bool kThree = !kVec || sizeof(typename Row::Raw) <= 32;
+    if (units <= 128 && (units > 96 ? rows >= 2048 : kThree && rows >= 2560)) {
+      auto go = [&](auto kernel) { oi_launch(kernel, ceil_div(rows, 8), 256, kVec ? 0 : 8 * 1024, s, row, q, ldq, scales, rows, cols, early); };
+      if constexpr (kThree) {
+        if (units <= 96) {
+          go(rows_int8_kernel<Row, kVec, 3, 32>);
+          return;
+        }
+      }
+      go(rows_int8_kernel<Row, kVec, 4, 32>);
       return;
     }
   }
@@ -391,10 +521,32 @@ void launch_rows(const Row& row, signed char* q, long long ldq, float* scales, i
   else oi_launch(long_rows_int8_kernel<Row>, rows, 1024, 0, s, row, q, ldq, scales, cols, early);
 }
 
+// Where rows are more than what L2 holds for the kernel ahead and this one or, of a norm, where the kernel above has one block on an SM
+// (320 threads or fewer of bfloat16 are two) and there are three for each.
+template <typename Row>
+bool ring_takes(const Row& row, int esize, int rows, int cols) {
+  if (cols % 8 != 0 || cols <= 8192 || cols > 8 * kRingUnits * 512 || 2 * row.bytes(cols) > kRingBytes) return false;
+  return (long long)rows * row.bytes(cols) >= 64 << 20 || (Row::kNorm && rows >= 3 * oi_sm_count() && (esize == 4 || cols > 10240));
+}
+template <typename Row>
+int launch_ring(const Row& row, signed char* q, long long ldq, float* scales, int rows, int cols, int early, cudaStream_t s) {
+  const int bytes = row.bytes(cols), blocks = 4 * bytes <= kRingBytes ? 2 : 1, fit = kRingBytes / blocks / bytes;
+  const int stages = fit < kRingMost ? fit : kRingMost, most = oi_sm_count() * blocks;
+  auto kernel = ring_rows_int8_kernel<Row>;
+  static bool allowed[64];
+  if (int bad = tc::allow_smem(kernel, kRingBytes, allowed)) return bad;
+  oi_launch(kernel, rows < most ? rows : most, ceil_div(cols, 8 * kRingUnits * 32) * 32, stages * bytes, s, row, q, ldq, scales, rows, cols, stages, early);
+  OI_CHECK_LAUNCH();
+  return OI_OK;
+}
+
 // vec: everything that a row is read from starts on 16-byte borders, and the next row's too, whether there is one or not: one row
 // of a matrix is shared out among the threads as it is among others
 template <typename Row>
 int launch(const Row& row, bool vec, void* q, long long ldq, float* scales, int rows, int cols, int early, cudaStream_t s) {
+  if constexpr (Row::kRing) {
+    if (vec && ring_takes(row, (int)sizeof(*row.x), rows, cols)) return launch_ring(row, (signed char*)q, ldq, scales, rows, cols, early, s);
+  }
   if (vec) launch_rows<Row, true>(row, (signed char*)q, ldq, scales, rows, cols, early, s);
   else launch_rows<Row, false>(row, (signed char*)q, ldq, scales, rows, cols, early, s);
   OI_CHECK_LAUNCH();
@@ -541,4 +693,13 @@ OI_API int oi_dequantize_int8(void* out, int dtype, long long ldo, const void* q
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == OI_F32) return launch_dequantize((float*)out, ldo, (const signed char*)q, ldq, scales, rows, cols, s);
   return launch_dequantize((bf16*)out, ldo, (const signed char*)q, ldq, scales, rows, cols, s);
+}
+
+int oi_take_rows_int8_error(int* error) {
+  OI_CHECK_CUDA(cudaMemcpyFromSymbol(error, g_rows_int8_error, sizeof(int)));
+  if (*error != 0) {
+    const int zero = 0;
+    OI_CHECK_CUDA(cudaMemcpyToSymbol(g_rows_int8_error, &zero, sizeof(int)));
+  }
+  return OI_OK;
 }

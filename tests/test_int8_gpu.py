@@ -172,6 +172,60 @@ def test_a_row_does_not_depend_on_the_rows_around_it(int8, width):
         assert torch.equal(one.values[0], gates.values[r]) and torch.equal(one.scales[0], gates.scales[r])
 
 
+@pytest.mark.parametrize("op,dtype,residual,rows,width,pad", [
+    ("norm", torch.bfloat16, True, 600, 12288, 0), ("norm", torch.bfloat16, True, 450, 16384, 8), ("norm", torch.bfloat16, False, 450, 10248, 24),
+    ("norm", torch.float32, True, 600, 8200, 4), ("norm", torch.float32, False, 450, 16376, 0), ("norm", torch.bfloat16, True, 4000, 8704, 0),
+    ("rows", torch.bfloat16, False, 4097, 8200, 0), ("rows", torch.bfloat16, False, 2100, 16384, 8)])
+def test_many_wide_rows(int8, op, dtype, residual, rows, width, pad):
+    """Wide rows, many at a time and one at a time: the same bits; some are zero, tiny or not finite."""
+    w = (1 + 0.1 * randn(width, seed=5)).to(DEV)
+    x, d = (torch.randn(rows, width, generator=torch.Generator(device=DEV).manual_seed(s), device=DEV).to(dtype) for s in (1, 2))
+    wide = torch.full((rows, width + pad), float("nan"), dtype=dtype, device=DEV)
+    x[5], d[5], x[151, 8], x[300, width - 1] = 0, 0, float("inf"), float("nan")
+    x[7] *= 1e-36
+    d[7] = 0
+    wide[:, :width] = x
+    room = torch.full((rows + 1, width + 24 - width % 8 + 64), 99, dtype=torch.int8, device=DEV)
+    room = room.as_strided((rows + 1, width), (room.shape[1] // 16 * 16, 1))
+    scales = torch.full((rows + 1,), 7.0, device=DEV)
+    out = int8.Int8Rows(room[:rows], scales[:rows])
+
+    def call(at, delta, **kw):
+        return int8.quantize_int8(at, **kw) if op == "rows" else int8.rmsnorm_int8(at, w, 1e-6, delta=delta, **kw)
+    whole = call(wide[:, :width], d if residual else None, out=out)
+    assert torch.equal(wide[:, :width].nan_to_num(), ((x.float() + d.float()).to(dtype) if residual else x).nan_to_num())
+    assert bool((room[rows:] == 99).all()) and float(scales[rows]) == 7.0 and bool(torch.isnan(wide[:, width:]).all())
+    for r in [0, 5, 7, 147, 148, 151, 295, 296, 300, 301, rows - 2, rows - 1]:
+        one = call(x[r:r + 1].clone(), d[r:r + 1] if residual else None)
+        assert torch.equal(one.values[0], whole.values[r]), r
+        assert torch.equal(one.scales[0].nan_to_num(), whole.scales[r].nan_to_num()), r
+    s = whole.scales
+    assert float(s[5]) == 0 and bool(torch.isnan(s[[151, 300]]).all()) and not bool(whole.values[[5, 151, 300]].any())
+    assert int(torch.isfinite(s).sum()) == rows - 2
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,width", [(2559, 640), (2560, 640), (2560, 513), (2561, 767), (2048, 769), (4099, 1024)])
+def test_many_rows_of_half_a_block(int8, dtype, rows, width):
+    """Rows of 513 to 1,024 numbers, many at a time and one at a time: the same bits."""
+    x = torch.randn(rows, 2 * width, generator=torch.Generator(device=DEV).manual_seed(width), device=DEV).to(dtype)
+    held, gates = int8.quantize_int8(x[:, :width]), int8.silu_mul_int8(x)
+    for r in (0, 7, 8, rows // 2, rows - 1):
+        for many, one in ((held, int8.quantize_int8(x[r:r + 1, :width])), (gates, int8.silu_mul_int8(x[r:r + 1]))):
+            assert torch.equal(one.values[0], many.values[r]) and torch.equal(one.scales[0], many.scales[r])
+
+
+def test_many_wide_rows_take_themselves_as_the_residual_and_one_row_for_all(int8):
+    x, w = torch.randn(500, 12288, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).bfloat16(), torch.ones(12288, device=DEV)
+    a, b, one = x.clone(), x.clone(), x[3:4].clone()
+    held = int8.rmsnorm_int8(a, w, 1e-6, delta=a)
+    assert torch.equal(a, x + x)
+    alone = int8.rmsnorm_int8((x + x)[499:].clone(), w, 1e-6)
+    assert torch.equal(alone.values[0], held.values[499]) and torch.equal(alone.scales[0], held.scales[499])
+    int8.rmsnorm_int8(b, w, 1e-6, delta=one.expand(500, 12288))
+    assert torch.equal(b, (x.float() + one.float()).bfloat16())
+
+
 # ------------------------------------------------------------------------------------------------------------ gates
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
