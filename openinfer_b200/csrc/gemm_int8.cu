@@ -46,19 +46,20 @@ struct Scales {
 // Few rows. The product is formed transposed: 128 rows of w are the M side of tcgen05.mma, up to 256 rows of x (a multiple of
 // 16, `bn`) its N side, so a weight byte goes HBM -> TMA -> shared memory -> tensor core, and the accumulator [128 rows of
 // w x bn] lies in tensor memory. Grid (c, tiles of x, tiles of w; those that share a tile of w run together): a cluster of c CTAs (a power of two) shares one tile, CTA r
-// streaming k blocks [r * kb_per_rank, ...) of it, and adds up: row i of the accumulator (a row of w) belongs to CTA i / (128 / c),
-// into whose shared memory every CTA deposits its partial sums of it.
+// streaming k blocks [r * kb_per_rank, ...) of it. Columns of the accumulator (rows of x) belong to the CTAs by fours in turn: each
+// deposits what it has of the others' columns in their shared memory, 16 bytes a channel, and adds to its own, which stay in tensor
+// memory, what the others left there. (All of a channel's columns to one CTA, its own part through shared memory too, us: 264 x 4096 x 12288
+// 19.2 for 18.3, 400 x 2048 x 8192 14.5 for 12.5, 256 x 512 x 16384 10.2 for 9.2, 24 x 1024 x 1024 3.7 for 3.55.)
 //   warp 0     one thread issues the copies; the first ring-full of WEIGHT boxes is requested before the wait for the kernel
 //              ahead (programmatic dependent launch), which may still be writing x
 //   warp 1     allocates tensor memory (behind that wait: a kernel ahead that needs all of it may not have taken its own
 //              yet), one thread issues four products (K = 32) a stage
-//   the others (four to sixteen) read the accumulator (one row of w a thread) and deposit, or with c = 1 scale and store; then
-//              all warps add up, scale and store.
+//   the others (four to sixteen) read the accumulator (one row of w a thread), deposit and add up, scale and store
 // What the results cost shows in the instructions per column: with a column at a time, a branch and a cluster address each, and
 // six warps, 128 columns took 8,000 cycles to deposit and 8,700 to store (N 1024, K 1024, c 1); stored two channels a lane, by lanes that
 // trade halves, 4.6 us instead of 4.3 (500 x 4095 x 512).
 // Measured (us; what its bytes at the copy rate and its operations at twice the bfloat16 rate take): 32 x 24576 x 4096 19.6 (15.6),
-// 64 x 6144 x 4096 9.8 (4.0), 512 x 4096 x 4096 11.2 (5.2), 264 x 4096 x 12288 18.8 (8.5), a head of 151936 x 4096 with 64 rows 102 (98).
+// 64 x 6144 x 4096 8.8 (4.0), 512 x 4096 x 4096 10.5 (5.2), 264 x 4096 x 12288 18.4 (8.5), a head of 151936 x 4096 with 64 rows 102 (98).
 // Bound by what one SM takes in (some 110 GB/s, 32 KB a stage of 128 rows) and, short sums, by launch, x, results.
 constexpr int kFewColumns = 32, kMoreColumns = 64;      // up to so many rows of x a tile four warps read results, or eight, else sixteen
 
@@ -74,7 +75,6 @@ __global__ void __launch_bounds__(64 + 32 * kReaders)
 linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, TOut* out, long long ldo,
                         const Scales scales, const Shape g) {
   pdl_trigger();
-  constexpr int kThreads = 64 + 32 * kReaders;
   extern __shared__ __align__(1024) unsigned char smem[];
   const unsigned smem_base = tc::smem_u32(smem);
   const bool misaligned = (smem_base & 1023u) != 0;   // never seen; refuse rather than compute garbage
@@ -128,8 +128,7 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
   // what the sums are multiplied by is fetched under the copies: a channel's scale in its thread, later every row's in shared memory
   const int cols = min(g.bn, g.M - m0);  // rows of x in this tile
   const int quarter = warp & 3;          // a warp may only touch lanes [32 * (warp % 4), +32) of tensor memory
-  const int rows_mine = BM / csize;      // channels that this CTA adds up
-  const int n = n0 + (csize > 1 ? rank * rows_mine + (int)threadIdx.x % rows_mine : quarter * 32 + lane);
+  const int row = quarter * 32 + lane, n = n0 + row;
   const float sw = n < g.N ? scales.sw[n] : 0.f;
   tc::fence_before();
   __syncthreads();
@@ -193,28 +192,33 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
       tc::cluster_wait();
     }
   }
-  const int ld = g.bn + 4;               // words of a row of deposits: eight lanes' 16 bytes then lie in different banks
-  if (warp >= 2) {
-    const unsigned tmem_row = tmem_base + ((unsigned)(quarter * 32) << 16);
-    const int row = quarter * 32 + lane;
-    unsigned dst = 0;
-    if (csize > 1)
-      dst = tc::map_to_rank(smem_base + g.recv_offset, row / rows_mine) + (unsigned)((rank * rows_mine + row % rows_mine) * ld) * 4;
-#pragma unroll 1
-    for (int c0 = 16 * ((warp - 2) >> 2); c0 < cols; c0 += 4 * kReaders) {
-      unsigned v[16];
-      if (nkb > 0 && ok) {
-        tc::tmem_ld16(tmem_row + (unsigned)c0, v);
-        tc::tmem_ld_wait();
-      } else {
+  const unsigned tmem_row = tmem_base + ((unsigned)(quarter * 32) << 16);
+  auto read = [&](int c0, unsigned (&v)[16]) {                // sixteen columns of this thread's channel
+    if (nkb > 0 && ok) {
+      tc::tmem_ld16(tmem_row + (unsigned)c0, v);
+      tc::tmem_ld_wait();
+    } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = 0u;
-      }
+      for (int e = 0; e < 16; ++e) v[e] = 0u;
+    }
+  };
+  // Four columns are a piece; piece p belongs to CTA p % c, which gets 16 bytes a channel from each of the others.
+  const int first = 16 * ((warp - 2) >> 2), last_rank = csize - 1, shift = __popc(last_rank);
+  const unsigned recv = smem_base + g.recv_offset + (unsigned)row * 16;
+  if (warp >= 2) {
+#pragma unroll 1
+    for (int c0 = first; c0 < cols; c0 += 4 * kReaders) {
+      unsigned v[16];
+      read(c0, v);
       if (csize > 1) {
 #pragma unroll
-        for (int e = 0; e < 16; e += 4)
-          if (c0 + e < cols) asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};\n"
-                       ::"r"(dst + (unsigned)(c0 + e) * 4), "r"(v[e]), "r"(v[e + 1]), "r"(v[e + 2]), "r"(v[e + 3]) : "memory");
+        for (int e = 0; e < 16; e += 4) {
+          const int piece = (c0 + e) >> 2, owner = piece & last_rank;
+          if (c0 + e < cols && owner != rank)
+            asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};\n"
+                         ::"r"(tc::map_to_rank(recv, owner) + (unsigned)((piece >> shift) * last_rank + rank - (rank > owner)) * (BM * 16)),
+                           "r"(v[e]), "r"(v[e + 1]), "r"(v[e + 2]), "r"(v[e + 3]) : "memory");
+        }
       } else {
         float y[16];
 #pragma unroll
@@ -232,31 +236,39 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
       }
     }
   }
-  tc::fence_before();
   if (csize > 1) {
     __syncwarp();
     tc::cluster_arrive();                // this CTA's deposits are made ...
     tc::cluster_wait();                  // ... and so are everybody's; nothing remote is touched after this
-    // a channel and four rows of x a thread (rows_mine divides the threads: its channel stays)
-    const int local = (int)threadIdx.x % rows_mine, step = kThreads / rows_mine;
-    const unsigned char* mine = smem + g.recv_offset + (size_t)local * ld * 4;
-    if (n < g.N) {
-#pragma unroll 2
-      for (int c = (int)threadIdx.x / rows_mine * 4; c < cols; c += step * 4) {
-        int4 sum = make_int4(0, 0, 0, 0);
-        for (int q = 0; q < csize; ++q) {
-          const int4 part = *reinterpret_cast<const int4*>(mine + ((size_t)q * rows_mine * ld + c) * 4);
-          sum.x += part.x, sum.y += part.y, sum.z += part.z, sum.w += part.w;
+    if (warp >= 2) {
+      const unsigned char* mine = smem + g.recv_offset + (size_t)row * 16;
+#pragma unroll 1
+      for (int c0 = first; c0 < cols; c0 += 4 * kReaders) {
+        if (csize == 8 && ((c0 >> 4) & 1) != rank >> 2) continue;       // none of these four pieces
+        unsigned v[16];
+        read(c0, v);
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const int piece = (c0 + e) >> 2;
+          if ((piece & last_rank) != rank || c0 + e >= cols) continue;
+          int4 sum = make_int4((int)v[e], (int)v[e + 1], (int)v[e + 2], (int)v[e + 3]);
+          for (int q = 0; q < last_rank; ++q) {
+            const int4 part = *reinterpret_cast<const int4*>(mine + (size_t)((piece >> shift) * last_rank + q) * (BM * 16));
+            sum.x += part.x, sum.y += part.y, sum.z += part.z, sum.w += part.w;
+          }
+          const float4 sx = *reinterpret_cast<const float4*>(sx_s + c0 + e);
+          TOut* at = out + (size_t)(m0 + c0 + e) * ldo + n;
+          if (n < g.N) {
+            *at = from_f32<TOut>(finish(sum.x, sx.x, sw, b, biased));
+            if (c0 + e + 1 < cols) at[ldo] = from_f32<TOut>(finish(sum.y, sx.y, sw, b, biased));
+            if (c0 + e + 2 < cols) at[2 * ldo] = from_f32<TOut>(finish(sum.z, sx.z, sw, b, biased));
+            if (c0 + e + 3 < cols) at[3 * ldo] = from_f32<TOut>(finish(sum.w, sx.w, sw, b, biased));
+          }
         }
-        const float4 sx = *reinterpret_cast<const float4*>(sx_s + c);
-        TOut* at = out + (size_t)(m0 + c) * ldo + n;
-        *at = from_f32<TOut>(finish(sum.x, sx.x, sw, b, biased));
-        if (c + 1 < cols) at[ldo] = from_f32<TOut>(finish(sum.y, sx.y, sw, b, biased));
-        if (c + 2 < cols) at[2 * ldo] = from_f32<TOut>(finish(sum.z, sx.z, sw, b, biased));
-        if (c + 3 < cols) at[3 * ldo] = from_f32<TOut>(finish(sum.w, sx.w, sw, b, biased));
       }
     }
   }
+  tc::fence_before();
   if (*abort_flag && threadIdx.x == 0) {
     // copies that were issued may still be landing in this CTA's shared memory: give them time
     for (int i = 0; i < 1000; ++i) __nanosleep(1000);
@@ -736,7 +748,7 @@ int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const vo
   g.num_kb = ceil_div(K, BK);
   g.kb_per_rank = ceil_div(g.num_kb, c);
   g.tmem_cols = g.bn <= 32 ? 32 : g.bn <= 64 ? 64 : g.bn <= 128 ? 128 : 256;
-  const int stage = kBoxBytes + g.bn * BK, recv = c > 1 ? BM * (g.bn + 4) * 4 : 0;
+  const int stage = kBoxBytes + g.bn * BK, recv = ceil_div(g.bn / 4, c) * (c - 1) * BM * 16;
   // two CTAs on an SM, where there are more than SMs: one streams while the other ends, the next kernel's included
   const int budget = (long long)c * z * ceil_div(N, BM) <= (c == 8 ? 96 : oi_sm_count()) || g.bn > 128 ? kSmemOfOne : kSmemOfTwo;
   // deposits beside the ring, or over it when it is drained (a cluster's barrier more) where a ring beside them would be short (264 rows, N
@@ -826,7 +838,7 @@ int launch_few(TOut* out, long long ldo, const void* x, long long ldx, const voi
 // median 1.00.
 // Few rows: a stage of 128 bytes of K is 16 KB of w and `cols` rows of x at what one SM takes in, for as many CTAs as an SM has to
 // run; the weight's bytes come from memory and all copies through L2 (16 TB/s). Every round of CTAs costs 2.3 around its first copy
-// and its results, 0.006 to 0.008 a column of the accumulator, or added up over a cluster 0.5 and 0.038 a row of x. Clusters of four
+// and its results, 0.006 to 0.008 a column of the accumulator, or added up over a cluster 0.4 and 0.03 to 0.06 a column sent. Clusters of four
 // and eight do not fill the SMs (35 of four: two rounds).
 // Many rows: 4.5, and for each round of tiles its stages (16 KB of w and half the tile's rows of x for each CTA) or, where sums are
 // short, its results, which take longer where result rows do not start and end on 16-byte borders.
@@ -837,7 +849,7 @@ float few_rows_us(int M, int N, int num_kb, int c, int z, int sms) {
   const float rounds = (float)((ctas + at_once * on_an_sm - 1) / (at_once * on_an_sm));
   const float products = (float)((ctas + at_once - 1) / at_once) * kb * (0.185f + 0.0005f * cols);
   const float memory = (float)N * num_kb * BK / 6.4e6f, l2 = (float)ctas * kb * BK * (BM + cols) / 16e6f;
-  const float results = c > 1 ? 0.5f + 0.038f * cols : (bn > 128 ? 0.008f : 0.006f) * bn;
+  const float sent = cols * (c - 1.f) / c, results = c > 1 ? 0.4f + (sent < 32.f ? 0.06f * sent : 1.f + 0.03f * sent) : (bn > 128 ? 0.008f : 0.006f) * bn;
   const float around = 2.3f + results * on_an_sm, copies = memory > l2 ? memory : l2, work = products + (rounds - 1.f) * around;
   return around + (work > copies ? work : copies);
 }

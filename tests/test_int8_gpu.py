@@ -288,6 +288,10 @@ TILES = [(370, 2972, 7657), (574, 7354, 3863), (309, 8746, 3887), (629, 8798, 26
           (2455, 147, 3658), (1765, 513, 9245), (17, 34, 1061), (3053, 32, 3017), (105, 3407, 6918), (71, 2413, 5902), (129, 2256, 14702),
           (1, 32, 401), (33, 2092, 2422), (3112, 32, 5562), (2099, 32, 2845), (269, 1898, 7347), (21, 32, 786), (389, 36, 1449), (105, 1506, 10930),
           (65, 1113, 9920), (130, 1413, 14655), (1, 33, 917), (33, 830, 4806), (1164, 34, 14005), (812, 33, 5825), (22, 32, 977), (409, 36, 2770)]
+# The same for the sums that are cut, with columns that leave some of the CTAs without a part
+SLICES = [(1, 5145, 38), (73, 5536, 3470), (147, 6767, 4895), (142, 4907, 6373), (1, 4849, 390), (2332, 148, 2878), (2949, 287, 5675),
+          (4067, 158, 5709), (668, 46, 1779), (120, 2166, 9557), (140, 3095, 6274), (1, 2626, 4885), (33, 2561, 3541), (3653, 33, 5702),
+          (1370, 321, 6947), (123, 1374, 14983), (1, 32, 8836), (34, 814, 8161), (1454, 34, 12852), (1610, 72, 16138)]
 # Up to 16 rows: every length of the registers that hold x, one and two groups of eight rows, rows of w that the ring holds and that it does not
 FEW = [(8, 32, 8836), (7, 126, 9360), (1, 32, 33), (5, 46, 32), (8, 34, 2234), (3, 39, 2064), (2, 33, 4292), (8, 47, 5408), (10, 42, 34), (13, 34, 32),
        (16, 37, 2310), (14, 32, 2736), (9, 38, 4452), (16, 32, 5328), (8, 3650, 9116), (2, 4034, 8944), (1, 14218, 1377), (5, 14860, 1312),
@@ -310,7 +314,7 @@ def test_product(int8, rows, channels, width):
             assert torch.equal(out[:, :channels].cpu(), product_exactly(x, sx, w, sw, bias, dtype)) and bool((out[:, channels:] == -7.0).all())
 
 
-@pytest.mark.parametrize("rows,channels,width", TILES + FEW)
+@pytest.mark.parametrize("rows,channels,width", TILES + SLICES + FEW)
 def test_product_by_every_kind_of_tile(int8, rows, channels, width):
     (x, sx), (w, sw) = integers(rows, width, 1), integers(channels, width, 2)
     bias = randn(channels, seed=3)
