@@ -834,11 +834,11 @@ int launch_few(TOut* out, long long ldo, const void* x, long long ldx, const voi
 }
 
 // What a product takes in us, from what was measured (B200; N 32 to 152,000, K 128 to 16,000, 1 to 8,192 rows), to choose a kernel, its
-// tiles of x and the slices of K. Over 150 sizes, most of them drawn, the choice took at most 1.24 times the fastest choice's time, in the
+// tiles of x and the slices of K. Over 170 sizes, most of them drawn, the choice took at most 1.16 times the fastest choice's time, in the
 // median 1.00.
 // Few rows: a stage of 128 bytes of K is 16 KB of w and `cols` rows of x at what one SM takes in, for as many CTAs as an SM has to
-// run; the weight's bytes come from memory and all copies through L2 (16 TB/s). Every round of CTAs costs 2.3 around its first copy
-// and its results, 0.006 to 0.008 a column of the accumulator, or added up over a cluster 0.4 and 0.03 to 0.06 a column sent. Clusters of four
+// run; the weight's bytes come from memory and all copies through L2 (21 TB/s, less beside memory's). Every round of CTAs costs 2.2 around
+// its first copy and its results, 0.004 to 0.009 a column of the accumulator, or added up over a cluster 1.4 and 0.025 to 0.034 a column sent. Clusters of four
 // and eight do not fill the SMs (35 of four: two rounds).
 // Many rows: 4.5, and for each round of tiles its stages (16 KB of w and half the tile's rows of x for each CTA) or, where sums are
 // short, its results, which take longer where result rows do not start and end on 16-byte borders.
@@ -847,10 +847,10 @@ float few_rows_us(int M, int N, int num_kb, int c, int z, int sms) {
   const long long ctas = (long long)ceil_div(N, BM) * z * c;
   const int on_an_sm = ctas <= at_once || bn > 128 ? 1 : 2;
   const float rounds = (float)((ctas + at_once * on_an_sm - 1) / (at_once * on_an_sm));
-  const float products = (float)((ctas + at_once - 1) / at_once) * kb * (0.185f + 0.0005f * cols);
-  const float memory = (float)N * num_kb * BK / 6.4e6f, l2 = (float)ctas * kb * BK * (BM + cols) / 16e6f;
-  const float sent = cols * (c - 1.f) / c, results = c > 1 ? 0.4f + (sent < 32.f ? 0.06f * sent : 1.f + 0.03f * sent) : (bn > 128 ? 0.008f : 0.006f) * bn;
-  const float around = 2.3f + results * on_an_sm, copies = memory > l2 ? memory : l2, work = products + (rounds - 1.f) * around;
+  const float products = (float)((ctas + at_once - 1) / at_once) * kb * (0.171f + 0.00064f * cols);
+  const float memory = (float)N * num_kb * BK / 6.4e6f, l2 = (float)ctas * kb * BK * (BM + cols) / 20.8e6f + 0.6f * memory;
+  const float sent = cols * (c - 1.f) / c, results = c > 1 ? 0.38f + (sent < 32.f ? 0.025f * sent : 0.8f + 0.034f * (sent - 32.f)) : (bn > 128 ? 0.0086f : 0.004f) * bn;
+  const float around = (c > 1 ? 3.26f : 2.23f) + results * on_an_sm, copies = memory > l2 ? memory : l2, work = products + (rounds - 1.f) * around;
   return around + (work > copies ? work : copies);
 }
 // Up to 16 rows on mma.sync: 16 rows of w after another, a stage of 2,048 bytes of each at the copy rate or the barrier behind them; x

@@ -291,7 +291,9 @@ TILES = [(370, 2972, 7657), (574, 7354, 3863), (309, 8746, 3887), (629, 8798, 26
 # The same for the sums that are cut, with columns that leave some of the CTAs without a part
 SLICES = [(1, 5145, 38), (73, 5536, 3470), (147, 6767, 4895), (142, 4907, 6373), (1, 4849, 390), (2332, 148, 2878), (2949, 287, 5675),
           (4067, 158, 5709), (668, 46, 1779), (120, 2166, 9557), (140, 3095, 6274), (1, 2626, 4885), (33, 2561, 3541), (3653, 33, 5702),
-          (1370, 321, 6947), (123, 1374, 14983), (1, 32, 8836), (34, 814, 8161), (1454, 34, 12852), (1610, 72, 16138)]
+          (1370, 321, 6947), (123, 1374, 14983), (1, 32, 8836), (34, 814, 8161), (1454, 34, 12852), (1610, 72, 16138), (195, 9696, 1188),
+          (139, 11726, 762), (140, 11008, 534), (155, 10696, 33), (4, 4786, 8161), (35, 4300, 2844), (1870, 517, 4856), (30, 3497, 2275),
+          (1, 2441, 7291), (3695, 35, 9257), (2393, 142, 9751), (18, 34, 1533), (1, 32, 12445), (1369, 78, 13866), (18, 43, 1998)]
 # Up to 16 rows: every length of the registers that hold x, one and two groups of eight rows, rows of w that the ring holds and that it does not
 FEW = [(8, 32, 8836), (7, 126, 9360), (1, 32, 33), (5, 46, 32), (8, 34, 2234), (3, 39, 2064), (2, 33, 4292), (8, 47, 5408), (10, 42, 34), (13, 34, 32),
        (16, 37, 2310), (14, 32, 2736), (9, 38, 4452), (16, 32, 5328), (8, 3650, 9116), (2, 4034, 8944), (1, 14218, 1377), (5, 14860, 1312),
