@@ -45,8 +45,8 @@ struct Scales {
 // ------------------------------------------------------------------------------------------------
 // Few rows. The product is formed transposed: 128 rows of w are the M side of tcgen05.mma, up to 256 rows of x (a multiple of
 // 16, `bn`) its N side, so a weight byte goes HBM -> TMA -> shared memory -> tensor core, and the accumulator [128 rows of
-// w x bn] lies in tensor memory. Grid (c, tiles of x, tiles of w; those that share a tile of w run together): a cluster of c CTAs (a power of two) shares one tile, CTA r
-// streaming k blocks [r * kb_per_rank, ...) of it. Columns of the accumulator (rows of x) belong to the CTAs by fours in turn: each
+// w x bn] lies in tensor memory. Grid (c, tiles of x, tiles of w; those that share a tile of w run together): a cluster of c CTAs (a
+// power of two) shares one tile, CTA r streaming k blocks [r * kb_per_rank, ...) of it. Columns of the accumulator (rows of x) belong to the CTAs by fours in turn: each
 // deposits what it has of the others' columns in their shared memory, 16 bytes a channel, and adds to its own, which stay in tensor
 // memory, what the others left there. (All of a channel's columns to one CTA, its own part through shared memory too, us: 264 x 4096 x 12288
 // 19.2 for 18.3, 400 x 2048 x 8192 14.5 for 12.5, 256 x 512 x 16384 10.2 for 9.2, 24 x 1024 x 1024 3.7 for 3.55.)
@@ -838,8 +838,8 @@ int launch_few(TOut* out, long long ldo, const void* x, long long ldx, const voi
 // median 1.00.
 // Few rows: a stage of 128 bytes of K is 16 KB of w and `cols` rows of x at what one SM takes in, for as many CTAs as an SM has to
 // run; the weight's bytes come from memory and all copies through L2 (21 TB/s, less beside memory's). Every round of CTAs costs 2.2 around
-// its first copy and its results, 0.004 to 0.009 a column of the accumulator, or added up over a cluster 1.4 and 0.025 to 0.034 a column sent. Clusters of four
-// and eight do not fill the SMs (35 of four: two rounds).
+// its first copy and its results, 0.004 to 0.009 a column of the accumulator, or added up over a cluster 1.4 and 0.025 to 0.034 a column
+// sent. Clusters of four and eight do not fill the SMs (35 of four: two rounds).
 // Many rows: 4.5, and for each round of tiles its stages (16 KB of w and half the tile's rows of x for each CTA) or, where sums are
 // short, its results, which take longer where result rows do not start and end on 16-byte borders.
 float few_rows_us(int M, int N, int num_kb, int c, int z, int sms) {
@@ -849,7 +849,8 @@ float few_rows_us(int M, int N, int num_kb, int c, int z, int sms) {
   const float rounds = (float)((ctas + at_once * on_an_sm - 1) / (at_once * on_an_sm));
   const float products = (float)((ctas + at_once - 1) / at_once) * kb * (0.171f + 0.00064f * cols);
   const float memory = (float)N * num_kb * BK / 6.4e6f, l2 = (float)ctas * kb * BK * (BM + cols) / 20.8e6f + 0.6f * memory;
-  const float sent = cols * (c - 1.f) / c, results = c > 1 ? 0.38f + (sent < 32.f ? 0.025f * sent : 0.8f + 0.034f * (sent - 32.f)) : (bn > 128 ? 0.0086f : 0.004f) * bn;
+  const float sent = cols * (c - 1.f) / c, added = 0.38f + (sent < 32.f ? 0.025f * sent : 0.8f + 0.034f * (sent - 32.f));
+  const float results = c > 1 ? added : (bn > 128 ? 0.0086f : 0.004f) * bn;
   const float around = (c > 1 ? 3.26f : 2.23f) + results * on_an_sm, copies = memory > l2 ? memory : l2, work = products + (rounds - 1.f) * around;
   return around + (work > copies ? work : copies);
 }

@@ -354,13 +354,15 @@ rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows
   }
 }
 
-// Many wide rows. What bounds the kernel above there is that registers hold what is on the way as well as what is at hand: of a norm's row of
-// 12,288 with its residual one block fits an SM, and nothing is on the way while it exchanges and stores. Here rows come into shared memory by
-// bulk copies, two or more ahead, one or two blocks an SM take them in turn, and a norm's weights stay in registers. A row is shared
-// out as above, so its bits are the same. Measured (us, above -> this; bfloat16 norm with residual, without, plain rows): 4096 x 8704 58.0 -> 49.3,
-// 47.3 -> 44.1, 28.4 -> 23.3; 4096 x 12288 97.2 -> 57.0 (6.2 TB/s), 83.6 -> 46.1, 34.7 -> 28.7; 1200 x 12288, from L2, 21.9 -> 18.1, 19.3 -> 16.3,
-// 9.0 -> 9.4; 4096 x 16384 110 -> 87, 93 -> 54, 46.6 -> 35.6; 300 x 12288 7.5 -> 8.1; gates and rows of up to 8,192 are faster above, and so are
-// float32's plain rows (4096 x 12288 38 -> 43). Bound by memory; with a ring of two rows (16384 with residual) by the wait for the next.
+// Many wide rows. What bounds the kernel above there is that registers hold what is on the way as well as what is at hand: of a norm's
+// row of 12,288 with its residual one block fits an SM, and nothing is on the way while it exchanges and stores. Here rows come into
+// shared memory by bulk copies, two or more ahead, one or two blocks an SM take them in turn, and a norm's weights stay in registers. A
+// row is shared out as above, so its bits are the same. Measured (us, above -> this; bfloat16 norm with residual, without, plain rows):
+//   4096 x 8704   58.0 -> 49.3, 47.3 -> 44.1, 28.4 -> 23.3        1200 x 12288, from L2   21.9 -> 18.1, 19.3 -> 16.3, 9.0 -> 9.4
+//   4096 x 12288  97.2 -> 57.0 (6.2 TB/s), 83.6 -> 46.1, 34.7 -> 28.7        300 x 12288, from L2   7.5 -> 8.1, 7.1 -> 7.5, 3.8 -> 4.5
+//   4096 x 16384  110 -> 87, 93 -> 54, 46.6 -> 35.6
+// Gates and rows of up to 8,192 are faster above, and so are float32's plain rows (4096 x 12288 38 -> 43). Bound by memory; with a ring of
+// two or three rows for one block (16384 with residual) by the wait for the next.
 constexpr int kRingMost = 8, kRingUnits = 4, kRingBytes = 208 * 1024;
 
 template <typename Row>
