@@ -159,6 +159,21 @@ def test_norm_takes_itself_as_the_residual_and_one_row_for_all(int8):
     assert torch.equal(b, x + one)
 
 
+@pytest.mark.parametrize("first", [0, 1])
+def test_norm_of_rows_and_residuals_that_lie_in_turn(int8, first):
+    """x and delta are the halves of one matrix's rows: they share a range of memory and no number."""
+    both, w = randn(7, 512, dtype=torch.bfloat16).to(DEV), torch.ones(256, device=DEV)
+    halves = both[:, :256], both[:, 256:]
+    x, delta = halves[first], halves[1 - first]
+    alone, d = x.clone(), delta.clone()
+    want = int8.rmsnorm_int8(alone, w, 1e-6, delta=d)
+    held = int8.rmsnorm_int8(x, w, 1e-6, delta=delta)
+    assert torch.equal(x, alone) and torch.equal(delta, d)
+    assert torch.equal(held.values, want.values) and torch.equal(held.scales, want.scales)
+    with pytest.raises(int8.KernelError, match="not overlap"):
+        int8.rmsnorm_int8(both[:, :256], w, 1e-6, delta=both[:, 128:384])
+
+
 @pytest.mark.parametrize("width", [64, 256, 1024, 4096, 5001])
 def test_a_row_does_not_depend_on_the_rows_around_it(int8, width):
     x = randn(3000, width, dtype=torch.bfloat16).to(DEV)
