@@ -76,7 +76,8 @@ typedef __nv_bfloat16 bf16;
 // ---------------------------------------------------------------------------------------------
 int oi_pdl_enabled();
 void oi_fence_next_launch();   // the next kernel launched through oi_launch gets plain stream order (once)
-int oi_take_launch_fence();
+void oi_fence_stream(cudaStream_t stream);   // the next kernel launched through oi_launch on this stream does, whatever thread launches it (once)
+int oi_take_launch_fence(cudaStream_t stream);
 int oi_sm_count();         // multiprocessors of the device that was current at the first question (148 on a B200)
 void oi_count_launch();   // every kernel launched through oi_launch is counted (oi_launches)
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
@@ -98,7 +99,7 @@ inline void oi_launch_cluster(void (*kernel)(Params...), dim3 grid, dim3 block, 
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int na = 0;
-  const int fenced = oi_take_launch_fence();
+  const int fenced = oi_take_launch_fence(stream);
   if (oi_pdl_enabled() && !fenced) {
     attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[na].val.programmaticStreamSerializationAllowed = 1;

@@ -349,6 +349,7 @@ OI_API int oi_abi_version();
 OI_API unsigned long long oi_launches();
 OI_API int oi_launch_fence();   // the next kernel that the calling host thread launches gets plain stream order (once)
 OI_API int oi_launch_fence_pending();   // whether the calling thread's next kernel will
+OI_API int oi_stream_fence_pending(void* stream);   // whether the next kernel on this stream will, whatever thread launches it
 OI_API int oi_set_pdl(int enabled);
 OI_API int oi_device_info(int device, int* sm_major, int* sm_minor, int* sm_count, long long* l2_bytes);
 

@@ -564,7 +564,7 @@ bool on_borders(const void* p, long long ld, int esize) { return (uintptr_t)p % 
 template <typename T, bool kVec, bool kWide, int kTimes>
 __global__ void __launch_bounds__(256) dequantize_kernel(T* out, long long ldo, const signed char* q, long long ldq, const float* scales, int rows,
                                                          int cols, int lanes_log) {
-  pdl_start();
+  pdl_wait();                    // and no early trigger: see launch_dequantize
   if constexpr (kWide) lanes_log = 8;
   const int lanes = 1 << lanes_log, lane = threadIdx.x & (lanes - 1), step = kVec ? 1 : lanes;
   const long long r = ((long long)blockIdx.x << (8 - lanes_log)) + (threadIdx.x >> lanes_log);
@@ -607,6 +607,8 @@ __global__ void __launch_bounds__(256) dequantize_kernel(T* out, long long ldo, 
   }
 }
 
+// What is written may be a weight or a cache that later kernels read before their wait (a weight brought back for a bfloat16 product):
+// the kernel behind it on its stream starts when it has finished, whatever thread launches that one and whatever runs on other streams.
 template <typename T>
 int launch_dequantize(T* out, long long ldo, const signed char* q, long long ldq, const float* scales, int rows, int cols, cudaStream_t s) {
   const bool vec = on_borders(out, rows > 1 ? ldo : 0, sizeof(T));
@@ -621,6 +623,7 @@ int launch_dequantize(T* out, long long ldo, const signed char* q, long long ldq
   if (two) wide ? go(dequantize_kernel<T, true, true, 2>) : go(dequantize_kernel<T, true, false, 2>);
   else if (vec) wide ? go(dequantize_kernel<T, true, true, 1>) : go(dequantize_kernel<T, true, false, 1>);
   else wide ? go(dequantize_kernel<T, false, true, 1>) : go(dequantize_kernel<T, false, false, 1>);
+  oi_fence_stream(s);
   return OI_OK;
 }
 

@@ -1,6 +1,12 @@
 // Error reporting of the C ABI and a few device queries.
 #include <stdarg.h>
 
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+#include <utility>
+#include <vector>
+
 #include "common.cuh"
 
 static thread_local char g_error[512] = "";
@@ -31,9 +37,40 @@ OI_API int oi_launch_fence() {
   return OI_OK;
 }
 OI_API int oi_launch_fence_pending() { return g_fence_next; }
-int oi_take_launch_fence() {
-  const int v = g_fence_next;
+// The same for a stream: the next launch on it, by whatever thread, and no launch on another one. The streams (with their
+// devices) whose next launch that is; their number is looked at by each launch, the list only where there are some.
+static std::atomic<int> g_fenced_streams{0};
+static std::mutex g_streams_lock;
+static std::vector<std::pair<int, cudaStream_t>> g_streams;
+static std::pair<int, cudaStream_t> on_its_device(cudaStream_t stream) {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
+  return {dev, stream};
+}
+void oi_fence_stream(cudaStream_t stream) {
+  const auto it = on_its_device(stream);
+  std::lock_guard<std::mutex> hold(g_streams_lock);
+  if (std::find(g_streams.begin(), g_streams.end(), it) == g_streams.end()) g_streams.push_back(it);
+  g_fenced_streams.store((int)g_streams.size(), std::memory_order_release);
+}
+OI_API int oi_stream_fence_pending(void* stream) {
+  const auto it = on_its_device((cudaStream_t)stream);
+  std::lock_guard<std::mutex> hold(g_streams_lock);
+  return std::find(g_streams.begin(), g_streams.end(), it) != g_streams.end();
+}
+int oi_take_launch_fence(cudaStream_t stream) {
+  int v = g_fence_next;
   g_fence_next = 0;
+  if (g_fenced_streams.load(std::memory_order_acquire) != 0) {
+    const auto it = on_its_device(stream);
+    std::lock_guard<std::mutex> hold(g_streams_lock);
+    const auto at = std::find(g_streams.begin(), g_streams.end(), it);
+    if (at != g_streams.end()) {
+      g_streams.erase(at);
+      v = 1;
+    }
+    g_fenced_streams.store((int)g_streams.size(), std::memory_order_release);
+  }
   return v;
 }
 

@@ -212,7 +212,8 @@ def _results(out: Optional[torch.Tensor], dtype: torch.dtype, rows: int, width: 
 
 
 def dequantize_int8(rows: Int8Rows, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The numbers that 8-bit rows stand for, rounded once to ``dtype`` (float32 or bfloat16) or to that of ``out`` (row stride free)."""
+    """The numbers that 8-bit rows stand for, rounded once to ``dtype`` (float32 or bfloat16) or to that of ``out`` (row stride free).
+    They may be a weight, which a product fetches ahead: the next kernel on the stream starts when they are written."""
     q, ldq, count, width, scales, device = _int8_rows(*rows, "dequantize_int8")
     if _elsewhere(device):
         with torch.cuda.device(device):

@@ -159,3 +159,19 @@ def test_a_weight_given_other_tensors_is_waited_for_again():
     w.stream = 7
     w.operands()
     assert w.stream == 7
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: the launches have to fail")
+def test_the_kernel_behind_a_way_back_starts_when_that_has_finished():
+    """What ``dequantize_int8`` writes may be a weight, which products fetch ahead: the next launch on its stream, and on no other, is in
+    plain stream order."""
+    L = klib.load(verbose=False)
+    null, legacy, own = None, 1, 2                   # streams that are there without a device
+    for stream, others in ((null, (legacy, own)), (own, (null, legacy))):
+        L.oi_dequantize_int8(16, 1, 32, 16, 32, 16, 1, 32, stream)
+        assert L.oi_stream_fence_pending(stream) == 1
+        for other in others:
+            L.oi_quantize_int8(16, 32, 16, 16, 0, 32, 1, 32, 1, other)
+            assert L.oi_stream_fence_pending(other) == 0 and L.oi_stream_fence_pending(stream) == 1
+        L.oi_quantize_int8(16, 32, 16, 16, 0, 32, 1, 32, 1, stream)
+        assert L.oi_stream_fence_pending(stream) == 0

@@ -608,3 +608,52 @@ def test_refusals_on_the_device(int8):
                 lambda: int8.silu_mul_int8(torch.ones(3, 32, device=DEV), out=int8.empty_rows(3, 32, DEV))):
         with pytest.raises(KernelError):
             bad()
+
+
+@pytest.mark.parametrize("rows", [1, 8, 32])
+def test_a_weight_brought_back_is_not_fetched_ahead(int8, rows):
+    """A bfloat16 weight is written by ``dequantize_int8`` and multiplied at once, behind a kernel that takes a while: in a recorded
+    graph that is replayed with new values, and call by call with another stream's launch in between."""
+    from openinfer_b200.kernels.linear import linear
+    channels, width = 1024, 512
+    x = randn(rows, width, seed=1, dtype=torch.bfloat16).to(DEV)
+    held = [int8.quantize_int8(randn(channels, width, seed=s).to(DEV)) for s in range(4)]
+    want = []
+    for h in held:
+        w = int8.dequantize_int8(h)
+        torch.cuda.synchronize()
+        want.append(linear(x, w))
+    now, weight, busy = int8.empty_rows(channels, width, DEV), torch.zeros(channels, width, dtype=torch.bfloat16, device=DEV), randn(8192, 4096).to(DEV)
+
+    def chain():
+        for _ in range(4):
+            int8.quantize_int8(busy)
+        int8.dequantize_int8(now, out=weight)
+        return linear(x, weight)
+
+    def put(i):
+        now.values.copy_(held[i].values)
+        now.scales.copy_(held[i].scales)
+    put(0)
+    chain()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain()
+    for i in (1, 2, 3, 0, 2, 1):
+        put(i)
+        graph.replay()
+        assert torch.equal(got, want[i])
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in (1, 2, 3, 0, 2, 1):
+        with torch.cuda.stream(side):
+            put(i)
+            int8.quantize_int8(busy)
+            int8.dequantize_int8(now, out=weight)
+        with torch.cuda.stream(other):
+            int8.quantize_int8(x)
+        with torch.cuda.stream(side):
+            again = linear(x, weight)
+        torch.cuda.synchronize()
+        assert torch.equal(again, want[i])
