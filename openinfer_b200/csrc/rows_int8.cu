@@ -624,6 +624,7 @@ int launch_dequantize(T* out, long long ldo, const signed char* q, long long ldq
   else if (vec) wide ? go(dequantize_kernel<T, true, true, 1>) : go(dequantize_kernel<T, true, false, 1>);
   else wide ? go(dequantize_kernel<T, false, true, 1>) : go(dequantize_kernel<T, false, false, 1>);
   oi_fence_stream(s);
+  OI_CHECK_LAUNCH();
   return OI_OK;
 }
 

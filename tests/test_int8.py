@@ -175,3 +175,17 @@ def test_the_kernel_behind_a_way_back_starts_when_that_has_finished():
             assert L.oi_stream_fence_pending(other) == 0 and L.oi_stream_fence_pending(stream) == 1
         L.oi_quantize_int8(16, 32, 16, 16, 0, 32, 1, 32, 1, stream)
         assert L.oi_stream_fence_pending(stream) == 0
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: the launches have to fail")
+@pytest.mark.parametrize("name,args", [
+    ("oi_quantize_int8", (16, 32, 16, 16, 0, 32, 1, 32, 1)),
+    ("oi_rmsnorm_int8", (16, 32, 16, 16, 32, 0, 0, 0, 16, 0, 1, 32, 1e-6, 0.0, 1)),
+    ("oi_silu_mul_int8", (16, 32, 16, 16, 0, 64, 1, 32, 32, 1, 1)),
+    ("oi_dequantize_int8", (16, 1, 32, 16, 32, 16, 1, 32)),
+    ("oi_dequantize_int8", (16, 0, 32, 16, 32, 16, 1, 32)),
+    ("oi_linear_int8", (16, 1, 8, 16, 32, 16, 16, 32, 16, 0, 1, 8, 32)),
+])
+def test_a_launch_that_fails_is_an_error_of_its_call(name, args):
+    L = klib.load(verbose=False)
+    assert getattr(L, name)(*args, None) > 1
