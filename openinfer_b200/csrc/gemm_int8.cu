@@ -526,7 +526,8 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 // tensor-memory round trip, deposits and a cluster barrier there. One CTA per SM owns whole rows of w, 16 at a time, so no sums cross
 // CTAs:
 //   warp 8     copies rows into shared memory (cp.async.bulk, one copy per row of a stage, counted on an mbarrier), as many as the
-//              ring holds before the kernel ahead on the stream has finished
+//              ring holds before the kernel ahead on the stream has finished; it waits for that one, however long it takes, before
+//              it waits for a free stage, which is bounded
 //   warps 0-7  share out K (blocks of 128 bytes in turn). After the wait a warp reads its part of x straight into the registers that
 //              mma.sync takes as operand B (rows of x on the 8-column side); 16 rows of w are operand A. The k index inside a block is
 //              permuted alike for both, so 32 contiguous bytes of a row are a lane's fragments of four products. The eight warps'
@@ -614,13 +615,16 @@ linear_int8_few_kernel(const __grid_constant__ FewArgs a) {
     const unsigned long long once = tc::policy_evict_first();
     Ring at;
     int ahead = a.stages;
-    bool ok = true;
+    bool ok = true, waited = false;
     for (int grp = blockIdx.x; grp < a.groups && ok; grp += gridDim.x) {
       const int rows = min(16, a.N - grp * 16);
       const signed char* from = a.w + (size_t)grp * 16 * a.ldw;
       for (int c = 0; c < chunks; ++c, at.next(a.stages)) {
         if (ahead > 0) --ahead;
-        else if (!wait_on(empty_bar(at.stage), at.parity ^ 1, abort_flag, 21)) { ok = false; break; }
+        else {
+          if (!waited) pdl_wait(), waited = true;
+          if (!wait_on(empty_bar(at.stage), at.parity ^ 1, abort_flag, 21)) { ok = false; break; }
+        }
         const int k0 = (c + turn < chunks ? c + turn : c + turn - chunks) * kChunk;
         const unsigned len = (unsigned)min((a.K - k0 + 15) & ~15, kChunk), dst = ring + at.stage * kFewStage;
         if (leader) tc::mbar_expect_tx(full_bar(at.stage), rows * len);

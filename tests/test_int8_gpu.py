@@ -657,3 +657,29 @@ def test_a_weight_brought_back_is_not_fetched_ahead(int8, rows):
             again = linear(x, weight)
         torch.cuda.synchronize()
         assert torch.equal(again, want[i])
+
+
+@pytest.mark.parametrize("rows", [1, 16, 40])
+def test_a_product_behind_kernels_that_take_longer_than_its_own_waits_may(int8, rows):
+    """Its waits are bounded (two seconds) from when the kernels ahead have finished, not from when it has been started."""
+    x = int8.quantize_int8(randn(rows, 4096, seed=1).to(DEV))
+    weight = int8.Int8Weight.quantize(randn(24576, 4096, seed=2).to(DEV))
+    want = int8.linear_int8(x, weight)
+    width = 1 << 30                                    # one block's work for a second
+    zeros, norm_w = (torch.zeros(*shape, width, dtype=torch.bfloat16, device=DEV) for shape in ((1,), ()))
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+
+    def busy(times):
+        start.record()
+        for _ in range(times):
+            int8.rmsnorm_int8(zeros, norm_w, 1e-6, delta=zeros)
+    busy(1)
+    end.record()
+    torch.cuda.synchronize()
+    times = int(3000 / start.elapsed_time(end)) + 1
+    busy(times)
+    got = int8.linear_int8(x, weight)
+    end.record()
+    torch.cuda.synchronize()
+    assert start.elapsed_time(end) > 2500
+    assert torch.equal(got, want) and int8.status() == 0
