@@ -5,8 +5,11 @@
 //
 // Three kernels: for up to 16 rows on mma.sync, for few and for many rows on tcgen05. The operands of the latter two are staged by TMA as
 // rows of 128 bytes (128-byte swizzle); bytes beyond K or beyond the last row are zeros of the copy. Every wait on an mbarrier is
-// bounded: one that runs out sets an error word and a flag that ends all roles of the CTA, which still joins its cluster's barriers,
-// frees its tensor memory and returns. No load uses cluster multicast.
+// bounded: one that runs out sets an error word and a flag that ends all roles of the CTA, which writes NaN for the results that it did
+// not come to (of a cluster that adds up sums, all its CTAs do), still joins its cluster's barriers, frees its tensor memory and
+// returns. No load uses cluster multicast.
+#include <atomic>
+
 #include "oi_api.h"
 #include "tcgen05.cuh"
 
@@ -20,7 +23,15 @@ constexpr int kBoxBytes = BM * BK;
 
 __device__ int g_int8_error = 0;            // set to a non-zero code when a bounded wait ran out
 
-__device__ __forceinline__ bool wait_on(unsigned bar, unsigned parity, volatile int* abort_flag, int code) {
+// `runs_out`: the code of the wait that is taken as having run out, 0: none (oi_linear_int8_run_out, for tests)
+std::atomic<int> g_runs_out{0};
+__device__ __forceinline__ bool run_out(volatile int* abort_flag, int code) {
+  *abort_flag = 1;
+  atomicCAS(&g_int8_error, 0, code);
+  return false;
+}
+__device__ __forceinline__ bool wait_on(unsigned bar, unsigned parity, volatile int* abort_flag, int code, int runs_out) {
+  if (code == runs_out) return run_out(abort_flag, code);
   return tc::mbar_wait(bar, parity, abort_flag, &g_int8_error, code);
 }
 __device__ __forceinline__ float finish(int sum, float sx, float sw, float b, bool biased) {
@@ -68,6 +79,7 @@ struct Shape {
   int recv_offset;          // where deposits go: behind the ring, or over the drained ring (0)
   int scale_offset;         // scales of the tile's rows of x [bn]
   int bar_offset;
+  int runs_out;
 };
 
 template <typename TOut, int kReaders>
@@ -129,7 +141,7 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
   const int cols = min(g.bn, g.M - m0);  // rows of x in this tile
   const int quarter = warp & 3;          // a warp may only touch lanes [32 * (warp % 4), +32) of tensor memory
   const int row = quarter * 32 + lane, n = n0 + row;
-  const float sw = n < g.N ? scales.sw[n] : 0.f;
+  float sw = n < g.N ? scales.sw[n] : 0.f;
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -144,13 +156,13 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
   const bool biased = scales.bias != nullptr;
   const float b = biased && n < g.N ? scales.bias[n] : 0.f;
 
-  bool ok = true;
+  bool ok = !misaligned;
   if (warp == 0) {
     const bool leader = tc::elect_one();
     Ring at;
     for (int kb = g.stages; kb < nkb; ++kb, at.next(g.stages)) {
       const int s = at.stage;
-      if (!wait_on(empty_bar(s), at.parity, abort_flag, 1)) break;
+      if (!wait_on(empty_bar(s), at.parity, abort_flag, 1, g.runs_out)) break;
       if (leader) {
         tc::mbar_expect_tx(full_bar(s), stage_bytes);
         const unsigned dst = smem_base + s * stage_bytes;
@@ -165,7 +177,7 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     Ring at;
     for (int kb = 0; kb < nkb; ++kb, at.next(g.stages)) {
       const int s = at.stage;
-      ok = wait_on(full_bar(s), at.parity, abort_flag, 2);
+      ok = wait_on(full_bar(s), at.parity, abort_flag, 2, g.runs_out);
       if (!ok) break;
       tc::fence_after();
       const unsigned a_addr = smem_base + s * stage_bytes;
@@ -180,9 +192,11 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     }
     if (leader && ok && nkb > 0) tc::umma_commit(acc_full);
   } else if (nkb > 0) {
-    ok = wait_on(acc_full, 0, abort_flag, 3);
+    ok = __all_sync(0xffffffffu, wait_on(acc_full, 0, abort_flag, 3, g.runs_out));
     tc::fence_after();
   }
+  const float nan = __int_as_float(0x7fffffff);
+  if (!ok) sw = nan;                     // of a sum that did not come
   if (csize > 1) {
     __syncwarp();
     tc::cluster_wait();                  // phase 0
@@ -237,9 +251,12 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     }
   }
   if (csize > 1) {
+    if (warp >= 2 && !ok && lane < csize)  // the CTAs that add up hear of a part that did not come
+      asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(tc::map_to_rank(tc::smem_u32((const void*)abort_flag), lane)), "r"(1) : "memory");
     __syncwarp();
     tc::cluster_arrive();                // this CTA's deposits are made ...
     tc::cluster_wait();                  // ... and so are everybody's; nothing remote is touched after this
+    if (*abort_flag) sw = nan;
     if (warp >= 2) {
       const unsigned char* mine = smem + g.recv_offset + (size_t)row * 16;
 #pragma unroll 1
@@ -312,7 +329,7 @@ template <typename TOut>
 __global__ void __launch_bounds__(kPairThreads)
 linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                         const __grid_constant__ CUtensorMap map_out, TOut* out, long long ldo, const Scales scales, int M, int N, int num_kb,
-                        int bn, int stages, int tma_out) {
+                        int bn, int stages, int tma_out, int runs_out) {
   pdl_start();
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -363,7 +380,7 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
       for (int kb = 0; kb < num_kb; ++kb, at.next(stages)) {
         const int s = at.stage;
         if (ahead > 0) --ahead;
-        else if (!wait_on(empty_bar(s), at.parity ^ 1, abort_flag, 11)) { ok = false; break; }
+        else if (!wait_on(empty_bar(s), at.parity ^ 1, abort_flag, 11, runs_out)) { ok = false; break; }
         if (leader) {
           if (rank == 0) tc::mbar_expect_tx(full_bar(s), 2 * stage_bytes);
           const unsigned counted_on = tc::map_to_rank(full_bar(s), 0);
@@ -384,14 +401,15 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
       for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local) {
         const int a = local & 1;
         if (local >= 2) {
-          ok = tc::mbar_wait_cluster(acc_empty_bar(a), (unsigned)((local >> 1) - 1) & 1, abort_flag, &g_int8_error, 14);
+          ok = runs_out == 14 ? run_out(abort_flag, 14)
+                              : tc::mbar_wait_cluster(acc_empty_bar(a), (unsigned)((local >> 1) - 1) & 1, abort_flag, &g_int8_error, 14);
           if (!ok) break;
           tc::fence_after();
         }
         const unsigned tmem_acc = tmem_base + (unsigned)(a * 256);
         for (int kb = 0; kb < num_kb; ++kb, at.next(stages)) {
           const int s = at.stage;
-          ok = wait_on(full_bar(s), at.parity, abort_flag, 12);
+          ok = wait_on(full_bar(s), at.parity, abort_flag, 12, runs_out);
           if (!ok) break;
           tc::fence_after();
           const unsigned a_addr = smem_base + s * stage_bytes;
@@ -431,23 +449,25 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
       }
     };
     ask(pair);
+    bool ok = true;
     for (int tile = pair; tile < num_tiles; tile += num_pairs, ++local) {
       const int a = local & 1;
       const int m0 = (tile % m_tiles) * bn, n0 = (tile / m_tiles) * 256 + (int)rank * 128 + quarter * 32;
-      const float sw = next_sw, b = next_b;
+      float sw = next_sw, b = next_b;
       sx_s[lane] = next_sx[0];
       sx_s[32 + lane] = next_sx[1];
       __syncwarp();
       ask(tile + num_pairs);
-      if (!wait_on(acc_full_bar(a), (unsigned)(local >> 1) & 1, abort_flag, 13)) break;
+      if (ok) ok = __all_sync(0xffffffffu, wait_on(acc_full_bar(a), (unsigned)(local >> 1) & 1, abort_flag, 13, runs_out));
       tc::fence_after();
+      if (!ok) sw = __int_as_float(0x7fffffff);      // of sums that did not come
       const unsigned tmem_acc = tmem_base + (unsigned)(a * 256) + ((unsigned)(quarter * 32) << 16);
       const int turns = ((min(bn, M - m0) + kTake - 1) / kTake - part + kParts - 1) / kParts;      // groups of rows that are this warp's
 #pragma unroll 1
       for (int i = 0; i < kTurns; ++i) {
         unsigned v[kTake];
         const int row0 = (i * kParts + part) * kTake;
-        if (i < turns) {
+        if (i < turns && ok) {
           if constexpr (kTake == 32) tc::tmem_ld32(tmem_acc + (unsigned)row0, v);
           else tc::tmem_ld16(tmem_acc + (unsigned)row0, v);
           tc::tmem_ld_wait();
@@ -553,6 +573,7 @@ struct FewArgs {
   Scales scales;
   int M, N, K, groups, stages;
   int at_once;              // the ring holds all of a CTA's rows
+  int runs_out;
 };
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
@@ -623,7 +644,7 @@ linear_int8_few_kernel(const __grid_constant__ FewArgs a) {
         if (ahead > 0) --ahead;
         else {
           if (!waited) pdl_wait(), waited = true;
-          if (!wait_on(empty_bar(at.stage), at.parity ^ 1, abort_flag, 21)) { ok = false; break; }
+          if (!wait_on(empty_bar(at.stage), at.parity ^ 1, abort_flag, 21, a.runs_out)) { ok = false; break; }
         }
         const int k0 = (c + turn < chunks ? c + turn : c + turn - chunks) * kChunk;
         const unsigned len = (unsigned)min((a.K - k0 + 15) & ~15, kChunk), dst = ring + at.stage * kFewStage;
@@ -651,7 +672,7 @@ linear_int8_few_kernel(const __grid_constant__ FewArgs a) {
     const bool biased = a.scales.bias != nullptr;
     auto channel = [&](int first) { return ((long long)first + f * (int)gridDim.x) * 16 + col; };
     auto asked = [&](const float* of, int first) { return channel(first) < a.N ? of[channel(first)] : 0.f; };
-    bool ok = wait_on(full_bar(0), 0, abort_flag, 22);       // weights: not waited for behind x
+    bool ok = wait_on(full_bar(0), 0, abort_flag, 22, a.runs_out);       // weights: not waited for behind x
     pdl_wait();
     uint4 xr[B][NT][2];
 #pragma unroll
@@ -679,7 +700,7 @@ linear_int8_few_kernel(const __grid_constant__ FewArgs a) {
 #pragma unroll
       for (int c = 0; c < B / kChunkBlocks; ++c) {
         if (c < chunks) {
-          if (ok) ok = wait_on(full_bar(at.stage), at.parity, abort_flag, 22);
+          if (ok) ok = wait_on(full_bar(at.stage), at.parity, abort_flag, 22, a.runs_out);
           const unsigned src = my_w + at.stage * kFewStage;
 #pragma unroll
           for (int j = 0; j < kChunkBlocks; ++j) {
@@ -713,6 +734,7 @@ linear_int8_few_kernel(const __grid_constant__ FewArgs a) {
       const bool last = grp + (int)gridDim.x >= a.groups;
       if (++held == kHeld || last) {
         few_sync();
+        if (*abort_flag) sw = __int_as_float(0x7fffffff);    // of sums that did not come
         const long long n = channel(first);
         if (f < held && m < a.M && n < a.N) {
           const int* src = part + f * kFewWarps * kEach + col * kTokens + m;
@@ -747,7 +769,7 @@ template <typename TOut>
 int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
                 int c, int z, cudaStream_t s) {
   Shape g = {};
-  g.M = M, g.N = N;
+  g.M = M, g.N = N, g.runs_out = g_runs_out;
   g.bn = ceil_div(ceil_div(M, z), 16) * 16;                            // z tiles of x, of equal size
   g.num_kb = ceil_div(K, BK);
   g.kb_per_rank = ceil_div(g.num_kb, c);
@@ -802,7 +824,8 @@ int launch_pair(TOut* out, long long ldo, const void* x, long long ldx, const vo
   OI_REQUIRE(tiles < (1LL << 30), "linear_int8: %d rows of %d results are too many", M, N);
   const int most = oi_sm_count() / 2, pairs = tiles < most ? (int)tiles : most;
   const int fit = kPairRingBytes / (kBoxBytes + bn / 2 * BK), stages = fit < kPairMostStages ? fit : kPairMostStages;
-  oi_launch_cluster(kernel, 2 * pairs, kPairThreads, kPairSmem, s, 2, mw, mx, mo, out, ldo, scales, M, N, ceil_div(K, BK), bn, stages, (int)tma_out);
+  oi_launch_cluster(kernel, 2 * pairs, kPairThreads, kPairSmem, s, 2, mw, mx, mo, out, ldo, scales, M, N, ceil_div(K, BK), bn, stages, (int)tma_out,
+                    g_runs_out.load());
   OI_CHECK_LAUNCH();
   return OI_OK;
 }
@@ -813,7 +836,7 @@ int few_longest(int M) { return M <= 8 ? 12288 : M <= 16 ? 8192 : 0; }
 template <typename TOut>
 int launch_few(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
                cudaStream_t s) {
-  FewArgs f = {(const signed char*)x, (const signed char*)w, out, ldx, ldw, ldo, scales, M, N, K, ceil_div(N, 16), 0, 0};
+  FewArgs f = {(const signed char*)x, (const signed char*)w, out, ldx, ldw, ldo, scales, M, N, K, ceil_div(N, 16), 0, 0, g_runs_out};
   const int chunks = ceil_div(K, kChunk), grid = f.groups < oi_sm_count() ? f.groups : oi_sm_count();
   const long long wanted = (long long)ceil_div(f.groups, grid) * chunks;
   f.stages = wanted < kFewMostStages ? (int)wanted : kFewMostStages;
@@ -930,5 +953,11 @@ OI_API int oi_linear_int8_status(int* status) {
   }
   if (int rc = oi_take_rows_int8_error(status)) return rc;
   if (v != 0) *status = v;
+  return OI_OK;
+}
+
+// For tests: products launched from now on take the wait of this code as having run out (0: none).
+OI_API int oi_linear_int8_run_out(int code) {
+  g_runs_out = code;
   return OI_OK;
 }

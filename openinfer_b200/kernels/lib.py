@@ -101,6 +101,7 @@ _SIGNATURES = {
     "oi_dequantize_int8": [P, I, L, P, L, P, I, I, P],
     "oi_linear_int8": [P, I, L, P, L, P, P, L, P, P, I, I, I, P],
     "oi_linear_int8_status": [ctypes.POINTER(c_int)],
+    "oi_linear_int8_run_out": [I],
     "oi_gemm_tcgen05_glu": [P, L, P, L, P, L, I, I, I, I, I, F, P],
 }
 

@@ -683,3 +683,30 @@ def test_a_product_behind_kernels_that_take_longer_than_its_own_waits_may(int8, 
     torch.cuda.synchronize()
     assert start.elapsed_time(end) > 2500
     assert torch.equal(got, want) and int8.status() == 0
+
+
+@pytest.mark.parametrize("rows,channels,width,code,all_of_it", [
+    (3, 24576, 4096, 21, False), (3, 500, 4096, 22, True), (16, 1000, 2048, 22, True),                                     # up to 16 rows
+    (40, 130, 60000, 1, True), (40, 130, 8192, 2, True), (40, 130, 8192, 3, True), (70, 24576, 1000, 2, True), (70, 24576, 1000, 3, True),      # few
+    (2050, 4999, 3000, 11, False), (2050, 4999, 3000, 12, True), (2050, 5000, 3000, 13, True), (2050, 5000, 3000, 14, False)])              # many
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_wait_that_runs_out_makes_results_that_are_no_numbers(int8, dtype, rows, channels, width, code, all_of_it):
+    """The kernel behaves as if its wait ``code`` had lasted too long: what it did not come to is NaN, the status names the wait, and
+    the next product is as ever."""
+    (x, sx), (w, sw) = integers(rows, width, 1), integers(channels, width, 2)
+    held, weight = on_device(int8, x, sx), int8.Int8Weight(w.to(DEV), sw.to(DEV))
+    want = product_exactly(x, sx, w, sw, None, dtype)
+    out = torch.full((rows, channels + 8), -7.0, dtype=dtype, device=DEV)
+    L = int8._lib.load()
+    torch.cuda.synchronize()
+    try:
+        L.oi_linear_int8_run_out(code)
+        int8.linear_int8(held, weight, out=out[:, :channels])
+    finally:
+        L.oi_linear_int8_run_out(0)
+    assert int8.status() == code and int8.status() == 0
+    got = out[:, :channels].cpu()
+    none = torch.isnan(got)
+    assert bool(none.any()) and (not all_of_it or bool(none.all()))
+    assert torch.equal(got[~none], want[~none]) and bool((out[:, channels:] == -7.0).all())
+    assert torch.equal(int8.linear_int8(held, weight, out_dtype=dtype).cpu(), want) and int8.status() == 0
