@@ -235,7 +235,7 @@ class Int8Weight:
     of the functions above. Of a change that torch does not count (through ``.data``, or of tensors made in inference mode) tell
     with ``changed()``."""
 
-    __slots__ = ("values", "scales", "channels", "width", "device", "stream", "_seen", "_operands", "_counted")
+    __slots__ = ("values", "scales", "stream", "_seen", "_operands")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor) -> None:
         if values.dim() != 2 or values.dtype != torch.int8 or scales.shape != values.shape[:1]:
@@ -249,16 +249,27 @@ class Int8Weight:
             held = empty_rows(rows, width, values.device).values
             held.copy_(values)
             values = held
-        self.values, self.scales, self.device = values, scales.contiguous(), values.device
-        self.channels, self.width = rows, width
+        self.values, self.scales = values, scales.contiguous()
         self.stream = None          # of the last product: what wrote the weight is known to be done there
-        self._seen, self._counted = None, not self.values.is_inference()
         self.operands()
 
     def __setattr__(self, name: str, value) -> None:
         object.__setattr__(self, name, value)
         if name in ("values", "scales"):
-            object.__setattr__(self, "stream", None)      # other tensors: as after a change
+            object.__setattr__(self, "stream", None)      # other tensors: as after a change, and looked at before the next product
+            object.__setattr__(self, "_seen", None)
+
+    @property
+    def channels(self) -> int:
+        return self.values.shape[0]
+
+    @property
+    def width(self) -> int:
+        return self.values.shape[1]
+
+    @property
+    def device(self) -> torch.device:
+        return self.values.device
 
     def changed(self) -> None:
         """The weight's tensors hold new values: the next product waits for what is ahead of it."""
@@ -267,7 +278,8 @@ class Int8Weight:
     def operands(self):
         """What ``_int8_rows`` says of the weight; asked again when its tensors have been given other memory or values."""
         values, scales = self.values, self.scales
-        seen = (values.data_ptr(), scales.data_ptr(), values.shape, values.stride(), scales.shape, values._version if self._counted else 0)
+        seen = (values.data_ptr(), scales.data_ptr(), values.shape, values.stride(), values.dtype, scales.shape, scales.stride(), scales.dtype,
+                None if values.is_inference() else values._version)
         if seen != self._seen:
             self._operands = _int8_rows(values, scales, "Int8Weight")
             self._seen, self.stream = seen, None

@@ -189,3 +189,45 @@ def test_the_kernel_behind_a_way_back_starts_when_that_has_finished():
 def test_a_launch_that_fails_is_an_error_of_its_call(name, args):
     L = klib.load(verbose=False)
     assert getattr(L, name)(*args, None) > 1
+
+
+def test_a_weight_given_tensors_of_another_kind():
+    def product(w, x=ROWS, words="not on a CUDA device"):
+        refused(words, int8.linear_int8, int8.Int8Rows(x, torch.ones(len(x))), w)
+
+    b = torch.arange(1.0, 7.0)
+    w = int8.Int8Weight(ROWS.clone(), b[:3])
+    product(w)
+    w.scales = b[::2]                                          # at the same address, every other one
+    product(w, words="3 scales")
+    w.scales = b[:3]
+    w.scales.data = b[::2]                                     # the same without an assignment to the weight
+    product(w, words="3 scales")
+    w.scales = b[:3]
+    w.values = w.values.view(torch.uint8)                      # the same bytes, other numbers
+    product(w, words="int8 with float32 scales")
+    w.values = ROWS.clone()
+    w.values.data = w.values.view(torch.uint8)
+    product(w, words="int8 with float32 scales")
+    w.values, w.scales = torch.zeros(5, 64, dtype=torch.int8), torch.ones(5)
+    assert (w.channels, w.width, w.device) == (5, 64, torch.device("cpu"))
+    product(w, words="a weight of 5 x 64")
+    product(w, x=torch.zeros(3, 64, dtype=torch.int8))
+
+
+@pytest.mark.parametrize("first,second", [(False, True), (True, False)])
+def test_a_weight_given_tensors_of_inference_mode_or_other_ones(first, second):
+    """Changes of ordinary tensors are seen whatever the weight was made with; those of inference mode are told with ``changed``."""
+    def made(inference):
+        with torch.inference_mode(inference):
+            return ROWS.clone()
+    w = int8.Int8Weight(made(first), SCALES.clone())
+    w.values = made(second)
+    w.operands()
+    w.stream = 7
+    w.operands()
+    assert w.stream == 7
+    with torch.inference_mode(second):
+        w.values.fill_(3)
+    w.operands()
+    assert w.stream == (7 if second else None)
