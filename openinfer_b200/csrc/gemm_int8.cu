@@ -765,12 +765,17 @@ bool rows_on_borders(const TOut* out, long long ldo, int N) {
   return (uintptr_t)out % 16 == 0 && ldo * sizeof(TOut) % 16 == 0 && N * sizeof(TOut) % 16 == 0;
 }
 
-template <typename TOut>
-int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
-                int c, int z, cudaStream_t s) {
+// The height of z tiles of x, of equal size. (In sixteens: fewer of that height may hold all rows, and only those are launched. The
+// estimate below goes by the z that was asked for: so its constants were measured. Over 24 sizes where that makes a difference: 50 x 2816
+// x 2304 7.3 us with the empty tiles, 6.95 without; 125 x 640 x 7424 7.9 and 7.7; others the same. Of a choice among full tiles alone
+// 551 x 128 x 1792 took 5.9 us instead of 5.4.)
+int few_rows_height(int M, int z) { return ceil_div(ceil_div(M, z), 16) * 16; }
+
+// What a launch for c slices of K and tiles of bn rows of x needs, and its shared memory
+Shape few_rows_shape(int M, int N, int K, int c, int bn, int& smem) {
+  const int z = ceil_div(M, bn);
   Shape g = {};
-  g.M = M, g.N = N, g.runs_out = g_runs_out;
-  g.bn = ceil_div(ceil_div(M, z), 16) * 16;                            // z tiles of x, of equal size
+  g.M = M, g.N = N, g.runs_out = g_runs_out, g.bn = bn;
   g.num_kb = ceil_div(K, BK);
   g.kb_per_rank = ceil_div(g.num_kb, c);
   g.tmem_cols = g.bn <= 32 ? 32 : g.bn <= 64 ? 64 : g.bn <= 128 ? 128 : 256;
@@ -785,7 +790,16 @@ int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const vo
   g.recv_offset = own_room ? g.stages * stage : 0;
   g.scale_offset = own_room ? g.recv_offset + recv : (g.stages * stage > recv ? g.stages * stage : recv);
   g.bar_offset = g.scale_offset + g.bn * 4;
-  const int smem = g.bar_offset + 8 * (2 * g.stages + 1) + 16;
+  smem = g.bar_offset + 8 * (2 * g.stages + 1) + 16;
+  return g;
+}
+
+template <typename TOut>
+int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
+                int c, int bn, cudaStream_t s) {
+  int smem = 0;
+  const Shape g = few_rows_shape(M, N, K, c, bn, smem);
+  const int z = ceil_div(M, bn);
   OI_REQUIRE(ceil_div(N, BM) <= 65535, "linear_int8: %d channels are too many for %d rows", N, M);
   CUtensorMap mw, mx;
   int rc = tc::make_map_2d_i8(&mw, w, N, K, ldw, BM);
@@ -803,6 +817,11 @@ int launch_rows(TOut* out, long long ldo, const void* x, long long ldx, const vo
   if (rc) return rc;
   OI_CHECK_LAUNCH();
   return OI_OK;
+}
+
+int pair_stages(int bn) {
+  const int fit = kPairRingBytes / (kBoxBytes + bn / 2 * BK);
+  return fit < kPairMostStages ? fit : kPairMostStages;
 }
 
 template <typename TOut>
@@ -823,7 +842,7 @@ int launch_pair(TOut* out, long long ldo, const void* x, long long ldx, const vo
   const long long tiles = (long long)ceil_div(M, bn) * ceil_div(N, 256);
   OI_REQUIRE(tiles < (1LL << 30), "linear_int8: %d rows of %d results are too many", M, N);
   const int most = oi_sm_count() / 2, pairs = tiles < most ? (int)tiles : most;
-  const int fit = kPairRingBytes / (kBoxBytes + bn / 2 * BK), stages = fit < kPairMostStages ? fit : kPairMostStages;
+  const int stages = pair_stages(bn);
   oi_launch_cluster(kernel, 2 * pairs, kPairThreads, kPairSmem, s, 2, mw, mx, mo, out, ldo, scales, M, N, ceil_div(K, BK), bn, stages, (int)tma_out,
                     g_runs_out.load());
   OI_CHECK_LAUNCH();
@@ -833,14 +852,23 @@ int launch_pair(TOut* out, long long ldo, const void* x, long long ldx, const vo
 // The longest row of w beside M rows of x, which lie in registers; 0: too many rows
 int few_longest(int M) { return M <= 8 ? 12288 : M <= 16 ? 8192 : 0; }
 
+// Stages of all the rows of w of a CTA, and of its ring
+long long few_wanted(int N, int K) {
+  const int groups = ceil_div(N, 16);
+  return (long long)ceil_div(groups, groups < oi_sm_count() ? groups : oi_sm_count()) * ceil_div(K, kChunk);
+}
+int few_stages(int N, int K) {
+  const long long wanted = few_wanted(N, K);
+  return wanted < kFewMostStages ? (int)wanted : kFewMostStages;
+}
+
 template <typename TOut>
 int launch_few(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
                cudaStream_t s) {
   FewArgs f = {(const signed char*)x, (const signed char*)w, out, ldx, ldw, ldo, scales, M, N, K, ceil_div(N, 16), 0, 0, g_runs_out};
   const int chunks = ceil_div(K, kChunk), grid = f.groups < oi_sm_count() ? f.groups : oi_sm_count();
-  const long long wanted = (long long)ceil_div(f.groups, grid) * chunks;
-  f.stages = wanted < kFewMostStages ? (int)wanted : kFewMostStages;
-  f.at_once = wanted <= kFewMostStages;
+  f.stages = few_stages(N, K);
+  f.at_once = few_wanted(N, K) <= kFewMostStages;
   const int smem = kFewPart + f.stages * (kFewStage + 16) + 16;
   auto go = [&](auto kernel, bool (&allowed)[64]) {
     if (int bad = tc::allow_smem(kernel, kFewPart + kFewMostStages * (kFewStage + 16) + 16, allowed)) return bad;
@@ -898,26 +926,37 @@ float many_rows_us(int M, int N, int num_kb, int bn, bool f32, bool on_borders, 
   return 4.5f + (work > memory ? work : memory + 0.05f * work);      // (of equal ones that with the least to do)
 }
 
-template <typename TOut>
-int launch(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
-           cudaStream_t s) {
+enum { kFew, kRows, kPairs };
+struct Choice {
+  int kernel, bn, c;          // bn: rows of x a tile; c: slices of K
+};
+
+Choice choose(int M, int N, int K, bool f32, bool on_borders) {
   const int num_kb = ceil_div(K, BK), sms = oi_sm_count(), least = ceil_div(M, 256);
-  int best_c = 0, best_z = 0;
-  int best_bn = 256;
-  float best = 3.4e38f;
+  Choice best = {kPairs, 256, 1};
+  float best_us = 3.4e38f;
   for (int bn = 32; bn <= 256; bn += 32) {
-    const float us = many_rows_us(M, N, num_kb, bn, sizeof(TOut) == 4, rows_on_borders(out, ldo, N), sms);
-    if (us <= best) best = us, best_bn = bn;
+    const float us = many_rows_us(M, N, num_kb, bn, f32, on_borders, sms);
+    if (us <= best_us) best_us = us, best.bn = bn;
   }
   if (least <= 16 && ceil_div(N, BM) <= 65535) {
     for (int z = least; z <= 4 * least + 4 && z <= ceil_div(M, 16); ++z)
       for (int c = 1; c <= 8 && (c == 1 || (c - 1) * ceil_div(num_kb, c) < num_kb); c *= 2) {     // no slice without a stage
         const float us = few_rows_us(M, N, num_kb, c, z, sms);
-        if (us < best) best = us, best_c = c, best_z = z;
+        if (us < best_us) best_us = us, best = {kRows, few_rows_height(M, z), c};
       }
   }
-  if (M <= 16 && K <= few_longest(M) && few_us(M, N, K, sms) < best) return launch_few(out, ldo, x, ldx, w, ldw, scales, M, N, K, s);
-  return best_c ? launch_rows(out, ldo, x, ldx, w, ldw, scales, M, N, K, best_c, best_z, s) : launch_pair(out, ldo, x, ldx, w, ldw, scales, M, N, K, best_bn, s);
+  if (M <= 16 && K <= few_longest(M) && few_us(M, N, K, sms) < best_us) best = {kFew, 16, 1};
+  return best;
+}
+
+template <typename TOut>
+int launch(TOut* out, long long ldo, const void* x, long long ldx, const void* w, long long ldw, const Scales& scales, int M, int N, int K,
+           cudaStream_t s) {
+  const Choice by = choose(M, N, K, sizeof(TOut) == 4, rows_on_borders(out, ldo, N));
+  if (by.kernel == kFew) return launch_few(out, ldo, x, ldx, w, ldw, scales, M, N, K, s);
+  if (by.kernel == kRows) return launch_rows(out, ldo, x, ldx, w, ldw, scales, M, N, K, by.c, by.bn, s);
+  return launch_pair(out, ldo, x, ldx, w, ldw, scales, M, N, K, by.bn, s);
 }
 
 }  // namespace
@@ -959,5 +998,19 @@ OI_API int oi_linear_int8_status(int* status) {
 // For tests: products launched from now on take the wait of this code as having run out (0: none).
 OI_API int oi_linear_int8_run_out(int code) {
   g_runs_out = code;
+  return OI_OK;
+}
+
+// For tests: which kernel takes a product of these sizes (0: up to 16 rows, 1: few, 2: many), rows of x a tile, slices of K, tiles,
+// stages, and of few rows whether partial sums go over the ring. on_borders: result rows start and end on 16-byte borders.
+OI_API int oi_linear_int8_choice(int out_dtype, int on_borders, int M, int N, int K, int* choice) {
+  OI_REQUIRE(M >= 1 && N >= 1 && K >= 1 && K <= 131071, "linear_int8_choice: bad sizes M=%d N=%d K=%d", M, N, K);
+  const Choice by = choose(M, N, K, out_dtype == OI_F32, on_borders != 0);
+  int smem = 0;
+  const Shape g = by.kernel == kRows ? few_rows_shape(M, N, K, by.c, by.bn, smem) : Shape{};
+  choice[0] = by.kernel, choice[1] = by.bn, choice[2] = by.c;
+  choice[3] = ceil_div(M, by.bn) * ceil_div(N, by.kernel == kFew ? 16 : by.kernel == kRows ? BM : 256);
+  choice[4] = by.kernel == kRows ? g.stages : by.kernel == kPairs ? pair_stages(by.bn) : few_stages(N, K);
+  choice[5] = by.kernel == kRows && by.c > 1 && g.recv_offset == 0;
   return OI_OK;
 }

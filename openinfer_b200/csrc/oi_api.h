@@ -325,6 +325,7 @@ OI_API int oi_linear_int8(void* out, int out_dtype, long long ldo, const void* x
                           long long ldw, const float* sw, const float* bias, int M, int N, int K, void* stream);
 OI_API int oi_linear_int8_status(int* status);
 OI_API int oi_linear_int8_run_out(int code);      // for tests
+OI_API int oi_linear_int8_choice(int out_dtype, int on_borders, int M, int N, int K, int* choice);
 
 // gemm_tcgen05.cu
 OI_API int oi_gemm_tcgen05(void* C, int c_dtype, long long ldc, const void* A, long long lda, const void* W, long long

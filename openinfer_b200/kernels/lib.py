@@ -102,6 +102,7 @@ _SIGNATURES = {
     "oi_linear_int8": [P, I, L, P, L, P, P, L, P, P, I, I, I, P],
     "oi_linear_int8_status": [ctypes.POINTER(c_int)],
     "oi_linear_int8_run_out": [I],
+    "oi_linear_int8_choice": [I, I, I, I, I, ctypes.POINTER(c_int)],
     "oi_gemm_tcgen05_glu": [P, L, P, L, P, L, I, I, I, I, I, F, P],
 }
 

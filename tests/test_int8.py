@@ -231,3 +231,19 @@ def test_a_weight_given_tensors_of_inference_mode_or_other_ones(first, second):
         w.values.fill_(3)
     w.operands()
     assert w.stream == (7 if second else None)
+
+
+def choice(dtype, on_borders, rows, channels, width):
+    """(kernel, rows of x a tile, slices of the sum, tiles, stages, partial sums over the ring) of a product"""
+    L, said = klib.load(verbose=False), (ctypes.c_int * 6)()
+    assert L.oi_linear_int8_choice(int8._DT[dtype], on_borders, rows, channels, width, said) == 0
+    return tuple(said)
+
+
+def test_no_tile_of_a_product_lies_behind_the_last_row():
+    """Tiles are a multiple of sixteen rows high: as many as were asked for of that height may be more than there are rows for."""
+    for rows in [*range(1, 1200), *range(1200, 4097, 13)]:
+        for channels, width in ((128, 16384), (4096, 4096), (1000, 7000), (300, 1000)):
+            kernel, tile, slices, tiles, stages, over = choice(torch.bfloat16, True, rows, channels, width)
+            along = tiles // -(-channels // (16, 128, 256)[kernel])
+            assert (along - 1) * tile < rows <= along * tile and stages >= 1
