@@ -295,6 +295,7 @@ SHAPES = [(1, 1, 1), (1, 128, 128), (1, 5, 16), (2, 33, 31), (3, 130, 129), (8, 
           (256, 512, 512), (257, 2049, 333), (300, 6144, 256), (512, 513, 1025), (777, 1000, 2001), (1024, 2048, 640), (2050, 300, 4100), (5000, 130, 72), (1, 9000, 14000), (4, 64, 60000)]
 # Every kernel, width of its tiles, number of slices, of warps that read results, and place of the partial sums; result rows on 16-byte
 # borders, on four-byte borders, and on none; more tiles than pairs of CTAs.
+# (By the rule that chose when they were drawn. By the rule as it is, sizes for all of this are in test_int8_tiles.py, which asks it.)
 TILES = [(370, 2972, 7657), (574, 7354, 3863), (309, 8746, 3887), (629, 8798, 2673), (1532, 671, 7446), (1367, 3287, 3872), (442, 5427, 4611),
           (1789, 2761, 2951), (464, 4400, 7640), (1599, 1672, 2630), (1784, 3048, 757), (763, 4112, 1824), (2003, 5096, 186), (624, 5560, 2014),
           (1570, 9128, 55), (2496, 1736, 1546), (1845, 6736, 139), (616, 2552, 8097), (67, 10187, 33), (194, 9522, 546), (140, 15241, 130),
