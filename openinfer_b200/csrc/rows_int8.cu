@@ -616,10 +616,15 @@ int launch_dequantize(T* out, long long ldo, const signed char* q, long long ldq
   const int each = two ? 32 : 16;
   int lanes_log = 0;
   while (lanes_log < 8 && each << lanes_log < cols) ++lanes_log;
-  const dim3 grid(ceil_div(rows, 256 >> lanes_log), ceil_div(cols, each << lanes_log));
-  OI_REQUIRE(grid.y <= 65535, "dequantize_int8: bad sizes rows=%d cols=%d", rows, cols);
   const bool wide = lanes_log == 8;
-  auto go = [&](auto kernel) { oi_launch(kernel, grid, 256, 0, s, out, ldo, q, ldq, scales, rows, cols, lanes_log); };
+  constexpr int kMostColumns = 1 << 27;          // of a launch: a grid has 65,535 blocks along a row at most
+  auto go = [&](auto kernel) {
+    for (int c0 = 0; c0 < cols; c0 += kMostColumns) {
+      const int n = cols - c0 < kMostColumns ? cols - c0 : kMostColumns;
+      const dim3 grid(ceil_div(rows, 256 >> lanes_log), ceil_div(n, each << lanes_log));
+      oi_launch(kernel, grid, 256, 0, s, out + c0, ldo, q + c0, ldq, scales, rows, n, lanes_log);
+    }
+  };
   if (two) wide ? go(dequantize_kernel<T, true, true, 2>) : go(dequantize_kernel<T, true, false, 2>);
   else if (vec) wide ? go(dequantize_kernel<T, true, true, 1>) : go(dequantize_kernel<T, true, false, 1>);
   else wide ? go(dequantize_kernel<T, false, true, 1>) : go(dequantize_kernel<T, false, false, 1>);

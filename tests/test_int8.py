@@ -247,3 +247,13 @@ def test_no_tile_of_a_product_lies_behind_the_last_row():
             kernel, tile, slices, tiles, stages, over = choice(torch.bfloat16, True, rows, channels, width)
             along = tiles // -(-channels // (16, 128, 256)[kernel])
             assert (along - 1) * tile < rows <= along * tile and stages >= 1
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: the launches have to fail")
+@pytest.mark.parametrize("rows,width", [(1, 1 << 30), (1, (1 << 28) + 5), (3, 1 << 30), (1 << 30, 1)])
+def test_rows_of_every_length_that_are_made_are_brought_back(rows, width):
+    """The launch is come to (and fails): no size that ``quantize_int8`` takes is refused."""
+    L = klib.load(verbose=False)
+    assert L.oi_quantize_int8(16, width, 16, 16, 1, width, rows, width, 1, None) > 1
+    for code in (0, 1):
+        assert L.oi_dequantize_int8(16, code, width, 16, width, 16, rows, width, None) > 1

@@ -711,3 +711,19 @@ def test_a_wait_that_runs_out_makes_results_that_are_no_numbers(int8, dtype, row
     assert bool(none.any()) and (not all_of_it or bool(none.all()))
     assert torch.equal(got[~none], want[~none]) and bool((out[:, channels:] == -7.0).all())
     assert torch.equal(int8.linear_int8(held, weight, out_dtype=dtype).cpu(), want) and int8.status() == 0
+
+
+@pytest.mark.parametrize("rows,width,off", [(1, (1 << 28) + 21, 0), (1, (1 << 28) + 21, 1), (2, 3 << 27, 0)])
+def test_rows_that_one_launch_does_not_bring_back(int8, rows, width, off):
+    """More than 2^27 numbers a row, on 16-byte borders and off."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    held = int8.empty_rows(rows, width, DEV)
+    held.values.copy_(torch.randint(-127, 128, (rows, width), generator=g, dtype=torch.int8, device=DEV))
+    held.scales.copy_(torch.rand(rows, generator=g, device=DEV) + 0.1)
+    room = torch.full((rows, width + 8), -7.0, dtype=torch.bfloat16, device=DEV)
+    out = room[:, off:off + width]
+    int8.dequantize_int8(held, out=out)
+    assert bool((room[:, off + width:] == -7.0).all()) and bool((room[:, :off] == -7.0).all())
+    for first in range(0, width, 1 << 26):
+        part = slice(first, first + (1 << 26))
+        assert torch.equal(out[:, part], (held.values[:, part].float() * held.scales[:, None]).bfloat16())
