@@ -152,7 +152,7 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, delta: Op
             raise KernelError(f"rmsnorm_int8: rows that overlap (row stride {stride}, width {width}) cannot take a sum")
         size = 2 if code else 4
         if (d_address < address + ((rows - 1) * stride + width) * size and address < d_address + ((rows - 1) * d_stride + width) * size
-                and rows and (d_address, d_stride) != (address, stride)
+                and rows and (d_address, d_stride if rows > 1 else stride) != (address, stride)      # one row's stride means nothing
                 and not (d_stride == stride > 0 and width <= (d_address - address) // size % stride <= stride - width)):    # rows in turn
             raise KernelError("rmsnorm_int8: x and delta must be the same rows or not overlap")
     if _elsewhere(device):

@@ -257,3 +257,12 @@ def test_rows_of_every_length_that_are_made_are_brought_back(rows, width):
     assert L.oi_quantize_int8(16, width, 16, 16, 1, width, rows, width, 1, None) > 1
     for code in (0, 1):
         assert L.oi_dequantize_int8(16, code, width, 16, width, 16, rows, width, None) > 1
+
+
+def test_one_row_is_itself_whatever_its_stride():
+    wide = torch.zeros(4, 64)
+    x = wide[2:3, :32]
+    same = x.as_strided((1, 32), (32, 1))
+    for a, b in ((x, same), (same, x)):
+        refused("not on a CUDA device", lambda: int8.rmsnorm_int8(a, torch.ones(32), 1e-6, delta=b))
+    refused("not overlap", lambda: int8.rmsnorm_int8(x, torch.ones(32), 1e-6, delta=wide[2:3, 16:48]))
