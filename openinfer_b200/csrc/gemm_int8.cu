@@ -59,8 +59,8 @@ struct Scales {
 // w x bn] lies in tensor memory. Grid (c, tiles of x, tiles of w; those that share a tile of w run together): a cluster of c CTAs (a
 // power of two) shares one tile, CTA r streaming k blocks [r * kb_per_rank, ...) of it. Columns of the accumulator (rows of x) belong to the CTAs by fours in turn: each
 // deposits what it has of the others' columns in their shared memory, 16 bytes a channel, and adds to its own, which stay in tensor
-// memory, what the others left there. (All of a channel's columns to one CTA, its own part through shared memory too, us: 264 x 4096 x 12288
-// 19.2 for 18.3, 400 x 2048 x 8192 14.5 for 12.5, 256 x 512 x 16384 10.2 for 9.2, 24 x 1024 x 1024 3.7 for 3.55.)
+// memory, what the others left there. (All of a channel's columns to one CTA, its own part through shared memory too, us, weights from L2: 264 x
+// 4096 x 12288 19.2 for 18.3, 400 x 2048 x 8192 14.5 for 12.5, 256 x 512 x 16384 10.2 for 9.2, 24 x 1024 x 1024 3.7 for 3.55.)
 //   warp 0     one thread issues the copies; the first ring-full of WEIGHT boxes is requested before the wait for the kernel
 //              ahead (programmatic dependent launch), which may still be writing x
 //   warp 1     allocates tensor memory (behind that wait: a kernel ahead that needs all of it may not have taken its own
@@ -69,8 +69,9 @@ struct Scales {
 // What the results cost shows in the instructions per column: with a column at a time, a branch and a cluster address each, and
 // six warps, 128 columns took 8,000 cycles to deposit and 8,700 to store (N 1024, K 1024, c 1); stored two channels a lane, by lanes that
 // trade halves, 4.6 us instead of 4.3 (500 x 4095 x 512).
-// Measured (us; what its bytes at the copy rate and its operations at twice the bfloat16 rate take): 32 x 24576 x 4096 19.6 (15.6),
-// 64 x 6144 x 4096 8.8 (4.0), 512 x 4096 x 4096 10.5 (5.2), 264 x 4096 x 12288 18.4 (8.5), a head of 151936 x 4096 with 64 rows 102 (98).
+// Measured (us, weights in turn, so from memory; in brackets what its bytes at the copy rate or its operations at twice the bfloat16 rate
+// take): 32 x 24576 x 4096 18.5 (15.7), 64 x 6144 x 4096 8.8 (4.0), 512 x 4096 x 4096 10.6 (5.2), 264 x 4096 x 12288 18.4 (8.5; from L2 17.4),
+// 777 x 5003 x 2001 into float32 11.8 (4.7).
 // Bound by what one SM takes in (some 110 GB/s, 32 KB a stage of 128 rows) and, short sums, by launch, x, results.
 constexpr int kFewColumns = 32, kMoreColumns = 64;      // up to so many rows of x a tile four warps read results, or eight, else sixteen
 
@@ -310,8 +311,9 @@ linear_int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 //               CTA's "drained" barrier. A warp scales 32 channels of a few rows, turns them in shared memory, and a TMA store carries
 //               them out: 4096 x 4096 x 512 takes 18.5 us so (float32 21; 16.5 with channels across the tile, whose rows need
 //               no turning, but then tiles are 256 rows high), with 16-byte stores by the warps 3 and 8 more.
-// Measured (us; at twice the bfloat16 rate): 8192 x 24576 x 4096 496 (502; 3.33 POP/s, the library's bfloat16 product 1017), 2048 x 4096 x 4096
-// 26 (21), 777 x 24576 x 4096 63 (48; tiles of 256 rows 71), 264 x 24576 x 4096 31 (17.5; 36). Bound by the tensor cores and their power
+// Measured (us, by the clock that power leaves; at twice the bfloat16 rate): 8192 x 24576 x 4096 480 to 590 (502; 3.4 POP/s at best, the
+// library's bfloat16 product 1017), 2048 x 4096 x 4096 26 to 29 (21), 777 x 24576 x 4096 62 (48; tiles of 256 rows 71), 264 x 24576 x 4096 31 to 34
+// (17.5; 36), a head of 151936 x 4096 with 64 rows 102 (98). Bound by the tensor cores and their power
 // where tiles fill the pairs evenly, else by the last round of them; with K of 512 by the results.
 constexpr int kEpilogueWarps = 16;
 constexpr int kParts = kEpilogueWarps / 4;                          // the warps of a quarter of the lanes share the rows of x
@@ -782,8 +784,9 @@ Shape few_rows_shape(int M, int N, int K, int c, int bn, int& smem) {
   const int stage = kBoxBytes + g.bn * BK, recv = ceil_div(g.bn / 4, c) * (c - 1) * BM * 16;
   // two CTAs on an SM, where there are more than SMs: one streams while the other ends, the next kernel's included
   const int budget = (long long)c * z * ceil_div(N, BM) <= (c == 8 ? 96 : oi_sm_count()) || g.bn > 128 ? kSmemOfOne : kSmemOfTwo;
-  // deposits beside the ring, or over it when it is drained (a cluster's barrier more) where a ring beside them would be short (264 rows, N
-  // 4096, K 12288, c 2: three stages beside them 23.4 us, six under them 19.7)
+  // deposits beside the ring, or over it when it is drained (a cluster's barrier more) where a ring beside them would have fewer than five
+  // stages and a CTA has more (us, beside and over: 100 x 18984 x 17386, two stages and three, 97.1 and 81.0; 65 x 19024 x 20234, three and
+  // four, 92.5 and 86.3; 264 x 4096 x 12288, five and six, 18.6 and 18.6; 128 x 4096 x 8192, seven and eight, 12.0 and 12.8)
   const bool own_room = recv <= budget - 256 - g.bn * 4 - (g.kb_per_rank < 5 ? g.kb_per_rank : 5) * stage;
   g.stages = (budget - 256 - g.bn * 4 - (own_room ? recv : 0)) / stage;
   if (g.stages > kMostStages) g.stages = kMostStages;

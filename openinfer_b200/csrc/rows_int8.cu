@@ -15,8 +15,9 @@ __device__ int g_rows_int8_error = 0;       // set to a non-zero code when a bou
 // |y| as bits: ordered like the numbers, infinities above all finite ones and NaNs above those
 __device__ __forceinline__ unsigned magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
 
-// act(gate) * up by the special-function unit's exponential and reciprocal (2 ulp each): what follows is a rounding to 8 bits. A gate far
-// below zero is an infinite exponential and a zero.
+// act(gate) * up by the special-function unit's exponential and reciprocal: what follows is a rounding to 8 bits. They are within 2 units
+// in the last place each, but the exponent is rounded before them: e^-t is off by up to |t| roundings more (some 30 units at 60). Where it
+// passes 2^126 (t below -87.3) its reciprocal is below the normal numbers, and the result a zero.
 template <int ACT>
 __device__ __forceinline__ float gated(float g, float u) {
   const float t = ACT == OI_ACT_GELU_TANH ? 1.5957691216057308f * (g + 0.044715f * g * g * g) : g;
@@ -224,13 +225,15 @@ struct GateRow {
 // a block. kVec: 16 bytes a load, eight neighbours a thread; else neighbours lie in neighbouring threads and the bytes are put
 // together in shared memory. One exchange between the warps, of the largest magnitude and a norm's sum of squares at once; so a norm's
 // integers are made of x * w alone, and its reciprocal root mean square goes into the scale. How a norm's row is shared out goes by
-// its length alone, so that its result does not depend on how many there are. early: the next kernel may be scheduled while this one
-// runs (not where the rows may be those of a weight: a product fetches its weight before it waits).
+// its length, and by whether its operands and the rows behind them start on 16-byte borders, so that its result does not depend on how many
+// there are. early: the next kernel may be scheduled while this one runs (not where the rows may be those of a weight: a product fetches
+// its weight before it waits).
 //
 // Bound by memory, or at few rows by the chain load, exchange, store; beside memory by instructions (issue slots 64 to 69 % busy at
 // 16384 x 4096). Measured (bytes read and written, each once): norm with residual of 8192 x 4096 39.6 us (5.9 TB/s; read once for each thing
-// asked of the row 150), 4096 x 8192 42 (5.6), 65536 x 128 9.9, one row of 4,096 2.1; gate of 4096 x 12288 47 (5.3; four units a thread in 384
-// threads 60, two in 768 so), plain rows of 8192 x 4096 19.4 (5.2), 6144 x 4097 in float32 off every border 33 (3.8).
+// asked of the row 150), 4096 x 8192 42 (5.6), 65536 x 128 9.9, one row of 4,096 1.8; gate of 4096 x 12288 46.5 (5.4; four units a thread in 384
+// threads 60, two in 768 so; wider ones than 768 threads hold by two have four: 12,296 65, 14,336 66, 16,384 71), plain rows of 8192 x 4096
+// 19.4 (5.2), 6144 x 4097 in float32 off every border 33 (3.8), 333 x 5001 so 5.8: four bytes a load there.
 template <typename Row, bool kVec, int UNITS, int LANES>
 __global__ void __launch_bounds__(LANES || UNITS == 1 ? 256 : UNITS == 2 ? 768 : 512)
 rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows, int cols, int early) {
@@ -360,7 +363,10 @@ rows_int8_kernel(Row row, signed char* q, long long ldq, float* scales, int rows
 // row is shared out as above, so its bits are the same. Measured (us, above -> this; bfloat16 norm with residual, without, plain rows):
 //   4096 x 8704   58.0 -> 49.3, 47.3 -> 44.1, 28.4 -> 23.3        1200 x 12288, from L2   21.9 -> 18.1, 19.3 -> 16.3, 9.0 -> 9.4
 //   4096 x 12288  97.2 -> 57.0 (6.2 TB/s), 83.6 -> 46.1, 34.7 -> 28.7        300 x 12288, from L2   7.5 -> 8.1, 7.1 -> 7.5, 3.8 -> 4.5
-//   4096 x 16384  110 -> 87, 93 -> 54, 46.6 -> 35.6
+//   4096 x 16384  110 -> 86, 93 -> 53, 46.6 -> 35.6
+// Without a residual that is 1.7 to 2.7 times the bytes' time (16.3, 23.1, 30.8). Shared memory is given out for two blocks an SM, but of a
+// norm, with 97 registers a thread, one fits (of plain rows, with 57, two): the second half of the blocks runs behind the first, 14 % of an
+// SM's warps are there, and the exchange of a row is overlapped by nothing.
 // Gates and rows of up to 8,192 are faster above, and so are float32's plain rows (4096 x 12288 38 -> 43). Bound by memory; with a ring of
 // two or three rows for one block (16384 with residual) by the wait for the next.
 constexpr int kRingMost = 8, kRingUnits = 4, kRingBytes = 208 * 1024;
@@ -559,7 +565,9 @@ bool on_borders(const void* p, long long ld, int esize) { return (uintptr_t)p % 
 
 // Sixteen numbers a thread: neighbours where rows start on 16-byte borders, else one of each 1 << lanes_log; 256 >> lanes_log rows a
 // block (65536 x 128 with a block a row 69 us, 5.9 so). Bound by memory: many long rows give a thread both its loads (kTimes 2) before
-// it stores (8192 x 4096 16.2 us, 6.2 TB/s, for 18.9 with one; 8 x 4096 1.5 for 1.3 and 8192 x 640 4.8 for 3.8, so one there).
+// it stores (the same buffers each time, some of them in L2: 8192 x 4096 16.2 us for 18.9 with one; 8 x 4096 1.5 for 1.3 and 8192 x 640 4.8
+// for 3.8, so one there). From memory 8192 x 4096 takes 19.1 us (5.3 TB/s), 4096 x 12288 30.1; 6144 x 4097 into rows off every border 21, one
+// byte a load and two a store.
 // A byte becomes a number without a conversion: with its sign turned it is the last byte of 2^23 + 128 + q.
 template <typename T, bool kVec, bool kWide, int kTimes>
 __global__ void __launch_bounds__(256) dequantize_kernel(T* out, long long ldo, const signed char* q, long long ldq, const float* scales, int rows,

@@ -136,7 +136,8 @@ def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
 
 def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, delta: Optional[torch.Tensor] = None,
                  weight_offset: float = 0.0, out: Optional[Int8Rows] = None) -> Int8Rows:
-    """x * rsqrt(mean(x^2) + eps) * (weight_offset + weight), row by row, as 8-bit integers.
+    """x * rsqrt(mean(x^2) + eps) * (weight_offset + weight), row by row, as 8-bit integers. A row's integers are made of x * (weight_offset
+    + weight), its root mean square goes into the scale: a number within float32's rounding of a half may become either neighbour.
 
     ``delta``: x <- x + delta first (rounded, stored in x), the norm is of the sum as it is stored."""
     code, rows, width, stride = _float_rows(x, "rmsnorm_int8")
