@@ -8,6 +8,8 @@
 // bounded: one that runs out sets an error word and a flag that ends all roles of the CTA, which writes NaN for the results that it did
 // not come to (of a cluster that adds up sums, all its CTAs do), still joins its cluster's barriers, frees its tensor memory and
 // returns. No load uses cluster multicast.
+#include <limits.h>
+
 #include <atomic>
 
 #include "oi_api.h"
@@ -1012,7 +1014,8 @@ OI_API int oi_linear_int8_choice(int out_dtype, int on_borders, int M, int N, in
   int smem = 0;
   const Shape g = by.kernel == kRows ? few_rows_shape(M, N, K, by.c, by.bn, smem) : Shape{};
   choice[0] = by.kernel, choice[1] = by.bn, choice[2] = by.c;
-  choice[3] = ceil_div(M, by.bn) * ceil_div(N, by.kernel == kFew ? 16 : by.kernel == kRows ? BM : 256);
+  const long long tiles = (long long)ceil_div(M, by.bn) * ceil_div(N, by.kernel == kFew ? 16 : by.kernel == kRows ? BM : 256);
+  choice[3] = tiles < INT_MAX ? (int)tiles : INT_MAX;
   choice[4] = by.kernel == kRows ? g.stages : by.kernel == kPairs ? pair_stages(by.bn) : few_stages(N, K);
   choice[5] = by.kernel == kRows && by.c > 1 && g.recv_offset == 0;
   return OI_OK;

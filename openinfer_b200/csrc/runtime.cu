@@ -62,12 +62,14 @@ int oi_take_launch_fence(cudaStream_t stream) {
   int v = g_fence_next;
   g_fence_next = 0;
   if (g_fenced_streams.load(std::memory_order_acquire) != 0) {
-    const auto it = on_its_device(stream);
     std::lock_guard<std::mutex> hold(g_streams_lock);
-    const auto at = std::find(g_streams.begin(), g_streams.end(), it);
-    if (at != g_streams.end()) {
-      g_streams.erase(at);
-      v = 1;
+    // the device is asked for where the handle is the same: a stream that nothing is launched on again costs others a look at the list
+    if (std::any_of(g_streams.begin(), g_streams.end(), [&](const auto& s) { return s.second == stream; })) {
+      const auto at = std::find(g_streams.begin(), g_streams.end(), on_its_device(stream));
+      if (at != g_streams.end()) {
+        g_streams.erase(at);
+        v = 1;
+      }
     }
     g_fenced_streams.store((int)g_streams.size(), std::memory_order_release);
   }

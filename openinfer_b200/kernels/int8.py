@@ -324,7 +324,7 @@ def linear_int8(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = 
 
 
 def status() -> int:
-    """0, or which bounded wait of a product ran out since the last call (synchronises the device)."""
+    """0, or which bounded wait of a product ran out since the last call: what it would have made is NaN (synchronises the device)."""
     from ctypes import byref, c_int
     v = c_int(0)
     _lib.check(_lib.load().oi_linear_int8_status(byref(v)), "linear_int8_status")
